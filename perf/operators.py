@@ -576,7 +576,7 @@ def _route_grad_exact(c, d):
     seen = torch.zeros_like(x).scatter_(1, idx.clamp(min=0), 1.0) * alive
     given = torch.zeros_like(x).scatter_(1, idx.clamp(min=0), d["dweights"]) * alive
     if c["renorm"]:
-        total = (p * seen).sum(1, keepdim=True).clamp(min=1e-300)
+        total = torch.where(alive, (p * seen).sum(1, keepdim=True), torch.ones_like(p[:, :1]))
         given = seen * (given / total - (given * p).sum(1, keepdim=True) / total**2)
     dp = given + d["dloss"] * c["experts"] / (n * n * idx.shape[1]) * d["counts"]
     return {"dlogits": p * dp - p * (p * dp).sum(1, keepdim=True)}
