@@ -23,6 +23,8 @@ EXPORTS = [
     "ascb200_event_destroy", "ascb200_event_record", "ascb200_stream_wait_event", "ascb200_event_elapsed_ms", "ascb200_gemm", "ascb200_grouped_gemm",
     "ascb200_gemm_mxfp4_noalloc", "ascb200_noalloc_status", "ascb200_mx_scale_prepacked_bytes", "ascb200_mx_scale_prepack", "ascb200_fp4_transpose", "ascb200_shard_nslab", "ascb200_shard_groups_lpt", "ascb200_comm_unique_id", "ascb200_comm_init", "ascb200_comm_init_all", "ascb200_comm_destroy", "ascb200_group_start", "ascb200_group_end", "ascb200_allgather_slabs", "ascb200_interleave_slabs", "ascb200_graph_begin", "ascb200_graph_end", "ascb200_graph_launch", "ascb200_graph_destroy",
     "ascb200_nz_unpack", "ascb200_quant_policy", "ascb200_quant_policy_rm", "ascb200_dequant_policy", "ascb200_softmax_flash_v2", "ascb200_softmax", "ascb200_log_softmax", "ascb200_antiquant", "ascb200_softmax_flash", "ascb200_softmax_grad", "ascb200_simple_softmax", "ascb200_quant_per_tensor", "ascb200_quant_per_channel", "ascb200_softmax_quant", "ascb200_dequant",
+    "ascb200_rms_norm", "ascb200_rms_norm_grad", "ascb200_rms_norm_grad_workspace_bytes", "ascb200_route", "ascb200_route_workspace_bytes",
+    "ascb200_route_grad",
 ]
 
 
@@ -37,6 +39,42 @@ class GemmDesc(C.Structure):
         ("epilogue", C.c_int32), ("quant_dev", C.c_void_p), ("quant_scalar", C.c_uint64),
         ("tok_scale_dev", C.c_void_p), ("ch_scale_dev", C.c_void_p),
         ("relu", C.c_int32), ("act", C.c_int32), ("atomic", C.c_int32), ("scale_flags", C.c_int32), ("c_layout", C.c_int32), ("reserved", C.c_int32 * 1),
+    ]
+
+
+class RmsNormDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32), ("gamma_dtype", C.c_int32),
+        ("x_dev", C.c_void_p), ("ldx", C.c_int64), ("residual_dev", C.c_void_p), ("ld_residual", C.c_int64), ("gamma_dev", C.c_void_p),
+        ("sum_dev", C.c_void_p), ("ld_sum", C.c_int64), ("y_dev", C.c_void_p), ("ldy", C.c_int64), ("q_dev", C.c_void_p), ("ldq", C.c_int64),
+        ("scale_dev", C.c_void_p), ("rstd_dev", C.c_void_p), ("eps", C.c_float), ("q_dtype", C.c_int32), ("scale_mode", C.c_int32),
+        ("group_size", C.c_int32), ("reserved", C.c_int32 * 2),
+    ]
+
+
+class RmsNormGradDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32), ("gamma_dtype", C.c_int32),
+        ("dy_dev", C.c_void_p), ("ld_dy", C.c_int64), ("h_dev", C.c_void_p), ("ldh", C.c_int64), ("rstd_dev", C.c_void_p), ("gamma_dev", C.c_void_p),
+        ("dh_dev", C.c_void_p), ("ld_dh", C.c_int64), ("dx_dev", C.c_void_p), ("ld_dx", C.c_int64), ("dgamma_dev", C.c_void_p),
+        ("dgamma_dtype", C.c_int32), ("reserved", C.c_int32), ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class RouteDesc(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int32), ("experts", C.c_int32), ("top_k", C.c_int32), ("dtype", C.c_int32), ("logits_dev", C.c_void_p), ("ld_logits", C.c_int64),
+        ("valid_dev", C.c_void_p), ("idx_dev", C.c_void_p), ("weights_dev", C.c_void_p), ("counts_dev", C.c_void_p), ("num_tokens_dev", C.c_void_p),
+        ("prob_mean_dev", C.c_void_p), ("loss_dev", C.c_void_p), ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("renorm", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class RouteGradDesc(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int32), ("experts", C.c_int32), ("top_k", C.c_int32), ("dtype", C.c_int32), ("logits_dev", C.c_void_p), ("ld_logits", C.c_int64),
+        ("idx_dev", C.c_void_p), ("counts_dev", C.c_void_p), ("num_tokens_dev", C.c_void_p), ("dloss_dev", C.c_void_p), ("dweights_dev", C.c_void_p),
+        ("dlogits_dev", C.c_void_p), ("ld_dlogits", C.c_int64), ("renorm", C.c_int32), ("reserved", C.c_int32),
     ]
 
 
@@ -126,6 +164,14 @@ def lib():
                                                C.c_float, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]
         _lib.ascb200_dequant.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                          C.c_int32, C.c_float, C.c_void_p]
+        _lib.ascb200_rms_norm.argtypes = [C.POINTER(RmsNormDesc), C.c_void_p]
+        _lib.ascb200_rms_norm_grad.argtypes = [C.POINTER(RmsNormGradDesc), C.c_void_p]
+        _lib.ascb200_rms_norm_grad_workspace_bytes.argtypes = [C.c_int32, C.c_int32]
+        _lib.ascb200_rms_norm_grad_workspace_bytes.restype = C.c_size_t
+        _lib.ascb200_route.argtypes = [C.POINTER(RouteDesc), C.c_void_p]
+        _lib.ascb200_route_workspace_bytes.argtypes = [C.c_int32, C.c_int32]
+        _lib.ascb200_route_workspace_bytes.restype = C.c_size_t
+        _lib.ascb200_route_grad.argtypes = [C.POINTER(RouteGradDesc), C.c_void_p]
     return _lib
 
 
@@ -318,6 +364,35 @@ def dequant_policy(src, dst, m, n, src_dtype, scale_dtype, dst_dtype, policy, sc
 def dequant(src, dst, m, n, cal, n_dst, dst_dtype, scale=None, scale_dtype=F32, scale_scalar=0.0, stream=None):
     return lib().ascb200_dequant(_ptr(src), _ptr(dst), m, n, cal, n_dst, dst_dtype, _ptr(scale), scale_dtype, C.c_float(scale_scalar),
                                  stream)
+
+
+# The operators of a feed-forward block take a descriptor (RmsNormDesc, ...) whose *_dev fields hold device addresses (`DevBuf.ptr`);
+# a caller keeps it for its buffers and gives it to every call.
+SCALE_PER_TOKEN, SCALE_PER_GROUP, SCALE_MX = 0, 1, 2
+
+
+def rms_norm(desc, stream=None):
+    return lib().ascb200_rms_norm(desc, stream)
+
+
+def rms_norm_grad_workspace_bytes(m, k):
+    return lib().ascb200_rms_norm_grad_workspace_bytes(m, k)
+
+
+def rms_norm_grad(desc, stream=None):
+    return lib().ascb200_rms_norm_grad(desc, stream)
+
+
+def route_workspace_bytes(tokens, experts):
+    return lib().ascb200_route_workspace_bytes(tokens, experts)
+
+
+def route(desc, stream=None):
+    return lib().ascb200_route(desc, stream)
+
+
+def route_grad(desc, stream=None):
+    return lib().ascb200_route_grad(desc, stream)
 
 
 class Graph:

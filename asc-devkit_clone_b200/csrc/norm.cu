@@ -1,0 +1,685 @@
+// Root-mean-square norm with the residual's addition and an 8-bit output with scales, and its gradients.
+//
+//   h = x + residual,   rstd = 1 / sqrt(mean(h^2) + eps),   y = (h * gamma) * rstd
+//   q, scale: y in 8 bits with one scale per row, per group of columns, or e8m0 scales per 32 columns (MX)
+//
+// Memory bound: a row is read once, kept in registers in fp32, and every output is written once.  h is stored before the
+// reduction (it does not depend on it), so what stays in registers is h * gamma alone, and because
+// max|y| = max|h * gamma| * rstd the sum of squares and the largest magnitude of a row come out of one reduction.
+//
+// gradients, with hat = h * rstd and g = dy * gamma:   dx = rstd * (g - hat * mean(g * hat)) + dh,   dgamma = sum over rows of dy * hat
+// One pass as well: a block walks rows and owns the same columns in each, so dgamma is summed in its registers; the blocks'
+// partial sums go through the caller's workspace and are added in block order (no atomics: the result does not depend on timing).
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace ascb200 {
+namespace {
+
+// ---- rows in chunks of eight elements ------------------------------------------------------------------------------------
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<__half> {
+    uint4 v;
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+    uint4 v;
+};
+template <>
+struct Raw8<float> {
+    uint4 v, w;
+};
+
+// (not the read-only path: an output may be the row's own input)
+__device__ __forceinline__ uint4 ld_v4(const void* p)
+{
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+
+// Chunk c (elements 8 c .. 8 c + 7) of a row of k elements; elements past the row's end read as zero and are not touched.
+// VEC: rows start on 16 bytes.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_chunk(const T* row, int c, int k, Raw8<T>& r)
+{
+    if (VEC && c * 8 + 8 <= k) {
+        r.v = ld_v4(row + c * 8);
+        if constexpr (sizeof(T) == 4) r.w = ld_v4(row + c * 8 + 4);
+        return;
+    }
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        u[j] = 0u;
+        if (c * 8 + j < k) {
+            if constexpr (sizeof(T) == 4) u[j] = *reinterpret_cast<const uint32_t*>(row + c * 8 + j);
+            else u[j] = *reinterpret_cast<const uint16_t*>(row + c * 8 + j);
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+        r.v = make_uint4(u[0], u[1], u[2], u[3]);
+        r.w = make_uint4(u[4], u[5], u[6], u[7]);
+    } else {
+        r.v = make_uint4(u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16));
+    }
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&f)[8])
+{
+    f[0] = __uint_as_float(r.v.x), f[1] = __uint_as_float(r.v.y), f[2] = __uint_as_float(r.v.z), f[3] = __uint_as_float(r.v.w);
+    f[4] = __uint_as_float(r.w.x), f[5] = __uint_as_float(r.w.y), f[6] = __uint_as_float(r.w.z), f[7] = __uint_as_float(r.w.w);
+}
+__device__ __forceinline__ void unpack8(const Raw8<__half>& r, float (&f)[8])
+{
+    const __half2* h = reinterpret_cast<const __half2*>(&r.v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 v = __half22float2(h[j]);
+        f[2 * j] = v.x, f[2 * j + 1] = v.y;
+    }
+}
+__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& r, float (&f)[8])
+{
+    const uint32_t u[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[2 * j] = __uint_as_float(u[j] << 16), f[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+}
+// One rounding, to the output type; halves saturate at +-65504 like every fp16 output of the library, NaN is kept.
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half)
+{
+    uint32_t v;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
+    return v;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_chunk(T* row, int c, int k, const float (&f)[8])
+{
+    if constexpr (sizeof(T) == 4) {
+        if (VEC && c * 8 + 8 <= k) {
+            *reinterpret_cast<float4*>(row + c * 8) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(row + c * 8 + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c * 8 + j < k) row[c * 8 + j] = f[j];
+        }
+    } else {
+        const uint4 v = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
+        if (VEC && c * 8 + 8 <= k) {
+            *reinterpret_cast<uint4*>(row + c * 8) = v;
+        } else {
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c * 8 + j < k) reinterpret_cast<uint16_t*>(row)[c * 8 + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+        }
+    }
+}
+// gamma: NULL (ones), fp32, or the rows' type.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_gamma(const void* __restrict__ gamma, int gamma_f32, int c, int k, float (&g)[8])
+{
+    if (!gamma) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = 1.0f;
+    } else if (gamma_f32) {
+        if (VEC && c * 8 + 8 <= k) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(gamma) + 2 * c), b = __ldg(reinterpret_cast<const float4*>(gamma) + 2 * c + 1);
+            g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, g[4] = b.x, g[5] = b.y, g[6] = b.z, g[7] = b.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] = c * 8 + j < k ? __ldg(static_cast<const float*>(gamma) + c * 8 + j) : 0.0f;
+        }
+    } else {
+        if (VEC && sizeof(T) == 2 && c * 8 + 8 <= k) {
+            Raw8<T> r;
+            r.v = __ldg(reinterpret_cast<const uint4*>(gamma) + c);
+            unpack8(r, g);
+        } else {
+            Raw8<T> r;
+            load_chunk<T, false>(static_cast<const T*>(gamma), c, k, r);
+            unpack8(r, g);
+        }
+    }
+}
+
+__device__ __forceinline__ float max_nan(float a, float b)  // a NaN stays
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Sum and maximum over the TPR threads of a row; `red` holds one entry per warp and is not used again before the next barrier.
+template <int TPR>
+__device__ __forceinline__ void row_reduce(float& s, float& mx, float2* red)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    }
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+        if (l == 0) red[w] = make_float2(s, mx);
+        __syncthreads();
+        const float2 v = l < W ? red[l] : make_float2(0.0f, 0.0f);
+        s = v.x, mx = v.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            if (o >= W) continue;  // W is a power of two
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+        }
+        s = __shfl_sync(0xFFFFFFFFu, s, 0);
+        mx = __shfl_sync(0xFFFFFFFFu, mx, 0);
+    }
+}
+
+struct NormArgs {
+    const void* x;
+    const void* residual;
+    const void* gamma;
+    void* sum;
+    void* y;
+    void* q;
+    void* scale;
+    float* rstd;
+    long long ldx, ld_residual, ld_sum, ldy, ldq;
+    int m, k;
+    int gamma_f32;
+    int q_s8;         // 8-bit output: int8, else e4m3
+    int scale_mode;   // ASCB200_SCALE_*
+    int group_lanes;  // PER_GROUP / MX: lanes (of eight columns) per group, a power of two up to 32
+    float eps;
+};
+
+// Largest magnitude that a code stands for, in units of the scale.
+constexpr float kTopS8 = 127.0f, kTopE4M3 = 448.0f;
+
+// scale = amax / top and its reciprocal.  A scale under the smallest normal number counts as zero: its reciprocal would not
+// be finite, and codes times scale are then below 2^-117 anyway.  NaN stays NaN.
+__device__ __forceinline__ void scale_of(float amax, bool s8, float& scale, float& inv)
+{
+    const float s = s8 ? __fdiv_rn(amax, kTopS8) : __fdiv_rn(amax, kTopE4M3);
+    const bool none = s < 1.1754943508222875e-38f;
+    scale = none ? 0.0f : s;
+    inv = none ? 0.0f : __frcp_rn(s);
+}
+// MX: the shared exponent floor(log2 amax) - 8 (the exponent of the largest e4m3 power of two), biased by 127; 255 marks a block
+// that holds an infinity or a NaN.
+__device__ __forceinline__ uint32_t mx_scale_byte(float amax, float& inv)
+{
+    const uint32_t e = (__float_as_uint(amax) >> 23) & 0xFFu;
+    if (e == 255u) {
+        inv = __uint_as_float(0x7FC00000u);
+        return 255u;
+    }
+    const uint32_t byte = e > 8u ? e - 8u : 0u;
+    inv = __uint_as_float(byte == 0u ? 0x7F000000u : (254u - byte) << 23);  // 2^(127 - byte)
+    return byte;
+}
+
+__device__ __forceinline__ uint32_t s8_of(float v)  // nearest even, saturating, NaN -> 0
+{
+    int r;
+    asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(r) : "f"(v));
+    return static_cast<uint32_t>(r) & 0xFFu;
+}
+__device__ __forceinline__ uint32_t e4m3x2_of(float a, float b)
+{
+    uint16_t v;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(v) : "f"(b), "f"(a));
+    return v;
+}
+// Eight codes of y = f * mul.
+template <bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8, const float (&y)[8], float mul)
+{
+    uint32_t a, b;
+    if (s8) {
+        a = s8_of(y[0] * mul) | (s8_of(y[1] * mul) << 8) | (s8_of(y[2] * mul) << 16) | (s8_of(y[3] * mul) << 24);
+        b = s8_of(y[4] * mul) | (s8_of(y[5] * mul) << 8) | (s8_of(y[6] * mul) << 16) | (s8_of(y[7] * mul) << 24);
+    } else {
+        a = e4m3x2_of(y[0] * mul, y[1] * mul) | (e4m3x2_of(y[2] * mul, y[3] * mul) << 16);
+        b = e4m3x2_of(y[4] * mul, y[5] * mul) | (e4m3x2_of(y[6] * mul, y[7] * mul) << 16);
+    }
+    if (VEC && c * 8 + 8 <= k) {
+        *reinterpret_cast<uint2*>(row + c * 8) = make_uint2(a, b);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (c * 8 + j < k) row[c * 8 + j] = static_cast<uint8_t>((j < 4 ? a : b) >> (8 * (j & 3)));
+    }
+}
+
+// One row per TPR threads: a warp (blocks of 128 threads hold four rows) or the whole block.  Thread t owns chunks t, t + TPR, ...
+template <typename T, int TPR, int NCHUNK, bool VEC>
+__global__ void __launch_bounds__(TPR > 32 ? TPR : 128)
+rms_norm_kernel(const NormArgs p)
+{
+    __shared__ float2 red[32];
+    grid_dependency_wait();
+    const int t = TPR > 32 ? threadIdx.x : threadIdx.x & 31;
+    const long long row = TPR > 32 ? blockIdx.x : blockIdx.x * 4ll + (threadIdx.x >> 5);
+    if (row >= p.m) return;  // whole warps; never with a block per row
+    const int k = p.k;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.ld_residual : nullptr;
+    Raw8<T> xr[NCHUNK], rr[NCHUNK];
+#pragma unroll
+    for (int i = 0; i < NCHUNK; ++i) {
+        const int c = t + i * TPR;
+        if (c * 8 < k) {
+            load_chunk<T, VEC>(x, c, k, xr[i]);
+            if (r) load_chunk<T, VEC>(r, c, k, rr[i]);
+        }
+    }
+    float hg[NCHUNK][8];
+    float ss = 0.0f, amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NCHUNK; ++i) {
+        const int c = t + i * TPR;
+        if (c * 8 < k) {
+            float g[8];
+            unpack8(xr[i], hg[i]);
+            if (r) {
+                float v[8];
+                unpack8(rr[i], v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) hg[i][j] += v[j];
+            }
+            if (p.sum) store_chunk<T, VEC>(static_cast<T*>(p.sum) + row * p.ld_sum, c, k, hg[i]);
+            load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                ss = fmaf(hg[i][j], hg[i][j], ss);
+                hg[i][j] *= g[j];
+                amax = max_nan(amax, fabsf(hg[i][j]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) hg[i][j] = 0.0f;
+        }
+    }
+    row_reduce<TPR>(ss, amax, red);
+    const float rstd = __frsqrt_rn(__fdiv_rn(ss, static_cast<float>(k)) + p.eps);
+    if (p.rstd && t == 0) p.rstd[row] = rstd;
+    if (p.y) {
+        T* y = static_cast<T*>(p.y) + row * p.ldy;
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i) {
+            const int c = t + i * TPR;
+            if (c * 8 < k) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = hg[i][j] * rstd;
+                store_chunk<T, VEC>(y, c, k, v);
+            }
+        }
+    }
+    if (!p.q) return;
+    uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.ldq;
+    const bool s8 = p.q_s8 != 0;
+    float inv = 0.0f;
+    if (p.scale_mode == ASCB200_SCALE_PER_TOKEN) {
+        float scale;
+        scale_of(amax * rstd, s8, scale, inv);
+        if (t == 0) static_cast<float*>(p.scale)[row] = scale;
+    }
+    const int lanes = p.group_lanes;
+    const long long groups = (k + lanes * 8 - 1) / (lanes * 8);
+#pragma unroll
+    for (int i = 0; i < NCHUNK; ++i) {
+        const int c = t + i * TPR;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = hg[i][j] * rstd;
+        if (p.scale_mode != ASCB200_SCALE_PER_TOKEN) {
+            // a group is `lanes` neighbouring lanes: the whole warp takes part, lanes past the row's end with zeros
+            float g = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g = max_nan(g, fabsf(y[j]));
+            for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+            const bool first = (c & (lanes - 1)) == 0 && c * 8 < k;
+            if (p.scale_mode == ASCB200_SCALE_MX) {
+                const uint32_t byte = mx_scale_byte(g, inv);
+                if (first) static_cast<uint8_t*>(p.scale)[row * groups + c / lanes] = static_cast<uint8_t>(byte);
+            } else {
+                float scale;
+                scale_of(g, s8, scale, inv);
+                if (first) static_cast<float*>(p.scale)[row * groups + c / lanes] = scale;
+            }
+        }
+        if (c * 8 < k) store_codes<VEC>(q, c, k, s8, y, inv);
+    }
+}
+
+constexpr int kMaxNormK = 32768;
+
+template <typename T, bool VEC>
+int launch_norm(const NormArgs& p, int sms, cudaStream_t st)
+{
+    const int chunks = (p.k + 7) / 8;
+#define ASCB200_NORM_WARP(NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, 32, NC, VEC>, static_cast<unsigned>((p.m + 3ll) / 4), 128, 0, st, p))
+#define ASCB200_NORM_BLOCK(TPR, NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, TPR, NC, VEC>, p.m, TPR, 0, st, p))
+    if (chunks <= 32) ASCB200_NORM_WARP(1);
+    else if (chunks <= 64) ASCB200_NORM_WARP(2);
+    else if (chunks <= 128) ASCB200_NORM_WARP(4);
+    else if (chunks <= 256) ASCB200_NORM_BLOCK(128, 2);
+    else if (chunks <= 512) ASCB200_NORM_BLOCK(256, 2);
+    else if (chunks <= 1024) ASCB200_NORM_BLOCK(256, 4);
+    else if (chunks <= 2048) ASCB200_NORM_BLOCK(512, 4);
+    else ASCB200_NORM_BLOCK(1024, 4);
+#undef ASCB200_NORM_WARP
+#undef ASCB200_NORM_BLOCK
+    (void)sms;
+    return ASCB200_OK;
+}
+
+bool is_float_type(int dtype) { return dtype == ASCB200_F32 || dtype == ASCB200_F16 || dtype == ASCB200_BF16; }
+int float_bytes(int dtype) { return dtype == ASCB200_F32 ? 4 : 2; }
+
+// A matrix of rows `ld` elements apart: 0 stands for packed rows.  Returns false for a leading dimension under the row's length.
+bool resolve_ld(int64_t& ld, int k)
+{
+    if (ld == 0) ld = k;
+    return ld >= k;
+}
+bool element_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+bool rows_aligned(const void* p, int64_t ld, int bytes, int to) { return !p || (aligned_to(p, to) && (ld * bytes) % to == 0); }
+
+int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
+{
+    DeviceState* st = current_state();
+    if (!st) return ASCB200_ENODEV;
+    if (!desc) return ASCB200_EINVAL;
+    ascb200_rms_norm_desc d = *desc;
+    if (d.m < 0 || d.k <= 0 || !(d.eps >= 0.0f)) return ASCB200_EINVAL;
+    if (!is_float_type(d.dtype)) return ASCB200_EUNSUPPORTED;
+    if (d.gamma_dev && d.gamma_dtype != d.dtype && d.gamma_dtype != ASCB200_F32) return ASCB200_EUNSUPPORTED;
+    if (d.reserved[0] != 0 || d.reserved[1] != 0) return ASCB200_EINVAL;
+    if (!resolve_ld(d.ldx, d.k) || !resolve_ld(d.ld_residual, d.k) || !resolve_ld(d.ld_sum, d.k) || !resolve_ld(d.ldy, d.k) || !resolve_ld(d.ldq, d.k)) return ASCB200_EINVAL;
+    NormArgs p = {};
+    if (d.q_dev) {
+        if (d.q_dtype != ASCB200_S8 && d.q_dtype != ASCB200_FP8_E4M3) return ASCB200_EUNSUPPORTED;
+        if (!d.scale_dev && d.m > 0) return ASCB200_EINVAL;
+        int group = 256;
+        if (d.scale_mode == ASCB200_SCALE_PER_TOKEN) {
+            if (d.group_size != 0) return ASCB200_EINVAL;
+        } else if (d.scale_mode == ASCB200_SCALE_PER_GROUP) {
+            group = d.group_size;
+            if (group != 32 && group != 64 && group != 128 && group != 256) return ASCB200_EUNSUPPORTED;
+        } else if (d.scale_mode == ASCB200_SCALE_MX) {
+            if (d.q_dtype != ASCB200_FP8_E4M3) return ASCB200_EUNSUPPORTED;
+            if (d.group_size != 0 && d.group_size != 32) return ASCB200_EINVAL;
+            group = 32;
+        } else {
+            return ASCB200_EINVAL;
+        }
+        p.group_lanes = group / 8;
+        if (d.scale_mode != ASCB200_SCALE_MX && !element_aligned(d.scale_dev, 4)) return ASCB200_EALIGN;
+    } else {
+        if (!d.y_dev && d.m > 0) return ASCB200_EINVAL;  // nothing that depends on the norm would be written
+        p.group_lanes = 32;
+    }
+    if (d.k > kMaxNormK) return ASCB200_ETOOBIG;
+    if (d.m == 0) return ASCB200_OK;
+    if (!d.x_dev) return ASCB200_EINVAL;
+    if (d.sum_dev && d.sum_dev == d.y_dev) return ASCB200_EINVAL;
+    const int esz = float_bytes(d.dtype), gsz = float_bytes(d.gamma_dtype);
+    if (!element_aligned(d.x_dev, esz) || !element_aligned(d.residual_dev, esz) || !element_aligned(d.sum_dev, esz) || !element_aligned(d.y_dev, esz) ||
+        (d.gamma_dev && !element_aligned(d.gamma_dev, gsz)) || !element_aligned(d.rstd_dev, 4))
+        return ASCB200_EALIGN;
+    p.x = d.x_dev, p.residual = d.residual_dev, p.gamma = d.gamma_dev, p.sum = d.sum_dev, p.y = d.y_dev, p.q = d.q_dev, p.scale = d.scale_dev;
+    p.rstd = d.rstd_dev;
+    p.ldx = d.ldx, p.ld_residual = d.ld_residual, p.ld_sum = d.ld_sum, p.ldy = d.ldy, p.ldq = d.ldq;
+    p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32, p.q_s8 = d.q_dtype == ASCB200_S8, p.scale_mode = d.scale_mode, p.eps = d.eps;
+    // 16-byte accesses where every row of every tensor allows them; element by element otherwise
+    const bool vec = rows_aligned(d.x_dev, d.ldx, esz, 16) && rows_aligned(d.residual_dev, d.ld_residual, esz, 16) && rows_aligned(d.sum_dev, d.ld_sum, esz, 16) &&
+                     rows_aligned(d.y_dev, d.ldy, esz, 16) && rows_aligned(d.q_dev, d.ldq, 1, 8) && (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
+    const int sms = st->sm_count;
+    switch (d.dtype) {
+        case ASCB200_F16: return vec ? launch_norm<__half, true>(p, sms, stream) : launch_norm<__half, false>(p, sms, stream);
+        case ASCB200_BF16: return vec ? launch_norm<__nv_bfloat16, true>(p, sms, stream) : launch_norm<__nv_bfloat16, false>(p, sms, stream);
+        default: return vec ? launch_norm<float, true>(p, sms, stream) : launch_norm<float, false>(p, sms, stream);
+    }
+}
+
+// ---- gradients -----------------------------------------------------------------------------------------------------------------
+struct NormGradArgs {
+    const void* dy;
+    const void* h;
+    const float* rstd;
+    const void* gamma;
+    const void* dh;
+    void* dx;
+    float* partial;  // [blocks][k]
+    long long ld_dy, ldh, ld_dh, ld_dx;
+    int m, k;
+    int gamma_f32;
+};
+
+constexpr int kMaxGradBlocks = 296;  // rows of the workspace
+
+// TPR threads per row as above; a block holds ROWS rows at a time (blocks of 256 threads for warp rows).
+template <typename T, int TPR, int NCHUNK, bool VEC>
+__global__ void __launch_bounds__(TPR > 32 ? TPR : 256)
+rms_norm_grad_kernel(const NormGradArgs p)
+{
+    constexpr int ROWS = TPR > 32 ? 1 : 8;
+    __shared__ float2 red[2][32];
+    extern __shared__ float warp_acc[];  // warp rows: [8][TPR * NCHUNK * 8]
+    grid_dependency_wait();
+    const int t = TPR > 32 ? threadIdx.x : threadIdx.x & 31;
+    const int sub = TPR > 32 ? 0 : threadIdx.x >> 5;
+    const int k = p.k;
+    const float inv_k = __frcp_rn(static_cast<float>(k));
+    float acc[NCHUNK][8];
+#pragma unroll
+    for (int i = 0; i < NCHUNK; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
+    int parity = 0;
+    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + sub; row < p.m; row += gridDim.x * ROWS, parity ^= 1) {
+        const T* dy = static_cast<const T*>(p.dy) + row * p.ld_dy;
+        const T* h = static_cast<const T*>(p.h) + row * p.ldh;
+        const float rstd = __ldg(p.rstd + row);
+        Raw8<T> dr[NCHUNK], hr[NCHUNK], er[NCHUNK];
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i) {
+            const int c = t + i * TPR;
+            if (c * 8 < k) {
+                load_chunk<T, VEC>(dy, c, k, dr[i]);
+                load_chunk<T, VEC>(h, c, k, hr[i]);
+                if (p.dh) load_chunk<T, VEC>(static_cast<const T*>(p.dh) + row * p.ld_dh, c, k, er[i]);
+            }
+        }
+        float dot = 0.0f, none = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i) {
+            const int c = t + i * TPR;
+            if (c * 8 < k) {
+                float a[8], b[8], g[8];
+                unpack8(dr[i], a);
+                unpack8(hr[i], b);
+                load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = a[j] * (b[j] * rstd);  // dy * hat
+                    acc[i][j] += v;
+                    dot = fmaf(v, g[j], dot);
+                }
+            }
+        }
+        row_reduce<TPR>(dot, none, red[parity]);
+        const float mean = dot * inv_k;
+        T* dx = static_cast<T*>(p.dx) + row * p.ld_dx;
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i) {
+            const int c = t + i * TPR;
+            if (c * 8 < k) {
+                float a[8], b[8], g[8], e[8];
+                unpack8(dr[i], a);
+                unpack8(hr[i], b);
+                load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
+                if (p.dh) unpack8(er[i], e);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = rstd * (a[j] * g[j] - (b[j] * rstd) * mean);
+                    a[j] = p.dh ? v + e[j] : v;
+                }
+                store_chunk<T, VEC>(dx, c, k, a);
+            }
+        }
+    }
+    if (!p.partial) return;
+    float* out = p.partial + static_cast<size_t>(blockIdx.x) * k;
+    if constexpr (TPR > 32) {
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int col = (t + i * TPR) * 8 + j;
+                if (col < k) out[col] = acc[i][j];
+            }
+    } else {
+        constexpr int W = TPR * NCHUNK * 8;
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) warp_acc[sub * W + (t + i * TPR) * 8 + j] = acc[i][j];
+        __syncthreads();
+        for (int col = threadIdx.x; col < k; col += 256) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < ROWS; ++w) v += warp_acc[w * W + col];
+            out[col] = v;
+        }
+    }
+}
+
+// dgamma[col] = sum over the blocks' partial sums, in block order per thread and then over the eight warps in order.
+template <typename G>
+__global__ void __launch_bounds__(256)
+rms_norm_dgamma_kernel(const float* __restrict__ partial, G* __restrict__ dgamma, int blocks, int k)
+{
+    __shared__ float part[8][32];
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    float v = 0.0f;
+    if (col < k) {
+#pragma unroll 8
+        for (int b = w; b < blocks; b += 8) v += partial[static_cast<size_t>(b) * k + col];
+    }
+    part[w][lane] = v;
+    __syncthreads();
+    if (w == 0 && col < k) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) v += part[i][lane];
+        if constexpr (sizeof(G) == 4) dgamma[col] = v;
+        else reinterpret_cast<uint16_t*>(dgamma)[col] = static_cast<uint16_t>(pack2(v, 0.0f, G()) & 0xFFFFu);
+    }
+}
+
+template <typename T, int TPR, int NCHUNK, bool VEC>
+int launch_norm_grad_as(const NormGradArgs& p, int sms, cudaStream_t st, int* blocks)
+{
+    constexpr int rows = TPR > 32 ? 1 : 8;
+    constexpr size_t smem = TPR > 32 ? 0 : 8 * TPR * NCHUNK * 8 * sizeof(float);
+    *blocks = static_cast<int>(std::min<long long>((p.m + rows - 1ll) / rows, std::min(2 * sms, kMaxGradBlocks)));
+    ASCB200_CUDA(launch_pdl(rms_norm_grad_kernel<T, TPR, NCHUNK, VEC>, *blocks, TPR > 32 ? TPR : 256, smem, st, p));
+    return ASCB200_OK;
+}
+template <typename T, bool VEC>
+int launch_norm_grad(const NormGradArgs& p, int sms, cudaStream_t st, int* blocks)
+{
+    const int chunks = (p.k + 7) / 8;
+    if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, VEC>(p, sms, st, blocks);
+    if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, VEC>(p, sms, st, blocks);
+    if (chunks <= 128) return launch_norm_grad_as<T, 32, 4, VEC>(p, sms, st, blocks);
+    if (chunks <= 256) return launch_norm_grad_as<T, 128, 2, VEC>(p, sms, st, blocks);
+    if (chunks <= 512) return launch_norm_grad_as<T, 256, 2, VEC>(p, sms, st, blocks);
+    if (chunks <= 1024) return launch_norm_grad_as<T, 512, 2, VEC>(p, sms, st, blocks);
+    if (chunks <= 2048) return launch_norm_grad_as<T, 512, 4, VEC>(p, sms, st, blocks);
+    return launch_norm_grad_as<T, 1024, 4, VEC>(p, sms, st, blocks);
+}
+
+size_t grad_workspace(int m, int k) { return m <= 0 || k <= 0 ? 0 : static_cast<size_t>(std::min(m, kMaxGradBlocks)) * k * sizeof(float); }
+
+int run_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, cudaStream_t stream)
+{
+    DeviceState* st = current_state();
+    if (!st) return ASCB200_ENODEV;
+    if (!desc) return ASCB200_EINVAL;
+    ascb200_rms_norm_grad_desc d = *desc;
+    if (d.m < 0 || d.k <= 0 || d.reserved != 0) return ASCB200_EINVAL;
+    if (!is_float_type(d.dtype)) return ASCB200_EUNSUPPORTED;
+    if (d.gamma_dev && d.gamma_dtype != d.dtype && d.gamma_dtype != ASCB200_F32) return ASCB200_EUNSUPPORTED;
+    if (d.dgamma_dev && d.dgamma_dtype != d.dtype && d.dgamma_dtype != ASCB200_F32) return ASCB200_EUNSUPPORTED;
+    if (!resolve_ld(d.ld_dy, d.k) || !resolve_ld(d.ldh, d.k) || !resolve_ld(d.ld_dh, d.k) || !resolve_ld(d.ld_dx, d.k)) return ASCB200_EINVAL;
+    if (d.k > kMaxNormK) return ASCB200_ETOOBIG;
+    const int esz = float_bytes(d.dtype);
+    if (d.dgamma_dev && !element_aligned(d.dgamma_dev, float_bytes(d.dgamma_dtype))) return ASCB200_EALIGN;
+    if (d.m == 0) {
+        if (d.dgamma_dev) ASCB200_CUDA(cudaMemsetAsync(d.dgamma_dev, 0, static_cast<size_t>(d.k) * float_bytes(d.dgamma_dtype), stream));
+        return ASCB200_OK;
+    }
+    if (!d.dy_dev || !d.h_dev || !d.rstd_dev || !d.dx_dev) return ASCB200_EINVAL;
+    if (!element_aligned(d.dy_dev, esz) || !element_aligned(d.h_dev, esz) || !element_aligned(d.dh_dev, esz) || !element_aligned(d.dx_dev, esz) ||
+        !element_aligned(d.rstd_dev, 4) || (d.gamma_dev && !element_aligned(d.gamma_dev, float_bytes(d.gamma_dtype))))
+        return ASCB200_EALIGN;
+    if (d.dgamma_dev) {
+        if (!d.workspace_dev || d.workspace_bytes < grad_workspace(d.m, d.k)) return ASCB200_EINVAL;
+        if (!aligned_to(d.workspace_dev, 16)) return ASCB200_EALIGN;
+    }
+    NormGradArgs p = {};
+    p.dy = d.dy_dev, p.h = d.h_dev, p.rstd = d.rstd_dev, p.gamma = d.gamma_dev, p.dh = d.dh_dev, p.dx = d.dx_dev;
+    p.partial = d.dgamma_dev ? static_cast<float*>(d.workspace_dev) : nullptr;
+    p.ld_dy = d.ld_dy, p.ldh = d.ldh, p.ld_dh = d.ld_dh, p.ld_dx = d.ld_dx, p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32;
+    const bool vec = rows_aligned(d.dy_dev, d.ld_dy, esz, 16) && rows_aligned(d.h_dev, d.ldh, esz, 16) && rows_aligned(d.dh_dev, d.ld_dh, esz, 16) &&
+                     rows_aligned(d.dx_dev, d.ld_dx, esz, 16) && (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
+    int blocks = 0, rc;
+    const int sms = st->sm_count;
+    switch (d.dtype) {
+        case ASCB200_F16: rc = vec ? launch_norm_grad<__half, true>(p, sms, stream, &blocks) : launch_norm_grad<__half, false>(p, sms, stream, &blocks); break;
+        case ASCB200_BF16:
+            rc = vec ? launch_norm_grad<__nv_bfloat16, true>(p, sms, stream, &blocks) : launch_norm_grad<__nv_bfloat16, false>(p, sms, stream, &blocks);
+            break;
+        default: rc = vec ? launch_norm_grad<float, true>(p, sms, stream, &blocks) : launch_norm_grad<float, false>(p, sms, stream, &blocks);
+    }
+    if (rc != ASCB200_OK || !d.dgamma_dev) return rc;
+    const int grid = (d.k + 31) / 32;
+    if (d.dgamma_dtype == ASCB200_F32)
+        ASCB200_CUDA(launch_pdl(rms_norm_dgamma_kernel<float>, grid, 256, 0, stream, p.partial, static_cast<float*>(d.dgamma_dev), blocks, d.k));
+    else if (d.dgamma_dtype == ASCB200_F16)
+        ASCB200_CUDA(launch_pdl(rms_norm_dgamma_kernel<__half>, grid, 256, 0, stream, p.partial, static_cast<__half*>(d.dgamma_dev), blocks, d.k));
+    else
+        ASCB200_CUDA(launch_pdl(rms_norm_dgamma_kernel<__nv_bfloat16>, grid, 256, 0, stream, p.partial, static_cast<__nv_bfloat16*>(d.dgamma_dev), blocks, d.k));
+    return ASCB200_OK;
+}
+
+}  // namespace
+}  // namespace ascb200
+
+extern "C" {
+
+int ascb200_rms_norm(const ascb200_rms_norm_desc* desc, void* stream) { return ascb200::run_rms_norm(desc, static_cast<cudaStream_t>(stream)); }
+
+size_t ascb200_rms_norm_grad_workspace_bytes(int32_t m, int32_t k) { return ascb200::grad_workspace(m, k); }
+
+int ascb200_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, void* stream)
+{
+    return ascb200::run_rms_norm_grad(desc, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

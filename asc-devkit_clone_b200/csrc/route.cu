@@ -1,0 +1,508 @@
+// Routing of tokens to experts: softmax over the experts, the k most probable of them with their weights, the rows per expert as
+// ascb200_grouped_gemm takes them, a balance loss, and the gradients of both.
+//
+//   p[t, e] = softmax over the unmasked experts of logits[t]          (a logit of -inf masks its expert)
+//   idx[t, j], weights[t, j]: the j-th largest, ties to the lower index; weights p or p / sum of the chosen p
+//   counts[e] = tokens that chose e,   N = tokens in use,   P[e] = sum_t p[t, e] / N
+//   loss = E / (N top_k) * sum_e counts[e] * P[e]                     (1 for perfect balance)
+//
+// Gradients (counts are constants): dp[t, e] = dloss * E * counts[e] / (N^2 top_k) + (what the weights' gradient gives the chosen),
+// dlogits = p * (dp - sum_e p dp).
+//
+// One token per warp, its logits in registers (expert e in lane e % 32).  The sums over tokens stay in registers, then shared
+// memory, then one row of the workspace per block; a second kernel adds these rows in block order.  Integer atomics only, so
+// every output is reproducible.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace ascb200 {
+namespace {
+
+constexpr int kMaxExperts = 1024;     // what ascb200_grouped_gemm takes
+constexpr int kMaxTopK = 32;          // one choice per lane
+constexpr int kRouteWarps = 16;       // tokens at a time per block
+constexpr int kMaxRouteBlocks = 296;  // rows of the workspace
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr unsigned kAll = 0xFFFFFFFFu;
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    return v;
+}
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return f32_to_f16_sat(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return f32_to_bf16(v); }
+
+// Logits as unsigned integers in their order (the usual map of IEEE bit patterns), -0 as +0.  0: masked (-inf), never chosen;
+// 1: NaN, chosen after every number.
+constexpr uint32_t kMasked = 0u;
+__device__ __forceinline__ uint32_t order_key(float x)
+{
+    if (x != x) return 1u;
+    const uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));
+    const uint32_t key = b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+    return key == 0x007FFFFFu ? kMasked : key;
+}
+__device__ __forceinline__ float key_value(uint32_t key)
+{
+    if (key == 1u) return __uint_as_float(0x7FC00000u);
+    return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
+}
+
+struct RouteArgs {
+    const void* logits;
+    const uint8_t* valid;
+    int* idx;
+    float* weights;
+    long long* counts;
+    long long* num_tokens;
+    float* prob_mean;
+    float* loss;
+    float* part_prob;  // [blocks][experts]
+    int* part_count;   // [blocks][experts]
+    int* part_tokens;  // [blocks]
+    long long ld;
+    int tokens, experts, top_k, renorm;
+};
+
+// loss, means and counts from the sums of one expert; returns the expert's share of sum_e counts[e] P[e].
+__device__ __forceinline__ float finish_expert(const RouteArgs& p, int e, float prob, int count, float inv_n)
+{
+    const float mean = prob * inv_n;
+    if (p.counts) p.counts[e] = count;
+    if (p.prob_mean) p.prob_mean[e] = mean;
+    return static_cast<float>(count) * mean;
+}
+__device__ __forceinline__ float loss_of(const RouteArgs& p, float total, float inv_n)
+{
+    return total * inv_n * (static_cast<float>(p.experts) / static_cast<float>(p.top_k));
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+route_kernel(const RouteArgs p)
+{
+    extern __shared__ float s_prob[];  // [kRouteWarps][experts], then int [experts] counts
+    __shared__ int s_tokens[kRouteWarps];
+    __shared__ float s_part[kRouteWarps];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int E = p.experts, K = p.top_k;
+    int* s_count = reinterpret_cast<int*>(s_prob + kRouteWarps * E);
+    for (int e = threadIdx.x; e < E; e += kRouteWarps * 32) s_count[e] = 0;
+    __syncthreads();
+    grid_dependency_wait();
+    float acc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
+    int used = 0;
+    for (long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + w; t < p.tokens; t += gridDim.x * kRouteWarps) {
+        const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+        uint32_t key[NV];
+        uint32_t top = kMasked;
+        const bool open = !p.valid || p.valid[t] != 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = lane + 32 * i;
+            key[i] = (open && e < E) ? order_key(to_f32(row[e])) : kMasked;
+            top = max(top, key[i]);
+        }
+        top = __reduce_max_sync(kAll, top);
+        int my_idx = -1;
+        float my_w = 0.0f;
+        if (top != kMasked) {  // at least one expert to choose
+            ++used;
+            const float mx = key_value(top);
+            float prob[NV], sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                prob[i] = key[i] != kMasked ? exp2_approx((key_value(key[i]) - mx) * kLog2e) : 0.0f;
+                sum += prob[i];
+            }
+            const float inv = __frcp_rn(warp_sum(sum));
+#pragma unroll
+            for (int i = 0; i < NV; ++i) acc[i] = fmaf(prob[i], inv, acc[i]);
+            uint32_t my_key = kMasked;
+            for (int j = 0; j < K && top != kMasked; ++j) {
+                int e = kMaxExperts;
+#pragma unroll
+                for (int i = NV - 1; i >= 0; --i)
+                    if (key[i] == top) e = lane + 32 * i;
+                e = __reduce_min_sync(kAll, e);  // of equal logits the first expert
+                if (lane == j) my_idx = e, my_key = top;
+                top = kMasked;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    if (lane + 32 * i == e) key[i] = kMasked;
+                    top = max(top, key[i]);
+                }
+                top = __reduce_max_sync(kAll, top);
+            }
+            if (my_idx >= 0) {
+                my_w = exp2_approx((key_value(my_key) - mx) * kLog2e) * inv;
+                atomicAdd(&s_count[my_idx], 1);
+            }
+            if (p.renorm) {
+                const float chosen = warp_sum(my_w);  // lanes without a choice hold 0
+                if (my_idx >= 0) my_w = __fdiv_rn(my_w, chosen);
+            }
+        }
+        if (lane < K) {
+            p.idx[t * K + lane] = my_idx;
+            p.weights[t * K + lane] = my_w;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (lane + 32 * i < E) s_prob[w * E + lane + 32 * i] = acc[i];
+    if (lane == 0) s_tokens[w] = used;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kRouteWarps; ++i) n += s_tokens[i];
+    const float inv_n = __frcp_rn(static_cast<float>(max(n, 1)));
+    float share = 0.0f;
+    for (int e = threadIdx.x; e < E; e += kRouteWarps * 32) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRouteWarps; ++i) v += s_prob[i * E + e];
+        if (gridDim.x == 1) {
+            share += finish_expert(p, e, v, s_count[e], inv_n);
+        } else {
+            p.part_prob[static_cast<size_t>(blockIdx.x) * E + e] = v;
+            p.part_count[static_cast<size_t>(blockIdx.x) * E + e] = s_count[e];
+        }
+    }
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) p.part_tokens[blockIdx.x] = n;
+        return;
+    }
+    share = warp_sum(share);
+    if (lane == 0) s_part[w] = share;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRouteWarps; ++i) total += s_part[i];
+        if (p.loss) p.loss[0] = loss_of(p, total, inv_n);
+        if (p.num_tokens) p.num_tokens[0] = n;
+    }
+}
+
+// Adds the blocks' rows.  One cluster of eight blocks; each takes an eighth of the experts, 32 at a time, its eight warps a share
+// of the rows each; the shares of the loss meet in the first block's shared memory.
+constexpr int kFinishBlocks = 8;
+__global__ void __cluster_dims__(kFinishBlocks, 1, 1) __launch_bounds__(256)
+route_finish_kernel(const RouteArgs p, int blocks)
+{
+    __shared__ float s_p[8][32];
+    __shared__ int s_c[8][32];
+    __shared__ int s_n[8];
+    __shared__ float s_loss[kFinishBlocks];
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for below: every block of the cluster has started
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int n = 0;
+    for (int b = threadIdx.x; b < blocks; b += 256) n += p.part_tokens[b];
+    n = __reduce_add_sync(kAll, n);
+    if (lane == 0) s_n[w] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n += s_n[i];
+    const float inv_n = __frcp_rn(static_cast<float>(max(n, 1)));
+    const int per = (p.experts + kFinishBlocks - 1) / kFinishBlocks;
+    const int e1 = min(p.experts, (static_cast<int>(blockIdx.x) + 1) * per);
+    float share = 0.0f;
+    for (int base = blockIdx.x * per; base < e1; base += 32) {
+        const int e = base + lane;
+        float v = 0.0f;
+        int c = 0;
+        if (e < e1) {
+#pragma unroll 4
+            for (int b = w; b < blocks; b += 8) {
+                v += p.part_prob[static_cast<size_t>(b) * p.experts + e];
+                c += p.part_count[static_cast<size_t>(b) * p.experts + e];
+            }
+        }
+        __syncthreads();
+        s_p[w][lane] = v, s_c[w][lane] = c;
+        __syncthreads();
+        if (w == 0 && e < e1) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i) v += s_p[i][lane], c += s_c[i][lane];
+            share += finish_expert(p, e, v, c, inv_n);
+        }
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (w == 0) {
+        share = warp_sum(share);
+        if (lane == 0) {
+            uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(&s_loss[blockIdx.x])), first;
+            asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(first) : "r"(slot));
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(first), "f"(share) : "memory");
+        }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFinishBlocks; ++i) total += s_loss[i];
+        if (p.loss) p.loss[0] = loss_of(p, total, inv_n);
+        if (p.num_tokens) p.num_tokens[0] = n;
+    }
+}
+
+struct RouteGradArgs {
+    const void* logits;
+    const int* idx;
+    const long long* counts;
+    const long long* num_tokens;
+    const float* dloss;
+    const float* dweights;
+    void* dlogits;
+    long long ld, ld_out;
+    int tokens, experts, top_k, renorm;
+};
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(256)
+route_grad_kernel(const RouteGradArgs p)
+{
+    extern __shared__ float s_given[];  // [8][experts]: what the weights' gradient gives the chosen experts of a warp's token, else 0
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int E = p.experts, K = p.top_k;
+    float* given = s_given + w * E;
+    for (int e = lane; e < E; e += 32) given[e] = 0.0f;
+    __syncwarp();
+    grid_dependency_wait();
+    float coef = 0.0f;
+    if (p.dloss) {
+        const float n = static_cast<float>(max(*p.num_tokens, 1ll));
+        coef = *p.dloss * static_cast<float>(E) / (n * n * static_cast<float>(K));
+    }
+    float base[NV];  // dloss * E * counts[e] / (N^2 top_k)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) base[i] = (p.dloss && lane + 32 * i < E) ? coef * static_cast<float>(p.counts[lane + 32 * i]) : 0.0f;
+    for (long long t = static_cast<long long>(blockIdx.x) * 8 + w; t < p.tokens; t += gridDim.x * 8) {
+        const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+        T* out = static_cast<T*>(p.dlogits) + t * p.ld_out;
+        int my = lane < K ? p.idx[t * K + lane] : -1;
+        if (my >= E) my = -1;
+        const float gw = (p.dweights && my >= 0) ? p.dweights[t * K + lane] : 0.0f;
+        const bool in_use = __any_sync(kAll, my >= 0);
+        if (!in_use) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(0.0f);
+            continue;
+        }
+        float x[NV], mx = -__builtin_huge_valf();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] = lane + 32 * i < E ? to_f32(row[lane + 32 * i]) : -__builtin_huge_valf();
+            mx = fmaxf(mx, x[i]);
+        }
+        const float mine = my >= 0 ? to_f32(row[my]) : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] = exp2_approx((x[i] - mx) * kLog2e);
+            sum += x[i];
+        }
+        const float inv = __frcp_rn(warp_sum(sum));
+        float g = gw;
+        if (p.dweights && p.renorm) {
+            // weights = p / S over the chosen: d/dp = (gw - sum gw * weights) / S
+            const float pj = my >= 0 ? exp2_approx((mine - mx) * kLog2e) * inv : 0.0f;
+            const float s = warp_sum(pj), dot = warp_sum(gw * pj);
+            const float inv_s = __frcp_rn(s);
+            g = (gw - dot * inv_s) * inv_s;
+        }
+        if (my >= 0) atomicAdd(&given[my], g);
+        __syncwarp();
+        float dp[NV], dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] *= inv;
+            dp[i] = base[i] + (lane + 32 * i < E ? given[lane + 32 * i] : 0.0f);
+            dot = fmaf(x[i], dp[i], dot);
+        }
+        dot = warp_sum(dot);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(x[i] * (dp[i] - dot));
+        __syncwarp();
+        if (my >= 0) given[my] = 0.0f;
+        __syncwarp();
+    }
+}
+
+bool is_float_type(int dtype) { return dtype == ASCB200_F32 || dtype == ASCB200_F16 || dtype == ASCB200_BF16; }
+bool element_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int route_blocks(int tokens) { return static_cast<int>(std::min<long long>((tokens + kRouteWarps - 1ll) / kRouteWarps, kMaxRouteBlocks)); }
+size_t route_workspace(int tokens, int experts)
+{
+    if (tokens <= 0 || experts <= 0) return 0;
+    const int blocks = route_blocks(tokens);
+    return blocks == 1 ? 0 : static_cast<size_t>(blocks) * (2 * static_cast<size_t>(experts) + 1) * 4;
+}
+
+template <typename T, int NV>
+int launch_route_as(const RouteArgs& p, int blocks, cudaStream_t st)
+{
+    const size_t smem = (kRouteWarps + 1) * static_cast<size_t>(p.experts) * 4;
+    if (smem > 48 * 1024) {  // more than 722 experts
+        static bool configured[16] = {};
+        int dev = 0;
+        ASCB200_CUDA(cudaGetDevice(&dev));
+        if (!configured[dev & 15]) {
+            ASCB200_CUDA(cudaFuncSetAttribute(route_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kRouteWarps + 1) * kMaxExperts * 4));
+            configured[dev & 15] = true;
+        }
+    }
+    ASCB200_CUDA(launch_pdl(route_kernel<T, NV>, blocks, kRouteWarps * 32, smem, st, p));
+    if (blocks > 1) ASCB200_CUDA(launch_pdl(route_finish_kernel, kFinishBlocks, 256, 0, st, p, blocks));
+    return ASCB200_OK;
+}
+template <typename T>
+int launch_route(const RouteArgs& p, int blocks, cudaStream_t st)
+{
+    if (p.experts <= 32) return launch_route_as<T, 1>(p, blocks, st);
+    if (p.experts <= 64) return launch_route_as<T, 2>(p, blocks, st);
+    if (p.experts <= 128) return launch_route_as<T, 4>(p, blocks, st);
+    if (p.experts <= 256) return launch_route_as<T, 8>(p, blocks, st);
+    if (p.experts <= 512) return launch_route_as<T, 16>(p, blocks, st);
+    return launch_route_as<T, 32>(p, blocks, st);
+}
+
+template <typename T, int NV>
+int launch_route_grad_as(const RouteGradArgs& p, int sms, cudaStream_t st)
+{
+    const int blocks = static_cast<int>(std::min((p.tokens + 7ll) / 8, 8ll * sms));
+    ASCB200_CUDA(launch_pdl(route_grad_kernel<T, NV>, blocks, 256, 8 * static_cast<size_t>(p.experts) * 4, st, p));
+    return ASCB200_OK;
+}
+template <typename T>
+int launch_route_grad(const RouteGradArgs& p, int sms, cudaStream_t st)
+{
+    if (p.experts <= 32) return launch_route_grad_as<T, 1>(p, sms, st);
+    if (p.experts <= 64) return launch_route_grad_as<T, 2>(p, sms, st);
+    if (p.experts <= 128) return launch_route_grad_as<T, 4>(p, sms, st);
+    if (p.experts <= 256) return launch_route_grad_as<T, 8>(p, sms, st);
+    if (p.experts <= 512) return launch_route_grad_as<T, 16>(p, sms, st);
+    return launch_route_grad_as<T, 32>(p, sms, st);
+}
+
+// Sizes and types that ascb200_route and ascb200_route_grad share.
+int check_route(int tokens, int experts, int top_k, int dtype, int64_t& ld, int renorm)
+{
+    if (tokens < 0 || experts <= 0 || top_k <= 0 || top_k > experts || (renorm != 0 && renorm != 1)) return ASCB200_EINVAL;
+    if (experts > kMaxExperts || top_k > kMaxTopK) return ASCB200_ETOOBIG;
+    if (!is_float_type(dtype)) return ASCB200_EUNSUPPORTED;
+    if (ld == 0) ld = experts;
+    return ld < experts ? ASCB200_EINVAL : ASCB200_OK;
+}
+
+int run_route(const ascb200_route_desc* desc, cudaStream_t stream)
+{
+    DeviceState* st = current_state();
+    if (!st) return ASCB200_ENODEV;
+    if (!desc) return ASCB200_EINVAL;
+    ascb200_route_desc d = *desc;
+    const int rc = check_route(d.tokens, d.experts, d.top_k, d.dtype, d.ld_logits, d.renorm);
+    if (rc != ASCB200_OK) return rc;
+    if (d.reserved != 0) return ASCB200_EINVAL;
+    if (!element_aligned(d.counts_dev, 8) || !element_aligned(d.num_tokens_dev, 8) || !element_aligned(d.prob_mean_dev, 4) || !element_aligned(d.loss_dev, 4))
+        return ASCB200_EALIGN;
+    if (d.tokens == 0) {  // nothing was routed
+        if (d.counts_dev) ASCB200_CUDA(cudaMemsetAsync(d.counts_dev, 0, static_cast<size_t>(d.experts) * 8, stream));
+        if (d.num_tokens_dev) ASCB200_CUDA(cudaMemsetAsync(d.num_tokens_dev, 0, 8, stream));
+        if (d.prob_mean_dev) ASCB200_CUDA(cudaMemsetAsync(d.prob_mean_dev, 0, static_cast<size_t>(d.experts) * 4, stream));
+        if (d.loss_dev) ASCB200_CUDA(cudaMemsetAsync(d.loss_dev, 0, 4, stream));
+        return ASCB200_OK;
+    }
+    if (!d.logits_dev || !d.idx_dev || !d.weights_dev) return ASCB200_EINVAL;
+    if (!element_aligned(d.logits_dev, d.dtype == ASCB200_F32 ? 4 : 2) || !element_aligned(d.idx_dev, 4) || !element_aligned(d.weights_dev, 4)) return ASCB200_EALIGN;
+    const size_t need = route_workspace(d.tokens, d.experts);
+    if (need > 0 && (!d.workspace_dev || d.workspace_bytes < need)) return ASCB200_EINVAL;
+    if (need > 0 && !aligned_to(d.workspace_dev, 16)) return ASCB200_EALIGN;
+    RouteArgs p = {};
+    p.logits = d.logits_dev, p.valid = d.valid_dev, p.idx = d.idx_dev, p.weights = d.weights_dev;
+    p.counts = reinterpret_cast<long long*>(d.counts_dev), p.num_tokens = reinterpret_cast<long long*>(d.num_tokens_dev);
+    p.prob_mean = d.prob_mean_dev, p.loss = d.loss_dev;
+    p.ld = d.ld_logits, p.tokens = d.tokens, p.experts = d.experts, p.top_k = d.top_k, p.renorm = d.renorm;
+    const int blocks = std::min(route_blocks(d.tokens), std::max(2, 2 * st->sm_count));
+    if (need > 0) {
+        p.part_prob = static_cast<float*>(d.workspace_dev);
+        p.part_count = reinterpret_cast<int*>(p.part_prob + static_cast<size_t>(blocks) * d.experts);
+        p.part_tokens = p.part_count + static_cast<size_t>(blocks) * d.experts;
+    }
+    switch (d.dtype) {
+        case ASCB200_F16: return launch_route<__half>(p, blocks, stream);
+        case ASCB200_BF16: return launch_route<__nv_bfloat16>(p, blocks, stream);
+        default: return launch_route<float>(p, blocks, stream);
+    }
+}
+
+int run_route_grad(const ascb200_route_grad_desc* desc, cudaStream_t stream)
+{
+    DeviceState* st = current_state();
+    if (!st) return ASCB200_ENODEV;
+    if (!desc) return ASCB200_EINVAL;
+    ascb200_route_grad_desc d = *desc;
+    int rc = check_route(d.tokens, d.experts, d.top_k, d.dtype, d.ld_logits, d.renorm);
+    if (rc != ASCB200_OK) return rc;
+    if (d.ld_dlogits == 0) d.ld_dlogits = d.experts;
+    if (d.ld_dlogits < d.experts || d.reserved != 0) return ASCB200_EINVAL;
+    if (d.tokens == 0) return ASCB200_OK;
+    if (!d.logits_dev || !d.idx_dev || !d.dlogits_dev) return ASCB200_EINVAL;
+    if (d.dloss_dev && (!d.counts_dev || !d.num_tokens_dev)) return ASCB200_EINVAL;
+    const int esz = d.dtype == ASCB200_F32 ? 4 : 2;
+    if (!element_aligned(d.logits_dev, esz) || !element_aligned(d.dlogits_dev, esz) || !element_aligned(d.idx_dev, 4) || !element_aligned(d.counts_dev, 8) ||
+        !element_aligned(d.num_tokens_dev, 8) || !element_aligned(d.dloss_dev, 4) || !element_aligned(d.dweights_dev, 4))
+        return ASCB200_EALIGN;
+    RouteGradArgs p = {};
+    p.logits = d.logits_dev, p.idx = d.idx_dev, p.counts = reinterpret_cast<const long long*>(d.counts_dev);
+    p.num_tokens = reinterpret_cast<const long long*>(d.num_tokens_dev), p.dloss = d.dloss_dev, p.dweights = d.dweights_dev, p.dlogits = d.dlogits_dev;
+    p.ld = d.ld_logits, p.ld_out = d.ld_dlogits, p.tokens = d.tokens, p.experts = d.experts, p.top_k = d.top_k, p.renorm = d.renorm;
+    const int sms = st->sm_count;
+    switch (d.dtype) {
+        case ASCB200_F16: return launch_route_grad<__half>(p, sms, stream);
+        case ASCB200_BF16: return launch_route_grad<__nv_bfloat16>(p, sms, stream);
+        default: return launch_route_grad<float>(p, sms, stream);
+    }
+}
+
+}  // namespace
+}  // namespace ascb200
+
+extern "C" {
+
+size_t ascb200_route_workspace_bytes(int32_t tokens, int32_t experts) { return ascb200::route_workspace(tokens, experts); }
+
+int ascb200_route(const ascb200_route_desc* desc, void* stream) { return ascb200::run_route(desc, static_cast<cudaStream_t>(stream)); }
+
+int ascb200_route_grad(const ascb200_route_grad_desc* desc, void* stream) { return ascb200::run_route_grad(desc, static_cast<cudaStream_t>(stream)); }
+
+}  // extern "C"

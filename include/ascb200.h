@@ -425,6 +425,137 @@ ASCB200_API int ascb200_softmax_quant(const void* src_dev, void* dst_dev, float*
 ASCB200_API int ascb200_dequant(const int32_t* src_dev, void* dst_dev, int32_t m, int32_t n, int32_t cal_count, int32_t n_dst,
                                 int32_t dst_dtype, const void* scale_dev, int32_t scale_dtype, float scale_scalar, void* stream);
 
+/* ---- feed-forward block of a language model: norm, linear layer, routing ------------------------------ */
+/* What stands between the operators above in a transformer's feed-forward half: the norm that makes their quantised operand,
+ * the matrix product with the layer's bias, activation and residual, and the routing that makes ascb200_grouped_gemm's row
+ * counts; each with its gradients.  All take a descriptor that the caller keeps for its buffers; fields that are not used are 0.
+ * Leading dimensions count elements, 0 stands for packed rows.  Working memory, where an operator needs it, is the caller's
+ * (`workspace_dev`, at least ascb200_..._workspace_bytes, 16-byte aligned; nothing has to be in it before, nothing is kept in it
+ * from one call to the next): calls that may overlap in time, captured graphs among them, need one each.  No call allocates or
+ * synchronises, so all may be captured.  Tensors belong to the current device.  Outputs may not overlap inputs or each other
+ * except where it is said.  Results do not depend on timing: sums over rows are made in a fixed order. */
+
+/* How an 8-bit output is scaled: one fp32 per row; one fp32 per row and group of columns ([m, ceil(k / group_size)]); or MX: one
+ * e8m0 byte per row and 32 columns ([m, ceil(k / 32)], what scale_a_dev of the MXFP8 kinds takes). */
+enum { ASCB200_SCALE_PER_TOKEN = 0, ASCB200_SCALE_PER_GROUP = 1, ASCB200_SCALE_MX = 2 };
+
+/* Root-mean-square norm of rows with the residual's addition (RmsNorm of the reference's normalization family, extended by what
+ * follows it in a quantised layer):
+ *   h = x + residual;  rstd = 1 / sqrt(mean(h^2) + eps);  y = h * gamma * rstd          in fp32 throughout, one rounding per output.
+ * Outputs, each optional but y or q: sum = h; y; rstd; and y in 8 bits with its scales:
+ *   S8: scale = max|y| / 127, q = rint(y / scale);  FP8_E4M3: scale = max|y| / 448, q = e4m3(y / scale), over a row or a group;
+ *   MX: e = floor(log2(max|y|)) - 8 over 32 columns, scale byte = e + 127 (at least 0), q = e4m3(y / 2^e) saturating.
+ * With S8 and PER_TOKEN, q and scale are a_dev and tok_scale_dev of an A8W8 ascb200_gemm / ascb200_linear; with MX, a_dev and
+ * scale_a_dev of KIND_MXFP8_E4M3 (k a multiple of 64 there).
+ * All-zero rows and groups (and those whose scale would be under 2^-126) get scale 0 and codes 0.  A NaN or an infinity in a row
+ * makes its rstd, y and scales NaN (0 where only finite values meet an infinity's rstd of 0; MX scale byte 255); int8 codes are 0 there.
+ * F16 outputs saturate at +-65504.  Squares are summed in fp32: rows of |h| above 1e18 overflow.
+ * dtype (x, residual, sum, y): F32 / F16 / BF16; gamma: the same or F32, NULL for ones.  k up to 32768; any alignment of whole
+ * elements, fastest with every row on 16 bytes (q: 8).  sum or y may be x or residual themselves (same leading dimension). */
+typedef struct ascb200_rms_norm_desc {
+    int32_t m, k;
+    int32_t dtype, gamma_dtype;
+    const void* x_dev;
+    int64_t ldx;
+    const void* residual_dev;   /* NULL: h = x */
+    int64_t ld_residual;
+    const void* gamma_dev;      /* [k] */
+    void* sum_dev;              /* [m, k] h, or NULL */
+    int64_t ld_sum;
+    void* y_dev;                /* [m, k], or NULL */
+    int64_t ldy;
+    void* q_dev;                /* [m, k] bytes, or NULL */
+    int64_t ldq;
+    void* scale_dev;            /* beside q: fp32 or e8m0, packed */
+    float* rstd_dev;            /* [m], or NULL */
+    float eps;
+    int32_t q_dtype;            /* S8 / FP8_E4M3 */
+    int32_t scale_mode;         /* ASCB200_SCALE_*; MX with FP8_E4M3 only */
+    int32_t group_size;         /* PER_GROUP: 32, 64, 128 or 256; else 0 */
+    int32_t reserved[2];        /* must be zero */
+} ascb200_rms_norm_desc;
+ASCB200_API int ascb200_rms_norm(const ascb200_rms_norm_desc* desc, void* stream);
+
+/* Its gradients, from dy (the gradient of y; for a quantised y that of the value it stands for) and what the forward call left, h and rstd:
+ *   hat = h * rstd;  g = dy * gamma;  dx = rstd * (g - hat * mean(g * hat)) + dh;  dgamma = sum over rows of dy * hat.
+ * dh (NULL: 0) is the gradient that arrives at `sum` from its other uses; dx is the gradient of x and of the residual alike.
+ * dgamma (NULL: not wanted) is summed in fp32 and needs the workspace; its type is dtype or F32.  m = 0 gives dgamma = 0.
+ * dx may be dy, h or dh themselves (same leading dimension).  k up to 32768. */
+typedef struct ascb200_rms_norm_grad_desc {
+    int32_t m, k;
+    int32_t dtype, gamma_dtype;
+    const void* dy_dev;
+    int64_t ld_dy;
+    const void* h_dev;
+    int64_t ldh;
+    const float* rstd_dev;
+    const void* gamma_dev;
+    const void* dh_dev;
+    int64_t ld_dh;
+    void* dx_dev;
+    int64_t ld_dx;
+    void* dgamma_dev;
+    int32_t dgamma_dtype;
+    int32_t reserved;           /* must be zero */
+    void* workspace_dev;
+    size_t workspace_bytes;
+} ascb200_rms_norm_grad_desc;
+ASCB200_API size_t ascb200_rms_norm_grad_workspace_bytes(int32_t m, int32_t k);
+ASCB200_API int ascb200_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, void* stream);
+
+/* Routing of tokens to experts, in front of ascb200_grouped_gemm:
+ *   p = softmax over the unmasked experts of a token's logits (a logit of -inf masks its expert);
+ *   idx[t, :] = the top_k experts of the largest logits, largest first, of equal ones the lower index first;
+ *   weights[t, j] = p[t, idx[t, j]], divided by their sum over j when renorm != 0;
+ *   counts[e] = tokens that chose e (int64: group_counts_dev);  num_tokens = N, tokens in use;  prob_mean[e] = sum_t p[t, e] / N;
+ *   loss = E / (N top_k) * sum_e counts[e] * prob_mean[e], the balance loss (1 when counts and probabilities are level).
+ * A token whose valid byte is 0, or whose experts are all masked, is not in use: its idx are -1, its weights 0, and it counts
+ * nowhere.  Where fewer than top_k experts are unmasked, the rest of a token's idx are -1 and their weights 0.  NaN logits come after
+ * every number in idx; a NaN or +inf logit makes its token's weights, and so the means and the loss, NaN.  N = 0 gives zeros.
+ * logits F32 / F16 / BF16, arithmetic in fp32.  counts, num_tokens, prob_mean and loss may be NULL.
+ * Up to 1024 experts, top_k up to 32 and no more than the experts. */
+typedef struct ascb200_route_desc {
+    int32_t tokens, experts, top_k;
+    int32_t dtype;
+    const void* logits_dev;     /* [tokens, experts] */
+    int64_t ld_logits;
+    const uint8_t* valid_dev;   /* [tokens], or NULL: all valid */
+    int32_t* idx_dev;           /* [tokens, top_k] */
+    float* weights_dev;         /* [tokens, top_k] */
+    int64_t* counts_dev;        /* [experts] */
+    int64_t* num_tokens_dev;    /* [1] */
+    float* prob_mean_dev;       /* [experts] */
+    float* loss_dev;            /* [1] */
+    void* workspace_dev;        /* may be NULL where ascb200_route_workspace_bytes is 0 */
+    size_t workspace_bytes;
+    int32_t renorm;             /* 0 or 1 */
+    int32_t reserved;           /* must be zero */
+} ascb200_route_desc;
+ASCB200_API size_t ascb200_route_workspace_bytes(int32_t tokens, int32_t experts);
+ASCB200_API int ascb200_route(const ascb200_route_desc* desc, void* stream);
+
+/* The gradient of logits from those of the loss (dloss, one fp32 in device memory; NULL: 0) and of the weights (dweights; NULL: 0),
+ * with idx, counts and num_tokens as ascb200_route wrote them (counts and num_tokens only beside dloss).  Counts are constants:
+ *   dp[t, e] = dloss * E * counts[e] / (N^2 top_k) + [idx[t, j] = e] gw[t, j];  dlogits = p * (dp - sum_e p * dp),
+ *   gw = dweights, or (dweights - sum_j dweights * weights) / sum_j p[t, idx[t, j]] when renorm != 0.
+ * Tokens that are not in use get zeros.  dlogits may be logits itself (same leading dimension). */
+typedef struct ascb200_route_grad_desc {
+    int32_t tokens, experts, top_k;
+    int32_t dtype;              /* logits and dlogits */
+    const void* logits_dev;
+    int64_t ld_logits;
+    const int32_t* idx_dev;
+    const int64_t* counts_dev;
+    const int64_t* num_tokens_dev;
+    const float* dloss_dev;
+    const float* dweights_dev;  /* [tokens, top_k] */
+    void* dlogits_dev;
+    int64_t ld_dlogits;
+    int32_t renorm;             /* as in the forward call */
+    int32_t reserved;           /* must be zero */
+} ascb200_route_grad_desc;
+ASCB200_API int ascb200_route_grad(const ascb200_route_grad_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
