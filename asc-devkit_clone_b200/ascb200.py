@@ -24,7 +24,7 @@ EXPORTS = [
     "ascb200_gemm_mxfp4_noalloc", "ascb200_noalloc_status", "ascb200_mx_scale_prepacked_bytes", "ascb200_mx_scale_prepack", "ascb200_fp4_transpose", "ascb200_shard_nslab", "ascb200_shard_groups_lpt", "ascb200_comm_unique_id", "ascb200_comm_init", "ascb200_comm_init_all", "ascb200_comm_destroy", "ascb200_group_start", "ascb200_group_end", "ascb200_allgather_slabs", "ascb200_interleave_slabs", "ascb200_graph_begin", "ascb200_graph_end", "ascb200_graph_launch", "ascb200_graph_destroy",
     "ascb200_nz_unpack", "ascb200_quant_policy", "ascb200_quant_policy_rm", "ascb200_dequant_policy", "ascb200_softmax_flash_v2", "ascb200_softmax", "ascb200_log_softmax", "ascb200_antiquant", "ascb200_softmax_flash", "ascb200_softmax_grad", "ascb200_simple_softmax", "ascb200_quant_per_tensor", "ascb200_quant_per_channel", "ascb200_softmax_quant", "ascb200_dequant",
     "ascb200_rms_norm", "ascb200_rms_norm_grad", "ascb200_rms_norm_grad_workspace_bytes", "ascb200_route", "ascb200_route_workspace_bytes",
-    "ascb200_route_grad",
+    "ascb200_route_grad", "ascb200_linear", "ascb200_linear_grad", "ascb200_linear_grad_workspace_bytes",
 ]
 
 
@@ -58,6 +58,24 @@ class RmsNormGradDesc(C.Structure):
         ("dy_dev", C.c_void_p), ("ld_dy", C.c_int64), ("h_dev", C.c_void_p), ("ldh", C.c_int64), ("rstd_dev", C.c_void_p), ("gamma_dev", C.c_void_p),
         ("dh_dev", C.c_void_p), ("ld_dh", C.c_int64), ("dx_dev", C.c_void_p), ("ld_dx", C.c_int64), ("dgamma_dev", C.c_void_p),
         ("dgamma_dtype", C.c_int32), ("reserved", C.c_int32), ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [
+        ("kind", C.c_int32), ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("x_dev", C.c_void_p), ("ldx", C.c_int64), ("w_dev", C.c_void_p), ("ldw", C.c_int64),
+        ("trans_w", C.c_int32), ("act", C.c_int32), ("tok_scale_dev", C.c_void_p), ("ch_scale_dev", C.c_void_p), ("bias_dev", C.c_void_p), ("bias_dtype", C.c_int32),
+        ("y_dtype", C.c_int32), ("residual_dev", C.c_void_p), ("ld_residual", C.c_int64), ("y_dev", C.c_void_p), ("ldy", C.c_int64), ("z_dev", C.c_void_p),
+        ("ldz", C.c_int64), ("reserved", C.c_int64),
+    ]
+
+
+class LinearGradDesc(C.Structure):
+    _fields_ = [
+        ("kind", C.c_int32), ("m", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("act", C.c_int32), ("trans_w", C.c_int32), ("dy_dev", C.c_void_p), ("ld_dy", C.c_int64),
+        ("z_dev", C.c_void_p), ("ldz", C.c_int64), ("x_dev", C.c_void_p), ("ldx", C.c_int64), ("w_dev", C.c_void_p), ("ldw", C.c_int64), ("dx_dev", C.c_void_p),
+        ("ld_dx", C.c_int64), ("dw_dev", C.c_void_p), ("ld_dw", C.c_int64), ("dbias_dev", C.c_void_p), ("dw_dtype", C.c_int32), ("dbias_dtype", C.c_int32),
+        ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -172,6 +190,10 @@ def lib():
         _lib.ascb200_route_workspace_bytes.argtypes = [C.c_int32, C.c_int32]
         _lib.ascb200_route_workspace_bytes.restype = C.c_size_t
         _lib.ascb200_route_grad.argtypes = [C.POINTER(RouteGradDesc), C.c_void_p]
+        _lib.ascb200_linear.argtypes = [C.POINTER(LinearDesc), C.c_void_p]
+        _lib.ascb200_linear_grad.argtypes = [C.POINTER(LinearGradDesc), C.c_void_p]
+        _lib.ascb200_linear_grad_workspace_bytes.argtypes = [C.c_int32, C.c_int32]
+        _lib.ascb200_linear_grad_workspace_bytes.restype = C.c_size_t
     return _lib
 
 
@@ -381,6 +403,21 @@ def rms_norm_grad_workspace_bytes(m, k):
 
 def rms_norm_grad(desc, stream=None):
     return lib().ascb200_rms_norm_grad(desc, stream)
+
+
+ACT_NONE, ACT_FASTER_GELU, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3, 4, 5
+
+
+def linear(desc, stream=None):
+    return lib().ascb200_linear(desc, stream)
+
+
+def linear_grad_workspace_bytes(m, n):
+    return lib().ascb200_linear_grad_workspace_bytes(m, n)
+
+
+def linear_grad(desc, stream=None):
+    return lib().ascb200_linear_grad(desc, stream)
 
 
 def route_workspace_bytes(tokens, experts):

@@ -1,0 +1,98 @@
+// Activations of linear layers and their slopes, in fp32.
+#pragma once
+#include "common.cuh"
+
+namespace ascb200 {
+namespace act {
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + e^-x): one ex2, one rcp; an overflowing exponential gives the limit 0.
+__device__ __forceinline__ float sigmoid(float x) { return rcp_fast(1.0f + exp2_fast(-kLog2e * x)); }
+
+// GELU's tanh form is z * sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3).  Beyond |z| = 32 the sigmoid is 0 or 1 to the last bit;
+// the clamp keeps z^3 and z^2 finite.
+constexpr float kTanh2u = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+__device__ __forceinline__ float tanh_arg(float z)
+{
+    const float c = fminf(fmaxf(z, -32.0f), 32.0f);
+    return kTanh2u * c * fmaf(0.044715f * c, c, 1.0f);
+}
+
+// Upper tail of the normal distribution at |z|, and e^(-z^2 / 2): erfc by the rational approximation 7.1.26 of Abramowitz and Stegun
+// (absolute error of erf up to 1.5e-7).  Working with the tail keeps small results of negative z free of cancellation.
+__device__ __forceinline__ float normal_tail(float z, float& e)
+{
+    const float x = fabsf(z) * 0.7071067811865476f;
+    const float t = rcp_fast(fmaf(0.3275911f, x, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    e = exp2_fast(-kLog2e * x * x);
+    return 0.5f * p * t * e;
+}
+
+template <int ACT>
+__device__ __forceinline__ float value(float z)
+{
+    if constexpr (ACT == ASCB200_ACT_FASTER_GELU) return z * sigmoid(1.702f * z);
+    else if constexpr (ACT == ASCB200_ACT_RELU) {
+        float r;
+        asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+        return r;
+    } else if constexpr (ACT == ASCB200_ACT_GELU) {
+        float e;
+        const float tail = normal_tail(z, e);
+        return z > 0.0f ? fmaf(-z, tail, z) : z * tail;
+    } else if constexpr (ACT == ASCB200_ACT_GELU_TANH) return z * sigmoid(tanh_arg(z));
+    else if constexpr (ACT == ASCB200_ACT_SILU) return z * sigmoid(z);
+    else return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float slope(float z)
+{
+    if constexpr (ACT == ASCB200_ACT_FASTER_GELU) {
+        const float g = sigmoid(1.702f * z);
+        return g * fmaf(1.702f * z, 1.0f - g, 1.0f);
+    } else if constexpr (ACT == ASCB200_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    else if constexpr (ACT == ASCB200_ACT_GELU) {
+        float e;
+        const float tail = normal_tail(z, e);
+        return fmaf(z * 0.3989422804014327f, e, z > 0.0f ? 1.0f - tail : tail);
+    } else if constexpr (ACT == ASCB200_ACT_GELU_TANH) {
+        const float c = fminf(fmaxf(z, -32.0f), 32.0f);
+        const float g = sigmoid(tanh_arg(z));
+        return g * fmaf(kTanh2u * c * fmaf(0.134145f * c, c, 1.0f), 1.0f - g, 1.0f);
+    } else if constexpr (ACT == ASCB200_ACT_SILU) {
+        const float g = sigmoid(z);
+        return g * fmaf(z, 1.0f - g, 1.0f);
+    } else return 1.0f;
+}
+
+// Runs `body` with the activation as a compile-time constant `ACT`: the choice is made once per block of values.
+#define ASCB200_ACT_SWITCH(act, body)                                                                   \
+    switch (act) {                                                                                      \
+        case ASCB200_ACT_FASTER_GELU: { constexpr int ACT = ASCB200_ACT_FASTER_GELU; body } break;      \
+        case ASCB200_ACT_RELU: { constexpr int ACT = ASCB200_ACT_RELU; body } break;                    \
+        case ASCB200_ACT_GELU: { constexpr int ACT = ASCB200_ACT_GELU; body } break;                    \
+        case ASCB200_ACT_GELU_TANH: { constexpr int ACT = ASCB200_ACT_GELU_TANH; body } break;          \
+        case ASCB200_ACT_SILU: { constexpr int ACT = ASCB200_ACT_SILU; body } break;                    \
+        default: break;                                                                                 \
+    }
+
+}  // namespace act
+}  // namespace ascb200

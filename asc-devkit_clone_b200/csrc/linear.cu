@@ -1,0 +1,398 @@
+// Linear layers: matrix product with bias, activation and residual in its output stage, and its gradients.
+//
+//   y = act(z) + residual,   z = x w^T (int8: scaled per token and channel) + bias
+//
+// Many rows run on the tensor-core GEMM kernels with the output stage of a linear layer (gemm_linear.cu).  A few tokens run here:
+// the product then reads every weight once and is memory bound.
+//
+// Gradients: dz = dy * act'(z) and dbias = sum over rows of dz in one pass over dy and z, then dx = dz w and dw = dz^T x as plain GEMMs.
+#include <algorithm>
+
+#include "activation.cuh"
+#include "gemm_host.cuh"
+#include "partial_sum.cuh"
+
+namespace ascb200 {
+namespace {
+
+// ---- a few tokens ----------------------------------------------------------------------------------------------------------
+// The weights' rows are the 16-row operand of mma.sync m16n8 and the tokens its eight columns, so that every weight that comes from
+// memory is used by one instruction for all tokens.  A sum over k does not care for the order of k as long as both operands agree,
+// so a lane feeds the instructions straight from 16 contiguous bytes of a weight row (its first two words are the lane's k slots of
+// one instruction, the last two those of the next): 64 bytes of a row per pair of instructions, no shuffles and no shared memory.
+// A block owns 16 weight rows; its warps take 256-byte pieces of them in turn and add their sums in warp order through shared memory.
+constexpr int kRowsMaxTokens = 16;
+constexpr int kRowsTile = 16;   // weight rows per block
+constexpr int kRowsWarps = 8;
+constexpr int kRowsUnroll = 4;  // 64-byte chunks per warp and step
+
+struct RowsArgs {
+    const uint8_t* x;
+    const uint8_t* w;
+    const float* tok;
+    const float* ch;
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* z;
+    long long ldx, ldw;  // bytes
+    long long ld_residual, ldy, ldz;
+    int m, n, k_bytes;
+    int bias_f32, act;
+};
+
+template <int KIND>
+__device__ __forceinline__ void mma_16x8(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    if constexpr (KIND == ASCB200_KIND_S8) {
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    } else {
+        float* f = reinterpret_cast<float*>(c);
+        if constexpr (KIND == ASCB200_KIND_F16)
+            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                         : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3])
+                         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        else
+            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                         : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3])
+                         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+}
+
+// 16 bytes at `off` of a row of `bytes` bytes; what lies behind its end reads as zero and is not touched.
+template <bool STREAM>
+__device__ __forceinline__ uint4 load_piece(const uint8_t* row, int off, int bytes)
+{
+    uint4 r = make_uint4(0u, 0u, 0u, 0u);
+    if (off + 16 <= bytes) {
+        if constexpr (STREAM)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(row + off));
+        else
+            r = __ldg(reinterpret_cast<const uint4*>(row + off));
+    } else if (off < bytes) {
+        uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 15; ++j)
+            if (off + j < bytes) u[j >> 2] |= static_cast<uint32_t>(__ldg(row + off + j)) << (8 * (j & 3));
+        r = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float as_f32(T v);
+template <>
+__device__ __forceinline__ float as_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float as_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float as_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <int KIND, int NT, typename OT>  // NT: groups of eight tokens
+__global__ void __launch_bounds__(kRowsWarps * 32)
+linear_rows_kernel(const RowsArgs p)
+{
+    __shared__ uint32_t part[kRowsWarps][NT * 8][kRowsTile + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, q = lane & 3;
+    const int n0 = blockIdx.x * kRowsTile;
+    const uint8_t* w0 = p.w + min(n0 + g, p.n - 1) * p.ldw;
+    const uint8_t* w1 = p.w + min(n0 + g + 8, p.n - 1) * p.ldw;
+    grid_dependency_wait();
+    uint32_t acc[NT][4] = {};
+    for (int base = warp * (kRowsUnroll * 64); base < p.k_bytes; base += kRowsWarps * kRowsUnroll * 64) {
+        uint4 a[kRowsUnroll], b[kRowsUnroll], x[NT][kRowsUnroll];
+#pragma unroll
+        for (int u = 0; u < kRowsUnroll; ++u) {
+            const int off = base + u * 64 + q * 16;
+            a[u] = load_piece<true>(w0, off, p.k_bytes);
+            b[u] = load_piece<true>(w1, off, p.k_bytes);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < kRowsUnroll; ++u) {
+                x[t][u] = make_uint4(0u, 0u, 0u, 0u);
+                if (t * 8 + g < p.m) x[t][u] = load_piece<false>(p.x + (t * 8 + g) * p.ldx, base + u * 64 + q * 16, p.k_bytes);
+            }
+#pragma unroll
+        for (int u = 0; u < kRowsUnroll; ++u)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                mma_16x8<KIND>(acc[t], a[u].x, b[u].x, a[u].y, b[u].y, x[t][u].x, x[t][u].y);
+                mma_16x8<KIND>(acc[t], a[u].z, b[u].z, a[u].w, b[u].w, x[t][u].z, x[t][u].w);
+            }
+    }
+    // accumulators: rows g and g + 8, tokens 2 q and 2 q + 1
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[warp][t * 8 + 2 * q + (j & 1)][g + (j >> 1) * 8] = acc[t][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 8 * kRowsTile; i += kRowsWarps * 32) {
+        const int token = i / kRowsTile, col = i % kRowsTile, n = n0 + col;
+        if (token >= p.m || n >= p.n) continue;
+        float f;
+        if constexpr (KIND == ASCB200_KIND_S8) {
+            int s = 0;
+#pragma unroll
+            for (int v = 0; v < kRowsWarps; ++v) s += static_cast<int>(part[v][token][col]);
+            f = static_cast<float>(s) * p.ch[n];
+            if (p.tok) f *= p.tok[token];
+        } else {
+            f = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kRowsWarps; ++v) f += __uint_as_float(part[v][token][col]);
+        }
+        if (p.bias) f += p.bias_f32 ? static_cast<const float*>(p.bias)[n] : as_f32(static_cast<const OT*>(p.bias)[n]);
+        if (p.z) static_cast<OT*>(p.z)[token * p.ldz + n] = rounded<OT>(f);
+        ASCB200_ACT_SWITCH(p.act, { f = act::value<ACT>(f); })
+        if (p.residual) f += as_f32(static_cast<const OT*>(p.residual)[token * p.ld_residual + n]);
+        static_cast<OT*>(p.y)[token * p.ldy + n] = rounded<OT>(f);
+    }
+}
+
+template <int KIND, typename OT>
+int launch_rows_as(const RowsArgs& p, cudaStream_t st)
+{
+    const unsigned grid = static_cast<unsigned>((p.n + kRowsTile - 1) / kRowsTile);
+    if (p.m <= 8) ASCB200_CUDA(launch_pdl(linear_rows_kernel<KIND, 1, OT>, grid, kRowsWarps * 32, 0, st, p));
+    else ASCB200_CUDA(launch_pdl(linear_rows_kernel<KIND, 2, OT>, grid, kRowsWarps * 32, 0, st, p));
+    return ASCB200_OK;
+}
+template <int KIND>
+int launch_rows(const RowsArgs& p, int y_dtype, cudaStream_t st)
+{
+    if (y_dtype == ASCB200_F16) return launch_rows_as<KIND, __half>(p, st);
+    if (y_dtype == ASCB200_BF16) return launch_rows_as<KIND, __nv_bfloat16>(p, st);
+    return launch_rows_as<KIND, float>(p, st);
+}
+
+bool element_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+bool operand_aligned(const void* p, int64_t ld, int bytes) { return aligned_to(p, 16) && (ld * bytes) % 16 == 0; }
+int float_bytes(int dtype) { return dtype == ASCB200_F32 ? 4 : 2; }
+bool is_float_type(int dtype) { return dtype == ASCB200_F32 || dtype == ASCB200_F16 || dtype == ASCB200_BF16; }
+
+int run_linear(const ascb200_linear_desc* desc, cudaStream_t stream)
+{
+    if (!current_state()) return ASCB200_ENODEV;
+    if (!desc) return ASCB200_EINVAL;
+    ascb200_linear_desc d = *desc;
+    if (d.m < 0 || d.n < 0 || d.k <= 0 || d.reserved != 0 || (d.trans_w != 0 && d.trans_w != 1)) return ASCB200_EINVAL;
+    if (d.act < ASCB200_ACT_NONE || d.act > ASCB200_ACT_SILU) return ASCB200_EINVAL;
+    if (d.kind != ASCB200_KIND_F16 && d.kind != ASCB200_KIND_BF16 && d.kind != ASCB200_KIND_S8) return ASCB200_EUNSUPPORTED;
+    const bool s8 = d.kind == ASCB200_KIND_S8;
+    const int own = d.kind == ASCB200_KIND_F16 ? ASCB200_F16 : ASCB200_BF16;
+    if (s8 ? !is_float_type(d.y_dtype) : d.y_dtype != own && d.y_dtype != ASCB200_F32) return ASCB200_EUNSUPPORTED;
+    if (s8 && d.z_dev) return ASCB200_EUNSUPPORTED;
+    if (!s8 && (d.tok_scale_dev || d.ch_scale_dev)) return ASCB200_EINVAL;
+    if (d.bias_dev && d.bias_dtype != ASCB200_F32 && d.bias_dtype != d.y_dtype) return ASCB200_EUNSUPPORTED;
+    if (d.ldx == 0) d.ldx = d.k;
+    if (d.ldw == 0) d.ldw = d.trans_w ? d.k : d.n;
+    if (d.ld_residual == 0) d.ld_residual = d.n;
+    if (d.ldy == 0) d.ldy = d.n;
+    if (d.ldz == 0) d.ldz = d.n;
+    if (d.ldx < d.k || d.ldw < (d.trans_w ? d.k : d.n) || d.ld_residual < d.n || d.ldy < d.n || d.ldz < d.n) return ASCB200_EINVAL;
+    if (d.m == 0 || d.n == 0) return ASCB200_OK;
+    if (!d.x_dev || !d.w_dev || !d.y_dev || (s8 && !d.ch_scale_dev) || d.y_dev == d.z_dev) return ASCB200_EINVAL;
+    const int esz = s8 ? 1 : 2, osz = float_bytes(d.y_dtype);
+    if (!operand_aligned(d.x_dev, d.ldx, esz) || !operand_aligned(d.w_dev, d.ldw, esz)) return ASCB200_EALIGN;
+    if (!element_aligned(d.y_dev, osz) || !element_aligned(d.z_dev, osz) || !element_aligned(d.residual_dev, osz) || !element_aligned(d.tok_scale_dev, 4) ||
+        !element_aligned(d.ch_scale_dev, 4) || (d.bias_dev && !element_aligned(d.bias_dev, float_bytes(d.bias_dtype))))
+        return ASCB200_EALIGN;
+
+    // k * esz has to fit the 32-bit offsets within a row
+    if (d.m <= kRowsMaxTokens && d.trans_w && d.k <= (1 << 29)) {
+        RowsArgs p = {};
+        p.x = static_cast<const uint8_t*>(d.x_dev), p.w = static_cast<const uint8_t*>(d.w_dev), p.tok = d.tok_scale_dev, p.ch = d.ch_scale_dev;
+        p.bias = d.bias_dev, p.residual = d.residual_dev, p.y = d.y_dev, p.z = d.z_dev;
+        p.ldx = d.ldx * esz, p.ldw = d.ldw * esz, p.ld_residual = d.ld_residual, p.ldy = d.ldy, p.ldz = d.ldz;
+        p.m = d.m, p.n = d.n, p.k_bytes = d.k * esz, p.bias_f32 = d.bias_dtype == ASCB200_F32, p.act = d.act;
+        if (s8) return launch_rows<ASCB200_KIND_S8>(p, d.y_dtype, stream);
+        if (d.kind == ASCB200_KIND_F16) return launch_rows<ASCB200_KIND_F16>(p, d.y_dtype, stream);
+        return launch_rows<ASCB200_KIND_BF16>(p, d.y_dtype, stream);
+    }
+
+    ascb200_gemm_desc q = {};
+    q.kind = d.kind, q.m = d.m, q.n = d.n, q.k = d.k;
+    q.a_dev = d.x_dev, q.lda = d.ldx, q.b_dev = d.w_dev, q.ldb = d.ldw, q.trans_b = d.trans_w;
+    q.c_dev = d.y_dev, q.ldc = d.ldy, q.c_dtype = d.y_dtype;
+    q.c2_dev = d.z_dev, q.ldc2 = d.ldz, q.c2_dtype = d.y_dtype;
+    q.epilogue = s8 ? ASCB200_EPI_DEQUANT_TOKEN_CHANNEL : ASCB200_EPI_CAST;
+    q.tok_scale_dev = d.tok_scale_dev, q.ch_scale_dev = d.ch_scale_dev;
+    const gemm::LinearArgs lin = {d.bias_dev, d.bias_dtype == ASCB200_F32, d.act, d.residual_dev, d.ld_residual};
+    return gemm::run_gemm(&q, nullptr, 0, stream, nullptr, &lin);
+}
+
+// ---- gradients --------------------------------------------------------------------------------------------------------------
+// dz = dy * act'(z), rounded to the operands' type for the two products that follow (the rounding that any 16-bit product of it
+// needs); dbias from the fp32 values before that rounding.  A thread owns eight columns and walks down rows; memory bound.
+struct ActGradArgs {
+    const void* dy;
+    const void* z;
+    void* dz;
+    float* partial;  // [row blocks][n], or nullptr
+    long long ld_dy, ldz, ld_dz;
+    int m, n, act;
+    int vec;         // dy and z allow 16-byte loads
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int col, int n, bool vec, float (&f)[8])
+{
+    if (vec && col + 8 <= n) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + col));
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = as_f32(e[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = col + j < n ? as_f32(row[col + j]) : 0.0f;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+act_grad_kernel(const ActGradArgs p)
+{
+    __shared__ float part[8][256];
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int col = blockIdx.x * 256 + lane * 8;
+    float acc[8] = {};
+    if (col < p.n) {
+        for (long long row = static_cast<long long>(blockIdx.y) * 8 + warp; row < p.m; row += static_cast<long long>(gridDim.y) * 8) {
+            float dy[8];
+            load8(static_cast<const T*>(p.dy) + row * p.ld_dy, col, p.n, p.vec, dy);
+            if (p.act != ASCB200_ACT_NONE) {
+                float z[8];
+                load8(static_cast<const T*>(p.z) + row * p.ldz, col, p.n, p.vec, z);
+                ASCB200_ACT_SWITCH(p.act, {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dy[j] *= act::slope<ACT>(z[j]);
+                })
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += dy[j];
+            if (p.dz) {  // rows of dz are 16-byte aligned and have room for whole chunks; columns past n become zero
+                T out[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) out[j] = rounded<T>(dy[j]);
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.dz) + row * p.ld_dz + col) = *reinterpret_cast<const uint4*>(out);
+            }
+        }
+    }
+    if (!p.partial) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[warp][lane * 8 + j] = acc[j];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < p.n) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += part[i][threadIdx.x];
+        p.partial[static_cast<size_t>(blockIdx.y) * p.n + c] = v;
+    }
+}
+
+constexpr int kActGradBlocks = 592;  // blocks to aim for: four per SM
+int act_grad_row_blocks(int m, int n)
+{
+    const int cols = (n + 255) / 256;
+    return static_cast<int>(std::min<long long>((m + 7ll) / 8, std::max(1, std::min(296, kActGradBlocks / cols))));
+}
+size_t dz_bytes(int m, int n) { return (static_cast<size_t>(m) * ((static_cast<size_t>(n) + 7) / 8 * 8) * 2 + 255) / 256 * 256; }
+size_t linear_grad_workspace(int m, int n)
+{
+    return m <= 0 || n <= 0 ? 0 : dz_bytes(m, n) + static_cast<size_t>(act_grad_row_blocks(m, n)) * n * sizeof(float);
+}
+
+int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
+{
+    if (!current_state()) return ASCB200_ENODEV;
+    if (!desc) return ASCB200_EINVAL;
+    ascb200_linear_grad_desc d = *desc;
+    if (d.m < 0 || d.n <= 0 || d.k <= 0 || (d.trans_w != 0 && d.trans_w != 1)) return ASCB200_EINVAL;
+    if (d.act < ASCB200_ACT_NONE || d.act > ASCB200_ACT_SILU) return ASCB200_EINVAL;
+    if (d.kind != ASCB200_KIND_F16 && d.kind != ASCB200_KIND_BF16) return ASCB200_EUNSUPPORTED;
+    const int own = d.kind == ASCB200_KIND_F16 ? ASCB200_F16 : ASCB200_BF16;
+    if (d.dw_dev && d.dw_dtype != own && d.dw_dtype != ASCB200_F32) return ASCB200_EUNSUPPORTED;
+    if (d.dbias_dev && d.dbias_dtype != own && d.dbias_dtype != ASCB200_F32) return ASCB200_EUNSUPPORTED;
+    const int w_cols = d.trans_w ? d.k : d.n, w_rows = d.trans_w ? d.n : d.k;
+    if (d.ld_dy == 0) d.ld_dy = d.n;
+    if (d.ldz == 0) d.ldz = d.n;
+    if (d.ldx == 0) d.ldx = d.k;
+    if (d.ldw == 0) d.ldw = w_cols;
+    if (d.ld_dx == 0) d.ld_dx = d.k;
+    if (d.ld_dw == 0) d.ld_dw = w_cols;
+    if (d.ld_dy < d.n || d.ldz < d.n || d.ldx < d.k || d.ldw < w_cols || d.ld_dx < d.k || d.ld_dw < w_cols) return ASCB200_EINVAL;
+    const int dwsz = float_bytes(d.dw_dtype), dbsz = float_bytes(d.dbias_dtype);
+    if ((d.dw_dev && !element_aligned(d.dw_dev, dwsz)) || (d.dbias_dev && !element_aligned(d.dbias_dev, dbsz))) return ASCB200_EALIGN;
+    if (d.m == 0) {  // no rows: dw and dbias are sums of nothing
+        if (d.dw_dev) ASCB200_CUDA(cudaMemset2DAsync(d.dw_dev, static_cast<size_t>(d.ld_dw) * dwsz, 0, static_cast<size_t>(w_cols) * dwsz, w_rows, stream));
+        if (d.dbias_dev) ASCB200_CUDA(cudaMemsetAsync(d.dbias_dev, 0, static_cast<size_t>(d.n) * dbsz, stream));
+        return ASCB200_OK;
+    }
+    if (!d.dy_dev || (d.act != ASCB200_ACT_NONE && !d.z_dev) || (d.dx_dev && !d.w_dev) || (d.dw_dev && !d.x_dev)) return ASCB200_EINVAL;
+    if (!element_aligned(d.dy_dev, 2) || !element_aligned(d.z_dev, 2) || !element_aligned(d.dx_dev, 2)) return ASCB200_EALIGN;
+    if ((d.dx_dev && !operand_aligned(d.w_dev, d.ldw, 2)) || (d.dw_dev && !operand_aligned(d.x_dev, d.ldx, 2))) return ASCB200_EALIGN;
+
+    const bool products = d.dx_dev || d.dw_dev;
+    // dy itself is the operand where there is no activation and it can be one
+    const bool make_dz = products && (d.act != ASCB200_ACT_NONE || !operand_aligned(d.dy_dev, d.ld_dy, 2));
+    const void* dz = d.dy_dev;
+    int64_t ld_dz = d.ld_dy;
+    if (make_dz || d.dbias_dev) {
+        if (!d.workspace_dev || d.workspace_bytes < linear_grad_workspace(d.m, d.n)) return ASCB200_EINVAL;
+        if (!aligned_to(d.workspace_dev, 256)) return ASCB200_EALIGN;
+        ActGradArgs p = {};
+        p.dy = d.dy_dev, p.z = d.z_dev, p.ld_dy = d.ld_dy, p.ldz = d.ldz, p.m = d.m, p.n = d.n, p.act = d.act;
+        if (make_dz) {
+            dz = p.dz = d.workspace_dev;
+            ld_dz = p.ld_dz = (static_cast<int64_t>(d.n) + 7) / 8 * 8;
+        }
+        if (d.dbias_dev) p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(d.workspace_dev) + dz_bytes(d.m, d.n));
+        p.vec = operand_aligned(d.dy_dev, d.ld_dy, 2) && (d.act == ASCB200_ACT_NONE || operand_aligned(d.z_dev, d.ldz, 2));
+        const int rows = act_grad_row_blocks(d.m, d.n);
+        const dim3 grid((d.n + 255) / 256, rows);
+        if (d.kind == ASCB200_KIND_F16) ASCB200_CUDA(launch_pdl(act_grad_kernel<__half>, grid, 256, 0, stream, p));
+        else ASCB200_CUDA(launch_pdl(act_grad_kernel<__nv_bfloat16>, grid, 256, 0, stream, p));
+        if (d.dbias_dev) {
+            const int rc = sum_partials(p.partial, d.dbias_dev, d.dbias_dtype, rows, d.n, stream);
+            if (rc != ASCB200_OK) return rc;
+        }
+    }
+    if (d.dx_dev) {  // [m, k] = dz [m, n] * w
+        ascb200_gemm_desc q = {};
+        q.kind = d.kind, q.m = d.m, q.n = d.k, q.k = d.n;
+        q.a_dev = dz, q.lda = ld_dz, q.b_dev = d.w_dev, q.ldb = d.ldw, q.trans_b = !d.trans_w;
+        q.c_dev = d.dx_dev, q.ldc = d.ld_dx, q.c_dtype = own;
+        const int rc = gemm::run_gemm(&q, nullptr, 0, stream);
+        if (rc != ASCB200_OK) return rc;
+    }
+    if (d.dw_dev) {  // [n, k] = dz^T x, or [k, n] = x^T dz
+        ascb200_gemm_desc q = {};
+        q.kind = d.kind, q.m = w_rows, q.n = w_cols, q.k = d.m, q.trans_a = 1;
+        q.a_dev = d.trans_w ? dz : d.x_dev, q.lda = d.trans_w ? ld_dz : d.ldx;
+        q.b_dev = d.trans_w ? d.x_dev : dz, q.ldb = d.trans_w ? d.ldx : ld_dz;
+        q.c_dev = d.dw_dev, q.ldc = d.ld_dw, q.c_dtype = d.dw_dtype;
+        const int rc = gemm::run_gemm(&q, nullptr, 0, stream);
+        if (rc != ASCB200_OK) return rc;
+    }
+    return ASCB200_OK;
+}
+
+}  // namespace
+}  // namespace ascb200
+
+extern "C" {
+
+int ascb200_linear(const ascb200_linear_desc* desc, void* stream) { return ascb200::run_linear(desc, static_cast<cudaStream_t>(stream)); }
+
+size_t ascb200_linear_grad_workspace_bytes(int32_t m, int32_t n) { return ascb200::linear_grad_workspace(m, n); }
+
+int ascb200_linear_grad(const ascb200_linear_grad_desc* desc, void* stream) { return ascb200::run_linear_grad(desc, static_cast<cudaStream_t>(stream)); }
+
+}  // extern "C"

@@ -12,7 +12,7 @@
 // partial sums go through the caller's workspace and are added in block order (no atomics: the result does not depend on timing).
 #include <algorithm>
 
-#include "common.cuh"
+#include "partial_sum.cuh"
 
 namespace ascb200 {
 namespace {
@@ -568,29 +568,6 @@ rms_norm_grad_kernel(const NormGradArgs p)
     }
 }
 
-// dgamma[col] = sum over the blocks' partial sums, in block order per thread and then over the eight warps in order.
-template <typename G>
-__global__ void __launch_bounds__(256)
-rms_norm_dgamma_kernel(const float* __restrict__ partial, G* __restrict__ dgamma, int blocks, int k)
-{
-    __shared__ float part[8][32];
-    grid_dependency_wait();
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
-    float v = 0.0f;
-    if (col < k) {
-#pragma unroll 8
-        for (int b = w; b < blocks; b += 8) v += partial[static_cast<size_t>(b) * k + col];
-    }
-    part[w][lane] = v;
-    __syncthreads();
-    if (w == 0 && col < k) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) v += part[i][lane];
-        if constexpr (sizeof(G) == 4) dgamma[col] = v;
-        else reinterpret_cast<uint16_t*>(dgamma)[col] = static_cast<uint16_t>(pack2(v, 0.0f, G()) & 0xFFFFu);
-    }
-}
-
 template <typename T, int TPR, int NCHUNK, bool VEC>
 int launch_norm_grad_as(const NormGradArgs& p, int sms, cudaStream_t st, int* blocks)
 {
@@ -658,14 +635,7 @@ int run_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, cudaStream_t strea
         default: rc = vec ? launch_norm_grad<float, true>(p, sms, stream, &blocks) : launch_norm_grad<float, false>(p, sms, stream, &blocks);
     }
     if (rc != ASCB200_OK || !d.dgamma_dev) return rc;
-    const int grid = (d.k + 31) / 32;
-    if (d.dgamma_dtype == ASCB200_F32)
-        ASCB200_CUDA(launch_pdl(rms_norm_dgamma_kernel<float>, grid, 256, 0, stream, p.partial, static_cast<float*>(d.dgamma_dev), blocks, d.k));
-    else if (d.dgamma_dtype == ASCB200_F16)
-        ASCB200_CUDA(launch_pdl(rms_norm_dgamma_kernel<__half>, grid, 256, 0, stream, p.partial, static_cast<__half*>(d.dgamma_dev), blocks, d.k));
-    else
-        ASCB200_CUDA(launch_pdl(rms_norm_dgamma_kernel<__nv_bfloat16>, grid, 256, 0, stream, p.partial, static_cast<__nv_bfloat16*>(d.dgamma_dev), blocks, d.k));
-    return ASCB200_OK;
+    return sum_partials(p.partial, d.dgamma_dev, d.dgamma_dtype, blocks, d.k, stream);
 }
 
 }  // namespace

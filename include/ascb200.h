@@ -503,6 +503,73 @@ typedef struct ascb200_rms_norm_grad_desc {
 ASCB200_API size_t ascb200_rms_norm_grad_workspace_bytes(int32_t m, int32_t k);
 ASCB200_API int ascb200_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, void* stream);
 
+/* Activations of a linear layer: FASTER_GELU x / (1 + e^(-1.702 x)) (act = 1 of ascb200_gemm_desc); GELU x Phi(x); GELU_TANH its tanh form;
+ * SILU x / (1 + e^-x). */
+enum { ASCB200_ACT_NONE = 0, ASCB200_ACT_FASTER_GELU = 1, ASCB200_ACT_RELU = 2, ASCB200_ACT_GELU = 3, ASCB200_ACT_GELU_TANH = 4, ASCB200_ACT_SILU = 5 };
+
+/* A linear layer, with everything behind the product in its output stage:
+ *   z = x w^T + bias,  y = act(z) + residual                     F16 / BF16 operands, fp32 accumulation
+ *   z = (x w^T) * ch_scale[n] * tok_scale[m] + bias              S8 operands, int32 accumulation
+ * x [m, k]; w [n, k] (trans_w = 1) or [k, n] (trans_w = 0); z is kept in fp32 and rounded only where it is written (z_dev, for the gradients;
+ * F16 / BF16 operands).  y (and z, residual): the operands' type or F32; F32 / F16 / BF16 for S8.  bias [n]: F32 or y's type.
+ * F16 outputs saturate at +-65504.  x and w as for ascb200_gemm: 16-byte aligned, leading dimensions a multiple of 16 bytes (k and n of
+ * any size); the other tensors whole elements, fastest with rows on 16 bytes.  k >= 1.  y may be the residual itself (same leading dimension).
+ * Up to 16 rows with trans_w = 1 run a kernel that streams the weights once (a token at a time, or a few); the others the GEMM kernels.
+ * The order of the fp32 sums depends on which, and within each on the sizes alone. */
+typedef struct ascb200_linear_desc {
+    int32_t kind;               /* ASCB200_KIND_F16 / BF16 / S8 */
+    int32_t m, n, k;
+    const void* x_dev;
+    int64_t ldx;
+    const void* w_dev;
+    int64_t ldw;
+    int32_t trans_w;
+    int32_t act;                /* ASCB200_ACT_* */
+    const float* tok_scale_dev; /* S8: [m] or NULL (1) */
+    const float* ch_scale_dev;  /* S8: [n] */
+    const void* bias_dev;       /* [n] or NULL */
+    int32_t bias_dtype;
+    int32_t y_dtype;
+    const void* residual_dev;   /* [m, n] or NULL */
+    int64_t ld_residual;
+    void* y_dev;                /* [m, n] */
+    int64_t ldy;
+    void* z_dev;                /* [m, n] of y's type, or NULL */
+    int64_t ldz;
+    int64_t reserved;           /* must be zero */
+} ascb200_linear_desc;
+ASCB200_API int ascb200_linear(const ascb200_linear_desc* desc, void* stream);
+
+/* Its gradients, F16 / BF16 (the residual's is dy):
+ *   dz = dy * act'(z);  dbias = sum over rows of dz;  dx = dz w;  dw = dz^T x ([n, k], or [k, n] with trans_w = 0).
+ * z as the forward call wrote it in the operands' type (not read for ACT_NONE).  dz is rounded to the operands' type for the two products, dbias
+ * is summed in fp32 from the values before.  dx, dw and dbias may each be NULL (not wanted); dw and dbias: the operands' type or F32.
+ * The workspace (256-byte aligned) holds dz and the partial sums of dbias; without activation and dbias it is not needed when dy is
+ * aligned like x.  m = 0 gives dw = 0 and dbias = 0. */
+typedef struct ascb200_linear_grad_desc {
+    int32_t kind;
+    int32_t m, n, k;
+    int32_t act, trans_w;
+    const void* dy_dev;         /* [m, n] */
+    int64_t ld_dy;
+    const void* z_dev;          /* [m, n] */
+    int64_t ldz;
+    const void* x_dev;
+    int64_t ldx;
+    const void* w_dev;
+    int64_t ldw;
+    void* dx_dev;               /* [m, k] */
+    int64_t ld_dx;
+    void* dw_dev;
+    int64_t ld_dw;
+    void* dbias_dev;            /* [n] */
+    int32_t dw_dtype, dbias_dtype;
+    void* workspace_dev;
+    size_t workspace_bytes;
+} ascb200_linear_grad_desc;
+ASCB200_API size_t ascb200_linear_grad_workspace_bytes(int32_t m, int32_t n);
+ASCB200_API int ascb200_linear_grad(const ascb200_linear_grad_desc* desc, void* stream);
+
 /* Routing of tokens to experts, in front of ascb200_grouped_gemm:
  *   p = softmax over the unmasked experts of a token's logits (a logit of -inf masks its expert);
  *   idx[t, :] = the top_k experts of the largest logits, largest first, of equal ones the lower index first;
