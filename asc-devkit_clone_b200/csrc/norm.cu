@@ -41,23 +41,33 @@ __device__ __forceinline__ uint4 ld_v4(const void* p)
     return r;
 }
 
-// Chunk c (elements 8 c .. 8 c + 7) of a row of k elements; elements past the row's end read as zero and are not touched.
-// VEC: rows start on 16 bytes.
+// A thread's i-th eight columns.  VEC (every row of every tensor starts on 16 bytes): neighbours, starting at `first_column`.  Else: 32
+// columns apart, so that a warp's accesses of one element each are contiguous whatever the alignment (fp32 1000 x 1111: 16.6 us with
+// neighbouring columns, see the figures at the kernels).  Either way a warp owns 256 contiguous columns.
+template <bool VEC>
+constexpr int kColumnStep = VEC ? 1 : 32;
+template <int TPR, bool VEC>
+__device__ __forceinline__ int first_column(int t, int i)
+{
+    return VEC ? (t + i * TPR) * 8 : (i * TPR + (t & ~31)) * 8 + (t & 31);
+}
+
+// The eight elements at column c; elements past the row's end read as zero and are not touched.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_chunk(const T* row, int c, int k, Raw8<T>& r)
 {
-    if (VEC && c * 8 + 8 <= k) {
-        r.v = ld_v4(row + c * 8);
-        if constexpr (sizeof(T) == 4) r.w = ld_v4(row + c * 8 + 4);
+    if (VEC && c + 8 <= k) {
+        r.v = ld_v4(row + c);
+        if constexpr (sizeof(T) == 4) r.w = ld_v4(row + c + 4);
         return;
     }
     uint32_t u[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         u[j] = 0u;
-        if (c * 8 + j < k) {
-            if constexpr (sizeof(T) == 4) u[j] = *reinterpret_cast<const uint32_t*>(row + c * 8 + j);
-            else u[j] = *reinterpret_cast<const uint16_t*>(row + c * 8 + j);
+        if (c + j * kColumnStep<VEC> < k) {
+            if constexpr (sizeof(T) == 4) u[j] = *reinterpret_cast<const volatile uint32_t*>(row + c + j * kColumnStep<VEC>);
+            else u[j] = *reinterpret_cast<const volatile uint16_t*>(row + c + j * kColumnStep<VEC>);
         }
     }
     if constexpr (sizeof(T) == 4) {
@@ -103,23 +113,23 @@ template <typename T, bool VEC>
 __device__ __forceinline__ void store_chunk(T* row, int c, int k, const float (&f)[8])
 {
     if constexpr (sizeof(T) == 4) {
-        if (VEC && c * 8 + 8 <= k) {
-            *reinterpret_cast<float4*>(row + c * 8) = make_float4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float4*>(row + c * 8 + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        if (VEC && c + 8 <= k) {
+            *reinterpret_cast<float4*>(row + c) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(row + c + 4) = make_float4(f[4], f[5], f[6], f[7]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c * 8 + j < k) row[c * 8 + j] = f[j];
+                if (c + j * kColumnStep<VEC> < k) row[c + j * kColumnStep<VEC>] = f[j];
         }
     } else {
         const uint4 v = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
-        if (VEC && c * 8 + 8 <= k) {
-            *reinterpret_cast<uint4*>(row + c * 8) = v;
+        if (VEC && c + 8 <= k) {
+            *reinterpret_cast<uint4*>(row + c) = v;
         } else {
             const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c * 8 + j < k) reinterpret_cast<uint16_t*>(row)[c * 8 + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+                if (c + j * kColumnStep<VEC> < k) reinterpret_cast<uint16_t*>(row)[c + j * kColumnStep<VEC>] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
         }
     }
 }
@@ -130,24 +140,20 @@ __device__ __forceinline__ void load_gamma(const void* __restrict__ gamma, int g
     if (!gamma) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = 1.0f;
-    } else if (gamma_f32) {
-        if (VEC && c * 8 + 8 <= k) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(gamma) + 2 * c), b = __ldg(reinterpret_cast<const float4*>(gamma) + 2 * c + 1);
+    } else if (sizeof(T) == 4 || gamma_f32) {
+        const float* src = static_cast<const float*>(gamma) + c;
+        if (VEC && c + 8 <= k) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
             g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, g[4] = b.x, g[5] = b.y, g[6] = b.z, g[7] = b.w;
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = c * 8 + j < k ? __ldg(static_cast<const float*>(gamma) + c * 8 + j) : 0.0f;
+            for (int j = 0; j < 8; ++j) g[j] = c + j * kColumnStep<VEC> < k ? __ldg(src + j * kColumnStep<VEC>) : 0.0f;
         }
     } else {
-        if (VEC && sizeof(T) == 2 && c * 8 + 8 <= k) {
-            Raw8<T> r;
-            r.v = __ldg(reinterpret_cast<const uint4*>(gamma) + c);
-            unpack8(r, g);
-        } else {
-            Raw8<T> r;
-            load_chunk<T, false>(static_cast<const T*>(gamma), c, k, r);
-            unpack8(r, g);
-        }
+        Raw8<T> r;
+        if (VEC && c + 8 <= k) r.v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(gamma) + c));
+        else load_chunk<T, VEC>(static_cast<const T*>(gamma), c, k, r);
+        unpack8(r, g);
     }
 }
 
@@ -158,30 +164,27 @@ __device__ __forceinline__ float max_nan(float a, float b)  // a NaN stays
     return r;
 }
 
-// Sum and maximum over the TPR threads of a row; `red` holds one entry per warp and is not used again before the next barrier.
+// Largest of a warp's non-negative floats: their bit patterns are in the same order, and a NaN's is above infinity's.
+__device__ __forceinline__ float warp_max_abs(float v) { return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v))); }
+
+// Sum and (of non-negative values) maximum over the TPR threads of a row; `red` holds one entry per warp and is not used again before
+// the next barrier.
 template <int TPR>
 __device__ __forceinline__ void row_reduce(float& s, float& mx, float2* red)
 {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-    }
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    mx = warp_max_abs(mx);
     if constexpr (TPR > 32) {
-        constexpr int W = TPR / 32;
+        constexpr int W = TPR / 32;  // a power of two
         const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
         if (l == 0) red[w] = make_float2(s, mx);
         __syncthreads();
-        const float2 v = l < W ? red[l] : make_float2(0.0f, 0.0f);
-        s = v.x, mx = v.y;
+        const float2 v = red[l & (W - 1)];
+        s = v.x;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            if (o >= W) continue;  // W is a power of two
-            s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-            mx = max_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-        }
-        s = __shfl_sync(0xFFFFFFFFu, s, 0);
-        mx = __shfl_sync(0xFFFFFFFFu, mx, 0);
+        for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        mx = warp_max_abs(v.y);
     }
 }
 
@@ -241,24 +244,24 @@ __device__ __forceinline__ uint32_t e4m3x2_of(float a, float b)
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(v) : "f"(b), "f"(a));
     return v;
 }
-// Eight codes of y = f * mul.
+// Eight codes: y times the reciprocal of its scale.
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8, const float (&y)[8], float mul)
+__device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8, const float (&y)[8], const float (&mul)[8])
 {
     uint32_t a, b;
     if (s8) {
-        a = s8_of(y[0] * mul) | (s8_of(y[1] * mul) << 8) | (s8_of(y[2] * mul) << 16) | (s8_of(y[3] * mul) << 24);
-        b = s8_of(y[4] * mul) | (s8_of(y[5] * mul) << 8) | (s8_of(y[6] * mul) << 16) | (s8_of(y[7] * mul) << 24);
+        a = s8_of(y[0] * mul[0]) | (s8_of(y[1] * mul[1]) << 8) | (s8_of(y[2] * mul[2]) << 16) | (s8_of(y[3] * mul[3]) << 24);
+        b = s8_of(y[4] * mul[4]) | (s8_of(y[5] * mul[5]) << 8) | (s8_of(y[6] * mul[6]) << 16) | (s8_of(y[7] * mul[7]) << 24);
     } else {
-        a = e4m3x2_of(y[0] * mul, y[1] * mul) | (e4m3x2_of(y[2] * mul, y[3] * mul) << 16);
-        b = e4m3x2_of(y[4] * mul, y[5] * mul) | (e4m3x2_of(y[6] * mul, y[7] * mul) << 16);
+        a = e4m3x2_of(y[0] * mul[0], y[1] * mul[1]) | (e4m3x2_of(y[2] * mul[2], y[3] * mul[3]) << 16);
+        b = e4m3x2_of(y[4] * mul[4], y[5] * mul[5]) | (e4m3x2_of(y[6] * mul[6], y[7] * mul[7]) << 16);
     }
-    if (VEC && c * 8 + 8 <= k) {
-        *reinterpret_cast<uint2*>(row + c * 8) = make_uint2(a, b);
+    if (VEC && c + 8 <= k) {
+        *reinterpret_cast<uint2*>(row + c) = make_uint2(a, b);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (c * 8 + j < k) row[c * 8 + j] = static_cast<uint8_t>((j < 4 ? a : b) >> (8 * (j & 3)));
+            if (c + j * kColumnStep<VEC> < k) row[c + j * kColumnStep<VEC>] = static_cast<uint8_t>((j < 4 ? a : b) >> (8 * (j & 3)));
     }
 }
 
@@ -278,8 +281,8 @@ rms_norm_kernel(const NormArgs p)
     Raw8<T> xr[NCHUNK], rr[NCHUNK];
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = t + i * TPR;
-        if (c * 8 < k) {
+        const int c = first_column<TPR, VEC>(t, i);
+        if (c < k) {
             load_chunk<T, VEC>(x, c, k, xr[i]);
             if (r) load_chunk<T, VEC>(r, c, k, rr[i]);
         }
@@ -288,8 +291,8 @@ rms_norm_kernel(const NormArgs p)
     float ss = 0.0f, amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = t + i * TPR;
-        if (c * 8 < k) {
+        const int c = first_column<TPR, VEC>(t, i);
+        if (c < k) {
             float g[8];
             unpack8(xr[i], hg[i]);
             if (r) {
@@ -318,8 +321,8 @@ rms_norm_kernel(const NormArgs p)
         T* y = static_cast<T*>(p.y) + row * p.ldy;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = t + i * TPR;
-            if (c * 8 < k) {
+            const int c = first_column<TPR, VEC>(t, i);
+            if (c < k) {
                 float v[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = hg[i][j] * rstd;
@@ -338,29 +341,50 @@ rms_norm_kernel(const NormArgs p)
     }
     const int lanes = p.group_lanes;
     const long long groups = (k + lanes * 8 - 1) / (lanes * 8);
+    auto scale_group = [&](float g, int column, bool writes) {  // the group's largest magnitude -> its scale, stored, and the reciprocal
+        float r;
+        if (p.scale_mode == ASCB200_SCALE_MX) {
+            const uint32_t byte = mx_scale_byte(g, r);
+            if (writes) static_cast<uint8_t*>(p.scale)[row * groups + column / (lanes * 8)] = static_cast<uint8_t>(byte);
+        } else {
+            float scale;
+            scale_of(g, s8, scale, r);
+            if (writes) static_cast<float*>(p.scale)[row * groups + column / (lanes * 8)] = scale;
+        }
+        return r;
+    };
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = t + i * TPR;
-        float y[8];
+        const int c = first_column<TPR, VEC>(t, i);
+        float y[8], mul[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = hg[i][j] * rstd;
+        for (int j = 0; j < 8; ++j) y[j] = hg[i][j] * rstd, mul[j] = inv;
         if (p.scale_mode != ASCB200_SCALE_PER_TOKEN) {
-            // a group is `lanes` neighbouring lanes: the whole warp takes part, lanes past the row's end with zeros
-            float g = 0.0f;
+            // the whole warp takes part in a group's maximum, columns past the row's end with zeros
+            if constexpr (VEC) {  // a group is `lanes` neighbouring lanes
+                float g = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g = max_nan(g, fabsf(y[j]));
-            for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-            const bool first = (c & (lanes - 1)) == 0 && c * 8 < k;
-            if (p.scale_mode == ASCB200_SCALE_MX) {
-                const uint32_t byte = mx_scale_byte(g, inv);
-                if (first) static_cast<uint8_t*>(p.scale)[row * groups + c / lanes] = static_cast<uint8_t>(byte);
-            } else {
-                float scale;
-                scale_of(g, s8, scale, inv);
-                if (first) static_cast<float*>(p.scale)[row * groups + c / lanes] = scale;
+                for (int j = 0; j < 8; ++j) g = max_nan(g, fabsf(y[j]));
+                for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+                const float r = scale_group(g, c, (c / 8 & (lanes - 1)) == 0 && c < k);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mul[j] = r;
+            } else {  // a group is one, two, four or eight of the warp's 32-column runs
+                float g[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] = warp_max_abs(fabsf(y[j]));
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) {
+                    if (o * 4 >= lanes) break;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (!(j & o)) g[j] = g[j ^ o] = max_nan(g[j], g[j ^ o]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mul[j] = scale_group(g[j], c + j * 32, (t & 31) == 0 && (j * 4 & (lanes - 1)) == 0 && c + j * 32 < k);
             }
         }
-        if (c * 8 < k) store_codes<VEC>(q, c, k, s8, y, inv);
+        if (c < k) store_codes<VEC>(q, c, k, s8, y, mul);
     }
 }
 
@@ -471,12 +495,35 @@ struct NormGradArgs {
 
 constexpr int kMaxGradBlocks = 296;  // rows of the workspace
 
-// TPR threads per row as above; a block holds ROWS rows at a time (blocks of 256 threads for warp rows).
+template <typename T, int NCHUNK>
+struct GradRow {
+    Raw8<T> dy[NCHUNK], h[NCHUNK], dh[NCHUNK];
+    float rstd;
+};
+template <typename T, int TPR, int NCHUNK, bool VEC>
+__device__ __forceinline__ void load_grad_row(const NormGradArgs& p, long long row, int t, GradRow<T, NCHUNK>& r)
+{
+    if (row >= p.m) return;
+    r.rstd = __ldg(p.rstd + row);
+#pragma unroll
+    for (int i = 0; i < NCHUNK; ++i) {
+        const int c = first_column<TPR, VEC>(t, i);
+        if (c < p.k) {
+            load_chunk<T, VEC>(static_cast<const T*>(p.dy) + row * p.ld_dy, c, p.k, r.dy[i]);
+            load_chunk<T, VEC>(static_cast<const T*>(p.h) + row * p.ldh, c, p.k, r.h[i]);
+            if (p.dh) load_chunk<T, VEC>(static_cast<const T*>(p.dh) + row * p.ld_dh, c, p.k, r.dh[i]);
+        }
+    }
+}
+
+// TPR threads per row as above; a block holds ROWS rows at a time (blocks of 256 threads for warp rows).  Where registers allow, the next
+// row is requested before the current one is worked on.
 template <typename T, int TPR, int NCHUNK, bool VEC>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 256)
 rms_norm_grad_kernel(const NormGradArgs p)
 {
     constexpr int ROWS = TPR > 32 ? 1 : 8;
+    constexpr bool AHEAD = NCHUNK * sizeof(T) <= 8;
     __shared__ float2 red[2][32];
     extern __shared__ float warp_acc[];  // warp rows: [8][TPR * NCHUNK * 8]
     grid_dependency_wait();
@@ -490,28 +537,26 @@ rms_norm_grad_kernel(const NormGradArgs p)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
     int parity = 0;
-    for (long long row = static_cast<long long>(blockIdx.x) * ROWS + sub; row < p.m; row += gridDim.x * ROWS, parity ^= 1) {
-        const T* dy = static_cast<const T*>(p.dy) + row * p.ld_dy;
-        const T* h = static_cast<const T*>(p.h) + row * p.ldh;
-        const float rstd = __ldg(p.rstd + row);
-        Raw8<T> dr[NCHUNK], hr[NCHUNK], er[NCHUNK];
-#pragma unroll
-        for (int i = 0; i < NCHUNK; ++i) {
-            const int c = t + i * TPR;
-            if (c * 8 < k) {
-                load_chunk<T, VEC>(dy, c, k, dr[i]);
-                load_chunk<T, VEC>(h, c, k, hr[i]);
-                if (p.dh) load_chunk<T, VEC>(static_cast<const T*>(p.dh) + row * p.ld_dh, c, k, er[i]);
-            }
+    const long long step = static_cast<long long>(gridDim.x) * ROWS;
+    long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
+    GradRow<T, NCHUNK> r, next;
+    if constexpr (AHEAD) load_grad_row<T, TPR, NCHUNK, VEC>(p, row, t, next);
+    for (; row < p.m; row += step, parity ^= 1) {
+        if constexpr (AHEAD) {
+            r = next;
+            load_grad_row<T, TPR, NCHUNK, VEC>(p, row + step, t, next);
+        } else {
+            load_grad_row<T, TPR, NCHUNK, VEC>(p, row, t, r);
         }
+        const float rstd = r.rstd;
         float dot = 0.0f, none = 0.0f;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = t + i * TPR;
-            if (c * 8 < k) {
+            const int c = first_column<TPR, VEC>(t, i);
+            if (c < k) {
                 float a[8], b[8], g[8];
-                unpack8(dr[i], a);
-                unpack8(hr[i], b);
+                unpack8(r.dy[i], a);
+                unpack8(r.h[i], b);
                 load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -526,13 +571,13 @@ rms_norm_grad_kernel(const NormGradArgs p)
         T* dx = static_cast<T*>(p.dx) + row * p.ld_dx;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = t + i * TPR;
-            if (c * 8 < k) {
+            const int c = first_column<TPR, VEC>(t, i);
+            if (c < k) {
                 float a[8], b[8], g[8], e[8];
-                unpack8(dr[i], a);
-                unpack8(hr[i], b);
+                unpack8(r.dy[i], a);
+                unpack8(r.h[i], b);
                 load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
-                if (p.dh) unpack8(er[i], e);
+                if (p.dh) unpack8(r.dh[i], e);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float v = rstd * (a[j] * g[j] - (b[j] * rstd) * mean);
@@ -549,7 +594,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int col = (t + i * TPR) * 8 + j;
+                const int col = first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>;
                 if (col < k) out[col] = acc[i][j];
             }
     } else {
@@ -557,7 +602,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) warp_acc[sub * W + (t + i * TPR) * 8 + j] = acc[i][j];
+            for (int j = 0; j < 8; ++j) warp_acc[sub * W + first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>] = acc[i][j];
         __syncthreads();
         for (int col = threadIdx.x; col < k; col += 256) {
             float v = 0.0f;

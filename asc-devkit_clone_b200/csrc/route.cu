@@ -50,21 +50,56 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return f32_to_f16_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return f32_to_bf16(v); }
 
-// Logits as unsigned integers in their order (the usual map of IEEE bit patterns), -0 as +0.  0: masked (-inf), never chosen;
-// 1: NaN, chosen after every number.
-constexpr uint32_t kMasked = 0u;
-__device__ __forceinline__ uint32_t order_key(float x)
+// Largest of a warp's values; NaN only where all are.
+__device__ __forceinline__ float warp_max(float v)
 {
-    if (x != x) return 1u;
-    const uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));
-    const uint32_t key = b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
-    return key == 0x007FFFFFu ? kMasked : key;
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
-__device__ __forceinline__ float key_value(uint32_t key)
-{
-    if (key == 1u) return __uint_as_float(0x7FC00000u);
-    return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
-}
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// A lane's two best logits left, in the order of choice (value descending, expert ascending): the choice of k experts then takes
+// from the lanes' heads, and a lane looks through its logits again only after two of them were chosen, which is rare (8 choices
+// among 32 lanes: one token in twenty).  `last` / `last_e`: what it gave last, everything in front of that is gone.
+template <int NV>
+struct LaneBest {
+    float v1, v2;
+    int e1, e2, held;
+    __device__ __forceinline__ void scan(const float (&x)[NV], int lane, float last, int last_e)
+    {
+        v1 = v2 = kNegInf;
+        e1 = e2 = kMaxExperts;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = lane + 32 * i;
+            // (comparisons with a NaN are false: NaN logits are never among the best)
+            const bool left = x[i] < last || (x[i] == last && e > last_e);
+            const float v = left ? x[i] : kNegInf;
+            const bool first = v > v1, second = v > v2;  // equal values keep the lower expert, which came first
+            v2 = first ? v1 : second ? v : v2;
+            e2 = first ? e1 : second ? e : e2;
+            v1 = first ? v : v1;
+            e1 = first ? e : e1;
+        }
+        held = 2;
+    }
+    __device__ __forceinline__ void scan(const float (&x)[NV], int lane)  // from the start
+    {
+        v1 = v2 = kNegInf;
+        e1 = e2 = kMaxExperts;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = lane + 32 * i;
+            const bool first = x[i] > v1, second = x[i] > v2;
+            v2 = first ? v1 : second ? x[i] : v2;
+            e2 = first ? e1 : second ? e : e2;
+            v1 = first ? x[i] : v1;
+            e1 = first ? e : e1;
+        }
+        held = 2;
+    }
+};
 
 struct RouteArgs {
     const void* logits;
@@ -112,55 +147,89 @@ route_kernel(const RouteArgs p)
 #pragma unroll
     for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
     int used = 0;
-    for (long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + w; t < p.tokens; t += gridDim.x * kRouteWarps) {
-        const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-        uint32_t key[NV];
-        uint32_t top = kMasked;
-        const bool open = !p.valid || p.valid[t] != 0;
+    const long long step = static_cast<long long>(gridDim.x) * kRouteWarps;
+    long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + w;
+    constexpr bool AHEAD = NV <= 16;  // the next token's logits are requested before this one's are worked on
+    T raw[NV], ahead[NV];
+    uint8_t open = 1, open_ahead = 1;
+    auto load = [&](long long token, T (&to)[NV], uint8_t& valid) {
+        if (token >= p.tokens) return;
+        if (p.valid) valid = p.valid[token];
+        const T* row = static_cast<const T*>(p.logits) + token * p.ld;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = lane + 32 * i;
-            key[i] = (open && e < E) ? order_key(to_f32(row[e])) : kMasked;
-            top = max(top, key[i]);
+        for (int i = 0; i < NV; ++i)
+            if (lane + 32 * i < E) to[i] = row[lane + 32 * i];
+    };
+    if constexpr (AHEAD) load(t, ahead, open_ahead);
+    for (; t < p.tokens; t += step) {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) raw[i] = ahead[i];
+            open = open_ahead;
+            load(t + step, ahead, open_ahead);
+        } else {
+            load(t, raw, open);
         }
-        top = __reduce_max_sync(kAll, top);
         int my_idx = -1;
         float my_w = 0.0f;
-        if (top != kMasked) {  // at least one expert to choose
-            ++used;
-            const float mx = key_value(top);
-            float prob[NV], sum = 0.0f;
+        if (open) {
+            float x[NV];
+            bool nan = false;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                prob[i] = key[i] != kMasked ? exp2_approx((key_value(key[i]) - mx) * kLog2e) : 0.0f;
-                sum += prob[i];
+                x[i] = lane + 32 * i < E ? to_f32(raw[i]) : kNegInf;
+                nan |= x[i] != x[i];
             }
-            const float inv = __frcp_rn(warp_sum(sum));
+            const bool any_nan = __any_sync(kAll, nan);
+            LaneBest<NV> best;
+            best.scan(x, lane);
+            float top = warp_max(best.v1);
+            if (top != kNegInf || any_nan) {  // at least one expert to choose
+                ++used;
+                const float mx = top;
+                float my_logit = 0.0f;
+                int chosen = 0;
+                while (top != kNegInf) {
+                    const int e = __reduce_min_sync(kAll, best.v1 == top ? best.e1 : kMaxExperts);  // of equal logits the first expert
+                    if (lane == chosen) my_idx = e, my_logit = top;
+                    if (++chosen == K) break;
+                    if (best.e1 == e) {
+                        best.v1 = best.v2, best.e1 = best.e2, best.v2 = kNegInf;
+                        if (--best.held == 0) best.scan(x, lane, top, e);
+                    }
+                    top = warp_max(best.v1);
+                }
+                if (any_nan) {  // after every number, in the order of the experts
+                    int last = -1;
+                    while (chosen < K) {
+                        int e = kMaxExperts;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) acc[i] = fmaf(prob[i], inv, acc[i]);
-            uint32_t my_key = kMasked;
-            for (int j = 0; j < K && top != kMasked; ++j) {
-                int e = kMaxExperts;
-#pragma unroll
-                for (int i = NV - 1; i >= 0; --i)
-                    if (key[i] == top) e = lane + 32 * i;
-                e = __reduce_min_sync(kAll, e);  // of equal logits the first expert
-                if (lane == j) my_idx = e, my_key = top;
-                top = kMasked;
+                        for (int i = NV - 1; i >= 0; --i)
+                            if (x[i] != x[i] && lane + 32 * i > last) e = lane + 32 * i;
+                        e = __reduce_min_sync(kAll, e);
+                        if (e == kMaxExperts) break;
+                        if (lane == chosen) my_idx = e, my_logit = __uint_as_float(0x7FC00000u);
+                        last = e;
+                        ++chosen;
+                    }
+                }
+                float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    if (lane + 32 * i == e) key[i] = kMasked;
-                    top = max(top, key[i]);
+                    x[i] = exp2_approx((x[i] - mx) * kLog2e);
+                    sum += x[i];
                 }
-                top = __reduce_max_sync(kAll, top);
-            }
-            if (my_idx >= 0) {
-                my_w = exp2_approx((key_value(my_key) - mx) * kLog2e) * inv;
-                atomicAdd(&s_count[my_idx], 1);
-            }
-            if (p.renorm) {
-                const float chosen = warp_sum(my_w);  // lanes without a choice hold 0
-                if (my_idx >= 0) my_w = __fdiv_rn(my_w, chosen);
+                const float inv = __frcp_rn(warp_sum(sum));
+#pragma unroll
+                for (int i = 0; i < NV; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
+                if (my_idx >= 0) {
+                    my_w = exp2_approx((my_logit - mx) * kLog2e) * inv;
+                    atomicAdd(&s_count[my_idx], 1);
+                }
+                if (p.renorm) {
+                    const float total = warp_sum(my_w);  // lanes without a choice hold 0
+                    if (my_idx >= 0) my_w = __fdiv_rn(my_w, total);
+                }
             }
         }
         if (lane < K) {
@@ -205,38 +274,33 @@ route_kernel(const RouteArgs p)
     }
 }
 
-// Adds the blocks' rows.  One cluster of eight blocks; each takes an eighth of the experts, 32 at a time, its eight warps a share
-// of the rows each; the shares of the loss meet in the first block's shared memory.
-constexpr int kFinishBlocks = 8;
-__global__ void __cluster_dims__(kFinishBlocks, 1, 1) __launch_bounds__(256)
+// Adds the blocks' rows.  One cluster of eight blocks; each takes an eighth of the experts, 32 at a time, its 32 warps every 32nd row
+// each (ten loads per thread, all in flight); the shares of the loss meet in the first block's shared memory.
+constexpr int kFinishBlocks = 8, kFinishWarps = 32;
+__global__ void __cluster_dims__(kFinishBlocks, 1, 1) __launch_bounds__(kFinishWarps * 32)
 route_finish_kernel(const RouteArgs p, int blocks)
 {
-    __shared__ float s_p[8][32];
-    __shared__ int s_c[8][32];
-    __shared__ int s_n[8];
+    __shared__ float s_p[kFinishWarps][32];
+    __shared__ int s_c[kFinishWarps][32];
+    __shared__ int s_n[kFinishWarps];
     __shared__ float s_loss[kFinishBlocks];
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // waited for below: every block of the cluster has started
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int n = 0;
-    for (int b = threadIdx.x; b < blocks; b += 256) n += p.part_tokens[b];
+    int n = static_cast<int>(threadIdx.x) < blocks ? p.part_tokens[threadIdx.x] : 0;
     n = __reduce_add_sync(kAll, n);
     if (lane == 0) s_n[w] = n;
-    __syncthreads();
-    n = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) n += s_n[i];
-    const float inv_n = __frcp_rn(static_cast<float>(max(n, 1)));
     const int per = (p.experts + kFinishBlocks - 1) / kFinishBlocks;
     const int e1 = min(p.experts, (static_cast<int>(blockIdx.x) + 1) * per);
-    float share = 0.0f;
-    for (int base = blockIdx.x * per; base < e1; base += 32) {
+    float share = 0.0f, inv_n = 0.0f;
+    int total_n = 0;
+    for (int base = blockIdx.x * per; base < (static_cast<int>(blockIdx.x) + 1) * per; base += 32) {
         const int e = base + lane;
         float v = 0.0f;
         int c = 0;
         if (e < e1) {
-#pragma unroll 4
-            for (int b = w; b < blocks; b += 8) {
+#pragma unroll 10
+            for (int b = w; b < blocks; b += kFinishWarps) {
                 v += p.part_prob[static_cast<size_t>(b) * p.experts + e];
                 c += p.part_count[static_cast<size_t>(b) * p.experts + e];
             }
@@ -244,10 +308,14 @@ route_finish_kernel(const RouteArgs p, int blocks)
         __syncthreads();
         s_p[w][lane] = v, s_c[w][lane] = c;
         __syncthreads();
-        if (w == 0 && e < e1) {
+        if (w == 0) {
+            total_n = __reduce_add_sync(kAll, s_n[lane]);
+            inv_n = __frcp_rn(static_cast<float>(max(total_n, 1)));
+            if (e < e1) {
 #pragma unroll
-            for (int i = 1; i < 8; ++i) v += s_p[i][lane], c += s_c[i][lane];
-            share += finish_expert(p, e, v, c, inv_n);
+                for (int i = 1; i < kFinishWarps; ++i) v += s_p[i][lane], c += s_c[i][lane];
+                share += finish_expert(p, e, v, c, inv_n);
+            }
         }
     }
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -266,7 +334,7 @@ route_finish_kernel(const RouteArgs p, int blocks)
 #pragma unroll
         for (int i = 0; i < kFinishBlocks; ++i) total += s_loss[i];
         if (p.loss) p.loss[0] = loss_of(p, total, inv_n);
-        if (p.num_tokens) p.num_tokens[0] = n;
+        if (p.num_tokens) p.num_tokens[0] = total_n;
     }
 }
 
@@ -382,7 +450,7 @@ int launch_route_as(const RouteArgs& p, int blocks, cudaStream_t st)
         }
     }
     ASCB200_CUDA(launch_pdl(route_kernel<T, NV>, blocks, kRouteWarps * 32, smem, st, p));
-    if (blocks > 1) ASCB200_CUDA(launch_pdl(route_finish_kernel, kFinishBlocks, 256, 0, st, p, blocks));
+    if (blocks > 1) ASCB200_CUDA(launch_pdl(route_finish_kernel, kFinishBlocks, kFinishWarps * 32, 0, st, p, blocks));
     return ASCB200_OK;
 }
 template <typename T>
