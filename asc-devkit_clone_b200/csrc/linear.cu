@@ -235,58 +235,80 @@ struct ActGradArgs {
     void* dz;
     float* partial;  // [row blocks][n], or nullptr
     long long ld_dy, ldz, ld_dz;
-    int m, n, act;
-    int vec;         // dy and z allow 16-byte loads
+    int m, n;
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int col, int n, bool vec, float (&f)[8])
+struct alignas(16) Eight {
+    T e[8];
+};
+// VEC (rows of dy, z and dz start on 16 bytes and n is a multiple of 8): a lane's eight columns are neighbours.  Else they are 32 apart, so
+// that a warp's accesses of one element each are contiguous.  (One kernel that chose per row took 64 us for 4096 x 11008, and 117 with
+// four rows in flight: the two paths' loads met in the same registers and were waited for one by one.)
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int col, int n, Eight<T>& r)
 {
-    if (vec && col + 8 <= n) {
+    if constexpr (VEC) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + col));
-        const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = as_f32(e[j]);
+        r = *reinterpret_cast<const Eight<T>*>(&v);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = col + j < n ? as_f32(row[col + j]) : 0.0f;
+        for (int j = 0; j < 8; ++j) r.e[j] = col + 32 * j < n ? row[col + 32 * j] : rounded<T>(0.0f);
     }
 }
 
-template <typename T>
+template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256)
 act_grad_kernel(const ActGradArgs p)
 {
     __shared__ float part[8][256];
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int col = blockIdx.x * 256 + lane * 8;
+    const int in_block = VEC ? lane * 8 : lane, col = blockIdx.x * 256 + in_block;
     float acc[8] = {};
+    constexpr int U = 4;  // rows whose loads are in flight together
     if (col < p.n) {
-        for (long long row = static_cast<long long>(blockIdx.y) * 8 + warp; row < p.m; row += static_cast<long long>(gridDim.y) * 8) {
-            float dy[8];
-            load8(static_cast<const T*>(p.dy) + row * p.ld_dy, col, p.n, p.vec, dy);
-            if (p.act != ASCB200_ACT_NONE) {
-                float z[8];
-                load8(static_cast<const T*>(p.z) + row * p.ldz, col, p.n, p.vec, z);
-                ASCB200_ACT_SWITCH(p.act, {
+        const long long step = static_cast<long long>(gridDim.y) * 8;
+        for (long long row0 = static_cast<long long>(blockIdx.y) * 8 + warp; row0 < p.m; row0 += U * step) {
+            Eight<T> dyr[U], zr[U];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) dy[j] *= act::slope<ACT>(z[j]);
-                })
+            for (int u = 0; u < U; ++u) {
+                const long long row = min(row0 + u * step, static_cast<long long>(p.m) - 1);
+                load8<T, VEC>(static_cast<const T*>(p.dy) + row * p.ld_dy, col, p.n, dyr[u]);
+                if constexpr (ACT != ASCB200_ACT_NONE) load8<T, VEC>(static_cast<const T*>(p.z) + row * p.ldz, col, p.n, zr[u]);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += dy[j];
-            if (p.dz) {  // rows of dz are 16-byte aligned and have room for whole chunks; columns past n become zero
-                T out[8];
+            for (int u = 0; u < U; ++u) {
+                const long long row = row0 + u * step;
+                if (row >= p.m) break;
+                float dy[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) out[j] = rounded<T>(dy[j]);
-                *reinterpret_cast<uint4*>(static_cast<T*>(p.dz) + row * p.ld_dz + col) = *reinterpret_cast<const uint4*>(out);
+                for (int j = 0; j < 8; ++j) dy[j] = as_f32(dyr[u].e[j]);
+                if constexpr (ACT != ASCB200_ACT_NONE) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dy[j] *= act::slope<ACT>(as_f32(zr[u].e[j]));
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[j] += dy[j];
+                if (p.dz) {
+                    T* out = static_cast<T*>(p.dz) + row * p.ld_dz + col;
+                    if constexpr (VEC) {
+                        Eight<T> v;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v.e[j] = rounded<T>(dy[j]);
+                        *reinterpret_cast<Eight<T>*>(out) = v;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (col + 32 * j < p.n) out[32 * j] = rounded<T>(dy[j]);
+                    }
+                }
             }
         }
     }
     if (!p.partial) return;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) part[warp][lane * 8 + j] = acc[j];
+    for (int j = 0; j < 8; ++j) part[warp][in_block + (VEC ? j : 32 * j)] = acc[j];
     __syncthreads();
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c < p.n) {
@@ -295,6 +317,27 @@ act_grad_kernel(const ActGradArgs p)
         for (int i = 0; i < 8; ++i) v += part[i][threadIdx.x];
         p.partial[static_cast<size_t>(blockIdx.y) * p.n + c] = v;
     }
+}
+
+template <typename T, bool VEC>
+int launch_act_grad_as(const ActGradArgs& p, int act, dim3 grid, cudaStream_t st)
+{
+    switch (act) {
+#define ASCB200_ACT_GRAD(A) case A: ASCB200_CUDA(launch_pdl(act_grad_kernel<T, A, VEC>, grid, 256, 0, st, p)); return ASCB200_OK;
+        ASCB200_ACT_GRAD(ASCB200_ACT_FASTER_GELU)
+        ASCB200_ACT_GRAD(ASCB200_ACT_RELU)
+        ASCB200_ACT_GRAD(ASCB200_ACT_GELU)
+        ASCB200_ACT_GRAD(ASCB200_ACT_GELU_TANH)
+        ASCB200_ACT_GRAD(ASCB200_ACT_SILU)
+        default: ASCB200_CUDA(launch_pdl(act_grad_kernel<T, ASCB200_ACT_NONE, VEC>, grid, 256, 0, st, p)); return ASCB200_OK;
+#undef ASCB200_ACT_GRAD
+    }
+}
+
+template <typename T>
+int launch_act_grad(const ActGradArgs& p, int act, bool vec, dim3 grid, cudaStream_t st)
+{
+    return vec ? launch_act_grad_as<T, true>(p, act, grid, st) : launch_act_grad_as<T, false>(p, act, grid, st);
 }
 
 constexpr int kActGradBlocks = 592;  // blocks to aim for: four per SM
@@ -348,20 +391,20 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
         if (!d.workspace_dev || d.workspace_bytes < linear_grad_workspace(d.m, d.n)) return ASCB200_EINVAL;
         if (!aligned_to(d.workspace_dev, 256)) return ASCB200_EALIGN;
         ActGradArgs p = {};
-        p.dy = d.dy_dev, p.z = d.z_dev, p.ld_dy = d.ld_dy, p.ldz = d.ldz, p.m = d.m, p.n = d.n, p.act = d.act;
+        p.dy = d.dy_dev, p.z = d.z_dev, p.ld_dy = d.ld_dy, p.ldz = d.ldz, p.m = d.m, p.n = d.n;
         if (make_dz) {
             dz = p.dz = d.workspace_dev;
             ld_dz = p.ld_dz = (static_cast<int64_t>(d.n) + 7) / 8 * 8;
         }
         if (d.dbias_dev) p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(d.workspace_dev) + dz_bytes(d.m, d.n));
-        p.vec = operand_aligned(d.dy_dev, d.ld_dy, 2) && (d.act == ASCB200_ACT_NONE || operand_aligned(d.z_dev, d.ldz, 2));
+        const bool vec = d.n % 8 == 0 && operand_aligned(d.dy_dev, d.ld_dy, 2) && (d.act == ASCB200_ACT_NONE || operand_aligned(d.z_dev, d.ldz, 2));
         const int rows = act_grad_row_blocks(d.m, d.n);
         const dim3 grid((d.n + 255) / 256, rows);
-        if (d.kind == ASCB200_KIND_F16) ASCB200_CUDA(launch_pdl(act_grad_kernel<__half>, grid, 256, 0, stream, p));
-        else ASCB200_CUDA(launch_pdl(act_grad_kernel<__nv_bfloat16>, grid, 256, 0, stream, p));
+        const int rc = d.kind == ASCB200_KIND_F16 ? launch_act_grad<__half>(p, d.act, vec, grid, stream) : launch_act_grad<__nv_bfloat16>(p, d.act, vec, grid, stream);
+        if (rc != ASCB200_OK) return rc;
         if (d.dbias_dev) {
-            const int rc = sum_partials(p.partial, d.dbias_dev, d.dbias_dtype, rows, d.n, stream);
-            if (rc != ASCB200_OK) return rc;
+            const int rc2 = sum_partials(p.partial, d.dbias_dev, d.dbias_dtype, rows, d.n, stream);
+            if (rc2 != ASCB200_OK) return rc2;
         }
     }
     if (d.dx_dev) {  // [m, k] = dz [m, n] * w

@@ -33,6 +33,32 @@ struct Raw8<float> {
     uint4 v, w;
 };
 
+// Two fp32 operations per instruction, each rounded to nearest.  The kernels move seven to eight bytes per element, so at the memory's rate
+// an SM has about 30 instruction slots per element pair: unpacked arithmetic (31 instructions per element) held the forward pass at
+// 145 us for 16383 x 7168 where this form takes the figure at the kernel.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, w, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // (not the read-only path: an output may be the row's own input)
 __device__ __forceinline__ uint4 ld_v4(const void* p)
 {
@@ -41,9 +67,9 @@ __device__ __forceinline__ uint4 ld_v4(const void* p)
     return r;
 }
 
-// A thread's i-th eight columns.  VEC (every row of every tensor starts on 16 bytes): neighbours, starting at `first_column`.  Else: 32
-// columns apart, so that a warp's accesses of one element each are contiguous whatever the alignment (fp32 1000 x 1111: 16.6 us with
-// neighbouring columns, see the figures at the kernels).  Either way a warp owns 256 contiguous columns.
+// A thread's i-th eight columns.  VEC (every row of every tensor starts on 16 bytes and k is a multiple of 8): neighbours, starting at
+// `first_column`.  Else: 32 columns apart, so that a warp's accesses of one element each are contiguous whatever the alignment (gradients of
+// fp32 1000 x 1111: 16 us with neighbouring columns, 10.5 so).  Either way a warp owns 256 contiguous columns.
 template <bool VEC>
 constexpr int kColumnStep = VEC ? 1 : 32;
 template <int TPR, bool VEC>
@@ -52,11 +78,11 @@ __device__ __forceinline__ int first_column(int t, int i)
     return VEC ? (t + i * TPR) * 8 : (i * TPR + (t & ~31)) * 8 + (t & 31);
 }
 
-// The eight elements at column c; elements past the row's end read as zero and are not touched.
+// The eight elements at column c < k; elements past the row's end read as zero and are not touched.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_chunk(const T* row, int c, int k, Raw8<T>& r)
 {
-    if (VEC && c + 8 <= k) {
+    if constexpr (VEC) {
         r.v = ld_v4(row + c);
         if constexpr (sizeof(T) == 4) r.w = ld_v4(row + c + 4);
         return;
@@ -77,25 +103,22 @@ __device__ __forceinline__ void load_chunk(const T* row, int c, int k, Raw8<T>& 
         r.v = make_uint4(u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16));
     }
 }
-__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&f)[8])
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float2 (&f)[4])
 {
-    f[0] = __uint_as_float(r.v.x), f[1] = __uint_as_float(r.v.y), f[2] = __uint_as_float(r.v.z), f[3] = __uint_as_float(r.v.w);
-    f[4] = __uint_as_float(r.w.x), f[5] = __uint_as_float(r.w.y), f[6] = __uint_as_float(r.w.z), f[7] = __uint_as_float(r.w.w);
+    f[0] = make_float2(__uint_as_float(r.v.x), __uint_as_float(r.v.y)), f[1] = make_float2(__uint_as_float(r.v.z), __uint_as_float(r.v.w));
+    f[2] = make_float2(__uint_as_float(r.w.x), __uint_as_float(r.w.y)), f[3] = make_float2(__uint_as_float(r.w.z), __uint_as_float(r.w.w));
 }
-__device__ __forceinline__ void unpack8(const Raw8<__half>& r, float (&f)[8])
+__device__ __forceinline__ void unpack8(const Raw8<__half>& r, float2 (&f)[4])
 {
     const __half2* h = reinterpret_cast<const __half2*>(&r.v);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 v = __half22float2(h[j]);
-        f[2 * j] = v.x, f[2 * j + 1] = v.y;
-    }
+    for (int j = 0; j < 4; ++j) f[j] = __half22float2(h[j]);
 }
-__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& r, float (&f)[8])
+__device__ __forceinline__ void unpack8(const Raw8<__nv_bfloat16>& r, float2 (&f)[4])
 {
     const uint32_t u[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[2 * j] = __uint_as_float(u[j] << 16), f[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+    for (int j = 0; j < 4; ++j) f[j] = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xFFFF0000u));
 }
 // One rounding, to the output type; halves saturate at +-65504 like every fp16 output of the library, NaN is kept.
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half)
@@ -110,20 +133,20 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16)
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store_chunk(T* row, int c, int k, const float (&f)[8])
+__device__ __forceinline__ void store_chunk(T* row, int c, int k, const float2 (&f)[4])
 {
     if constexpr (sizeof(T) == 4) {
-        if (VEC && c + 8 <= k) {
-            *reinterpret_cast<float4*>(row + c) = make_float4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float4*>(row + c + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        if constexpr (VEC) {
+            *reinterpret_cast<float4*>(row + c) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+            *reinterpret_cast<float4*>(row + c + 4) = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + j * kColumnStep<VEC> < k) row[c + j * kColumnStep<VEC>] = f[j];
+                if (c + j * kColumnStep<VEC> < k) row[c + j * kColumnStep<VEC>] = j & 1 ? f[j / 2].y : f[j / 2].x;
         }
     } else {
-        const uint4 v = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
-        if (VEC && c + 8 <= k) {
+        const uint4 v = make_uint4(pack2(f[0].x, f[0].y, T()), pack2(f[1].x, f[1].y, T()), pack2(f[2].x, f[2].y, T()), pack2(f[3].x, f[3].y, T()));
+        if constexpr (VEC) {
             *reinterpret_cast<uint4*>(row + c) = v;
         } else {
             const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -135,23 +158,26 @@ __device__ __forceinline__ void store_chunk(T* row, int c, int k, const float (&
 }
 // gamma: NULL (ones), fp32, or the rows' type.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_gamma(const void* __restrict__ gamma, int gamma_f32, int c, int k, float (&g)[8])
+__device__ __forceinline__ void load_gamma(const void* __restrict__ gamma, int gamma_f32, int c, int k, float2 (&g)[4])
 {
     if (!gamma) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = 1.0f;
+        for (int j = 0; j < 4; ++j) g[j] = both(1.0f);
     } else if (sizeof(T) == 4 || gamma_f32) {
         const float* src = static_cast<const float*>(gamma) + c;
-        if (VEC && c + 8 <= k) {
+        if constexpr (VEC) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
-            g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, g[4] = b.x, g[5] = b.y, g[6] = b.z, g[7] = b.w;
+            g[0] = make_float2(a.x, a.y), g[1] = make_float2(a.z, a.w), g[2] = make_float2(b.x, b.y), g[3] = make_float2(b.z, b.w);
         } else {
+            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = c + j * kColumnStep<VEC> < k ? __ldg(src + j * kColumnStep<VEC>) : 0.0f;
+            for (int j = 0; j < 8; ++j) v[j] = c + j * kColumnStep<VEC> < k ? __ldg(src + j * kColumnStep<VEC>) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[j] = make_float2(v[2 * j], v[2 * j + 1]);
         }
     } else {
         Raw8<T> r;
-        if (VEC && c + 8 <= k) r.v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(gamma) + c));
+        if constexpr (VEC) r.v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(gamma) + c));
         else load_chunk<T, VEC>(static_cast<const T*>(gamma), c, k, r);
         unpack8(r, g);
     }
@@ -164,17 +190,23 @@ __device__ __forceinline__ float max_nan(float a, float b)  // a NaN stays
     return r;
 }
 
+__device__ __forceinline__ float max_abs(float m, float2 v)  // m >= 0
+{
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(v.x), "f"(v.y));
+    return r;
+}
 // Largest of a warp's non-negative floats: their bit patterns are in the same order, and a NaN's is above infinity's.
 __device__ __forceinline__ float warp_max_abs(float v) { return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v))); }
 
 // Sum and (of non-negative values) maximum over the TPR threads of a row; `red` holds one entry per warp and is not used again before
 // the next barrier.
-template <int TPR>
+template <int TPR, bool MAX = true>
 __device__ __forceinline__ void row_reduce(float& s, float& mx, float2* red)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    mx = warp_max_abs(mx);
+    if (MAX) mx = warp_max_abs(mx);
     if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;  // a power of two
         const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
@@ -184,7 +216,7 @@ __device__ __forceinline__ void row_reduce(float& s, float& mx, float2* red)
         s = v.x;
 #pragma unroll
         for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        mx = warp_max_abs(v.y);
+        if (MAX) mx = warp_max_abs(v.y);
     }
 }
 
@@ -232,31 +264,43 @@ __device__ __forceinline__ uint32_t mx_scale_byte(float amax, float& inv)
     return byte;
 }
 
-__device__ __forceinline__ uint32_t s8_of(float v)  // nearest even, saturating, NaN -> 0
+__device__ __forceinline__ uint32_t e4m3x2_of(float2 v)
 {
-    int r;
-    asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(r) : "f"(v));
-    return static_cast<uint32_t>(r) & 0xFFu;
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
+    return r;
 }
-__device__ __forceinline__ uint32_t e4m3x2_of(float a, float b)
+// Low bytes of four words.
+__device__ __forceinline__ uint32_t pack_bytes(float2 a, float2 b)
 {
-    uint16_t v;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(v) : "f"(b), "f"(a));
-    return v;
+    const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
 }
-// Eight codes: y times the reciprocal of its scale.
+// Eight codes of y * mul (mul: the reciprocals of the scales).  int8: |y * mul| is at most 127 and a bit, so adding 1.5 * 2^23 in the
+// same instruction rounds it once, to the nearest even integer, which is then the sum's low byte in two's complement; values whose
+// scale is NaN give 0.
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8, const float (&y)[8], const float (&mul)[8])
+__device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8, const float2 (&y)[4], const float2 (&mul)[4])
 {
     uint32_t a, b;
     if (s8) {
-        a = s8_of(y[0] * mul[0]) | (s8_of(y[1] * mul[1]) << 8) | (s8_of(y[2] * mul[2]) << 16) | (s8_of(y[3] * mul[3]) << 24);
-        b = s8_of(y[4] * mul[4]) | (s8_of(y[5] * mul[5]) << 8) | (s8_of(y[6] * mul[6]) << 16) | (s8_of(y[7] * mul[7]) << 24);
+        const float2 magic = both(12582912.0f);
+        float2 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = fma2(y[j], mul[j], magic);
+            if constexpr (!VEC) {  // the eight values may have different scales
+                if (mul[j].x != mul[j].x) v[j].x = 0.0f;
+                if (mul[j].y != mul[j].y) v[j].y = 0.0f;
+            }
+        }
+        a = pack_bytes(v[0], v[1]), b = pack_bytes(v[2], v[3]);
+        if (VEC && mul[0].x != mul[0].x) a = b = 0u;
     } else {
-        a = e4m3x2_of(y[0] * mul[0], y[1] * mul[1]) | (e4m3x2_of(y[2] * mul[2], y[3] * mul[3]) << 16);
-        b = e4m3x2_of(y[4] * mul[4], y[5] * mul[5]) | (e4m3x2_of(y[6] * mul[6], y[7] * mul[7]) << 16);
+        a = e4m3x2_of(mul2(y[0], mul[0])) | (e4m3x2_of(mul2(y[1], mul[1])) << 16);
+        b = e4m3x2_of(mul2(y[2], mul[2])) | (e4m3x2_of(mul2(y[3], mul[3])) << 16);
     }
-    if (VEC && c + 8 <= k) {
+    if constexpr (VEC) {
         *reinterpret_cast<uint2*>(row + c) = make_uint2(a, b);
     } else {
 #pragma unroll
@@ -287,33 +331,34 @@ rms_norm_kernel(const NormArgs p)
             if (r) load_chunk<T, VEC>(r, c, k, rr[i]);
         }
     }
-    float hg[NCHUNK][8];
-    float ss = 0.0f, amax = 0.0f;
+    float2 hg[NCHUNK][4], ss2 = both(0.0f);
+    float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
         const int c = first_column<TPR, VEC>(t, i);
         if (c < k) {
-            float g[8];
+            float2 g[4];
             unpack8(xr[i], hg[i]);
             if (r) {
-                float v[8];
+                float2 v[4];
                 unpack8(rr[i], v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) hg[i][j] += v[j];
+                for (int j = 0; j < 4; ++j) hg[i][j] = add2(hg[i][j], v[j]);
             }
             if (p.sum) store_chunk<T, VEC>(static_cast<T*>(p.sum) + row * p.ld_sum, c, k, hg[i]);
             load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                ss = fmaf(hg[i][j], hg[i][j], ss);
-                hg[i][j] *= g[j];
-                amax = max_nan(amax, fabsf(hg[i][j]));
+            for (int j = 0; j < 4; ++j) {
+                ss2 = fma2(hg[i][j], hg[i][j], ss2);
+                hg[i][j] = mul2(hg[i][j], g[j]);
+                amax = max_abs(amax, hg[i][j]);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) hg[i][j] = 0.0f;
+            for (int j = 0; j < 4; ++j) hg[i][j] = both(0.0f);
         }
     }
+    float ss = ss2.x + ss2.y;
     row_reduce<TPR>(ss, amax, red);
     const float rstd = __frsqrt_rn(__fdiv_rn(ss, static_cast<float>(k)) + p.eps);
     if (p.rstd && t == 0) p.rstd[row] = rstd;
@@ -323,9 +368,9 @@ rms_norm_kernel(const NormArgs p)
         for (int i = 0; i < NCHUNK; ++i) {
             const int c = first_column<TPR, VEC>(t, i);
             if (c < k) {
-                float v[8];
+                float2 v[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = hg[i][j] * rstd;
+                for (int j = 0; j < 4; ++j) v[j] = mul2(hg[i][j], both(rstd));
                 store_chunk<T, VEC>(y, c, k, v);
             }
         }
@@ -356,23 +401,23 @@ rms_norm_kernel(const NormArgs p)
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
         const int c = first_column<TPR, VEC>(t, i);
-        float y[8], mul[8];
+        float2 y[4], mul[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = hg[i][j] * rstd, mul[j] = inv;
+        for (int j = 0; j < 4; ++j) y[j] = mul2(hg[i][j], both(rstd)), mul[j] = both(inv);
         if (p.scale_mode != ASCB200_SCALE_PER_TOKEN) {
             // the whole warp takes part in a group's maximum, columns past the row's end with zeros
             if constexpr (VEC) {  // a group is `lanes` neighbouring lanes
                 float g = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g = max_nan(g, fabsf(y[j]));
+                for (int j = 0; j < 4; ++j) g = max_abs(g, y[j]);
                 for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
                 const float r = scale_group(g, c, (c / 8 & (lanes - 1)) == 0 && c < k);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) mul[j] = r;
+                for (int j = 0; j < 4; ++j) mul[j] = both(r);
             } else {  // a group is one, two, four or eight of the warp's 32-column runs
                 float g[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = warp_max_abs(fabsf(y[j]));
+                for (int j = 0; j < 8; ++j) g[j] = warp_max_abs(fabsf(j & 1 ? y[j / 2].y : y[j / 2].x));
 #pragma unroll
                 for (int o = 1; o < 8; o <<= 1) {
                     if (o * 4 >= lanes) break;
@@ -381,7 +426,9 @@ rms_norm_kernel(const NormArgs p)
                         if (!(j & o)) g[j] = g[j ^ o] = max_nan(g[j], g[j ^ o]);
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) mul[j] = scale_group(g[j], c + j * 32, (t & 31) == 0 && (j * 4 & (lanes - 1)) == 0 && c + j * 32 < k);
+                for (int j = 0; j < 8; ++j) g[j] = scale_group(g[j], c + j * 32, (t & 31) == 0 && (j * 4 & (lanes - 1)) == 0 && c + j * 32 < k);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mul[j] = make_float2(g[2 * j], g[2 * j + 1]);
             }
         }
         if (c < k) store_codes<VEC>(q, c, k, s8, y, mul);
@@ -468,8 +515,8 @@ int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
     p.rstd = d.rstd_dev;
     p.ldx = d.ldx, p.ld_residual = d.ld_residual, p.ld_sum = d.ld_sum, p.ldy = d.ldy, p.ldq = d.ldq;
     p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32, p.q_s8 = d.q_dtype == ASCB200_S8, p.scale_mode = d.scale_mode, p.eps = d.eps;
-    // 16-byte accesses where every row of every tensor allows them; element by element otherwise
-    const bool vec = rows_aligned(d.x_dev, d.ldx, esz, 16) && rows_aligned(d.residual_dev, d.ld_residual, esz, 16) && rows_aligned(d.sum_dev, d.ld_sum, esz, 16) &&
+    // 16-byte accesses where every row of every tensor allows them, element by element otherwise (see first_column)
+    const bool vec = d.k % 8 == 0 && rows_aligned(d.x_dev, d.ldx, esz, 16) && rows_aligned(d.residual_dev, d.ld_residual, esz, 16) && rows_aligned(d.sum_dev, d.ld_sum, esz, 16) &&
                      rows_aligned(d.y_dev, d.ldy, esz, 16) && rows_aligned(d.q_dev, d.ldq, 1, 8) && (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
     const int sms = st->sm_count;
     switch (d.dtype) {
@@ -505,25 +552,31 @@ __device__ __forceinline__ void load_grad_row(const NormGradArgs& p, long long r
 {
     if (row >= p.m) return;
     r.rstd = __ldg(p.rstd + row);
+    const T* dy = static_cast<const T*>(p.dy) + row * p.ld_dy;
+    const T* h = static_cast<const T*>(p.h) + row * p.ldh;
+    const T* dh = static_cast<const T*>(p.dh) + row * p.ld_dh;
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
         const int c = first_column<TPR, VEC>(t, i);
         if (c < p.k) {
-            load_chunk<T, VEC>(static_cast<const T*>(p.dy) + row * p.ld_dy, c, p.k, r.dy[i]);
-            load_chunk<T, VEC>(static_cast<const T*>(p.h) + row * p.ldh, c, p.k, r.h[i]);
-            if (p.dh) load_chunk<T, VEC>(static_cast<const T*>(p.dh) + row * p.ld_dh, c, p.k, r.dh[i]);
+            load_chunk<T, VEC>(dy, c, p.k, r.dy[i]);
+            load_chunk<T, VEC>(h, c, p.k, r.h[i]);
+            if (p.dh) load_chunk<T, VEC>(dh, c, p.k, r.dh[i]);
         }
     }
 }
 
-// TPR threads per row as above; a block holds ROWS rows at a time (blocks of 256 threads for warp rows).  Where registers allow, the next
-// row is requested before the current one is worked on.
+// TPR threads per row as above; a block holds ROWS rows at a time (blocks of 256 threads for warp rows).  Up to two chunks per thread keep gamma,
+// dy * gamma and hat in registers from the reduction to the output, and (16-bit types) request the next row before the current one is
+// worked on; more chunks read gamma and unpack dy and h twice.
 template <typename T, int TPR, int NCHUNK, bool VEC>
-__global__ void __launch_bounds__(TPR > 32 ? TPR : 256)
+__global__ void __launch_bounds__(TPR > 32 ? TPR : 256, TPR > 32 && NCHUNK == 1 && sizeof(T) == 2 && VEC ? 1024 / TPR : 1)
 rms_norm_grad_kernel(const NormGradArgs p)
 {
     constexpr int ROWS = TPR > 32 ? 1 : 8;
-    constexpr bool AHEAD = NCHUNK * sizeof(T) <= 8;
+    constexpr bool AHEAD = NCHUNK * sizeof(T) <= 4;
+    constexpr bool KEEP = NCHUNK <= 2;
+    constexpr int HELD = KEEP ? NCHUNK : 1;
     __shared__ float2 red[2][32];
     extern __shared__ float warp_acc[];  // warp rows: [8][TPR * NCHUNK * 8]
     grid_dependency_wait();
@@ -531,11 +584,16 @@ rms_norm_grad_kernel(const NormGradArgs p)
     const int sub = TPR > 32 ? 0 : threadIdx.x >> 5;
     const int k = p.k;
     const float inv_k = __frcp_rn(static_cast<float>(k));
-    float acc[NCHUNK][8];
+    float2 acc[NCHUNK][4], gamma[HELD][4], hat[HELD][4], g[HELD][4];
 #pragma unroll
-    for (int i = 0; i < NCHUNK; ++i)
+    for (int i = 0; i < NCHUNK; ++i) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) acc[i][j] = both(0.0f);
+        if constexpr (KEEP) {
+            const int c = first_column<TPR, VEC>(t, i);
+            if (c < k) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, gamma[i]);
+        }
+    }
     int parity = 0;
     const long long step = static_cast<long long>(gridDim.x) * ROWS;
     long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
@@ -548,42 +606,53 @@ rms_norm_grad_kernel(const NormGradArgs p)
         } else {
             load_grad_row<T, TPR, NCHUNK, VEC>(p, row, t, r);
         }
-        const float rstd = r.rstd;
-        float dot = 0.0f, none = 0.0f;
+        const float2 rstd = both(r.rstd);
+        float2 dot2 = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
             const int c = first_column<TPR, VEC>(t, i);
+            const int held = KEEP ? i : 0;
             if (c < k) {
-                float a[8], b[8], g[8];
+                float2 a[4];
                 unpack8(r.dy[i], a);
-                unpack8(r.h[i], b);
-                load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
+                unpack8(r.h[i], hat[held]);
+                if constexpr (!KEEP) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, gamma[held]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = a[j] * (b[j] * rstd);  // dy * hat
-                    acc[i][j] += v;
-                    dot = fmaf(v, g[j], dot);
+                for (int j = 0; j < 4; ++j) {
+                    hat[held][j] = mul2(hat[held][j], rstd);
+                    acc[i][j] = fma2(a[j], hat[held][j], acc[i][j]);
+                    g[held][j] = mul2(a[j], gamma[held][j]);
+                    dot2 = fma2(g[held][j], hat[held][j], dot2);
                 }
             }
         }
-        row_reduce<TPR>(dot, none, red[parity]);
-        const float mean = dot * inv_k;
+        float dot = dot2.x + dot2.y, none = 0.0f;
+        row_reduce<TPR, false>(dot, none, red[parity]);
+        const float2 minus_mean = both(-dot * inv_k);
         T* dx = static_cast<T*>(p.dx) + row * p.ld_dx;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
             const int c = first_column<TPR, VEC>(t, i);
+            const int held = KEEP ? i : 0;
             if (c < k) {
-                float a[8], b[8], g[8], e[8];
-                unpack8(r.dy[i], a);
-                unpack8(r.h[i], b);
-                load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
-                if (p.dh) unpack8(r.dh[i], e);
+                float2 e[4];
+                if constexpr (!KEEP) {
+                    float2 a[4];
+                    unpack8(r.dy[i], a);
+                    unpack8(r.h[i], hat[held]);
+                    load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, gamma[held]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = rstd * (a[j] * g[j] - (b[j] * rstd) * mean);
-                    a[j] = p.dh ? v + e[j] : v;
+                    for (int j = 0; j < 4; ++j) hat[held][j] = mul2(hat[held][j], rstd), g[held][j] = mul2(a[j], gamma[held][j]);
                 }
-                store_chunk<T, VEC>(dx, c, k, a);
+                if (p.dh) {
+                    unpack8(r.dh[i], e);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[j] = both(0.0f);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) e[j] = fma2(fma2(hat[held][j], minus_mean, g[held][j]), rstd, e[j]);
+                store_chunk<T, VEC>(dx, c, k, e);
             }
         }
     }
@@ -595,14 +664,14 @@ rms_norm_grad_kernel(const NormGradArgs p)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int col = first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>;
-                if (col < k) out[col] = acc[i][j];
+                if (col < k) out[col] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
             }
     } else {
         constexpr int W = TPR * NCHUNK * 8;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) warp_acc[sub * W + first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>] = acc[i][j];
+            for (int j = 0; j < 8; ++j) warp_acc[sub * W + first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
         __syncthreads();
         for (int col = threadIdx.x; col < k; col += 256) {
             float v = 0.0f;
@@ -628,9 +697,9 @@ int launch_norm_grad(const NormGradArgs& p, int sms, cudaStream_t st, int* block
     const int chunks = (p.k + 7) / 8;
     if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, VEC>(p, sms, st, blocks);
     if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, VEC>(p, sms, st, blocks);
-    if (chunks <= 128) return launch_norm_grad_as<T, 32, 4, VEC>(p, sms, st, blocks);
-    if (chunks <= 256) return launch_norm_grad_as<T, 128, 2, VEC>(p, sms, st, blocks);
-    if (chunks <= 512) return launch_norm_grad_as<T, 256, 2, VEC>(p, sms, st, blocks);
+    if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, VEC>(p, sms, st, blocks);
+    if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, VEC>(p, sms, st, blocks);
+    if (chunks <= 512) return launch_norm_grad_as<T, 512, 1, VEC>(p, sms, st, blocks);
     if (chunks <= 1024) return launch_norm_grad_as<T, 512, 2, VEC>(p, sms, st, blocks);
     if (chunks <= 2048) return launch_norm_grad_as<T, 512, 4, VEC>(p, sms, st, blocks);
     return launch_norm_grad_as<T, 1024, 4, VEC>(p, sms, st, blocks);
@@ -668,7 +737,7 @@ int run_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, cudaStream_t strea
     p.dy = d.dy_dev, p.h = d.h_dev, p.rstd = d.rstd_dev, p.gamma = d.gamma_dev, p.dh = d.dh_dev, p.dx = d.dx_dev;
     p.partial = d.dgamma_dev ? static_cast<float*>(d.workspace_dev) : nullptr;
     p.ld_dy = d.ld_dy, p.ldh = d.ldh, p.ld_dh = d.ld_dh, p.ld_dx = d.ld_dx, p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32;
-    const bool vec = rows_aligned(d.dy_dev, d.ld_dy, esz, 16) && rows_aligned(d.h_dev, d.ldh, esz, 16) && rows_aligned(d.dh_dev, d.ld_dh, esz, 16) &&
+    const bool vec = d.k % 8 == 0 && rows_aligned(d.dy_dev, d.ld_dy, esz, 16) && rows_aligned(d.h_dev, d.ldh, esz, 16) && rows_aligned(d.dh_dev, d.ld_dh, esz, 16) &&
                      rows_aligned(d.dx_dev, d.ld_dx, esz, 16) && (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
     int blocks = 0, rc;
     const int sms = st->sm_count;

@@ -59,47 +59,95 @@ __device__ __forceinline__ float warp_max(float v)
 }
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// A lane's two best logits left, in the order of choice (value descending, expert ascending): the choice of k experts then takes
-// from the lanes' heads, and a lane looks through its logits again only after two of them were chosen, which is rare (8 choices
-// among 32 lanes: one token in twenty).  `last` / `last_e`: what it gave last, everything in front of that is gone.
-template <int NV>
-struct LaneBest {
-    float v1, v2;
-    int e1, e2, held;
-    __device__ __forceinline__ void scan(const float (&x)[NV], int lane, float last, int last_e)
+// The choice works on one integer per logit: its bits in their order (as signed integers), with the expert in the low bits, the lower
+// expert larger.  The largest integer of the warp is then the next choice and its expert at once, and a lane keeps its three
+// largest with five integer minima and maxima per logit.  (Comparing values and carrying expert numbers beside them took 730
+// instructions per token of 256 experts and 8 choices, bound by the integer pipe; this takes about half.)  A 16-bit logit has at least 13
+// low zero bits as fp32, so this is exact; an fp32 logit loses its low bits to the expert, so a token among whose choices, or behind
+// the last of them, two neighbours agree in the remaining bits is chosen again exactly (choose_exactly).
+constexpr int kNoChoice = static_cast<int>(0x80000000u);
+constexpr int kLowest = static_cast<int>(0x80800000u);  // -FLT_MAX; smaller: -inf, or nothing
+__device__ __forceinline__ int order_key(float x, int e, int low_bits)
+{
+    const int b = __float_as_int(__fadd_rn(x, 0.0f));  // -0 as +0
+    return ((b ^ ((b >> 31) & 0x7FFFFFFF)) & ~low_bits) | (low_bits - e);
+}
+__device__ __forceinline__ float key_value(int key, int low_bits)
+{
+    const int b = key & ~low_bits;
+    return __int_as_float(b ^ ((b >> 31) & 0x7FFFFFFF));
+}
+struct Best3 {
+    int v1, v2, v3, held;
+    template <int NV>
+    __device__ __forceinline__ void scan(const int (&key)[NV], int below)
     {
-        v1 = v2 = kNegInf;
-        e1 = e2 = kMaxExperts;
+        v1 = v2 = v3 = kNoChoice;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = lane + 32 * i;
-            // (comparisons with a NaN are false: NaN logits are never among the best)
-            const bool left = x[i] < last || (x[i] == last && e > last_e);
-            const float v = left ? x[i] : kNegInf;
-            const bool first = v > v1, second = v > v2;  // equal values keep the lower expert, which came first
-            v2 = first ? v1 : second ? v : v2;
-            e2 = first ? e1 : second ? e : e2;
-            v1 = first ? v : v1;
-            e1 = first ? e : e1;
+            const int k = key[i] < below ? key[i] : kNoChoice;
+            v3 = max(v3, min(v2, k));
+            v2 = max(v2, min(v1, k));
+            v1 = max(v1, k);
         }
-        held = 2;
+        held = 3;
     }
-    __device__ __forceinline__ void scan(const float (&x)[NV], int lane)  // from the start
+    template <int NV>
+    __device__ __forceinline__ void scan(const int (&key)[NV])
     {
-        v1 = v2 = kNegInf;
-        e1 = e2 = kMaxExperts;
+        v1 = v2 = v3 = kNoChoice;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = lane + 32 * i;
-            const bool first = x[i] > v1, second = x[i] > v2;
-            v2 = first ? v1 : second ? x[i] : v2;
-            e2 = first ? e1 : second ? e : e2;
-            v1 = first ? x[i] : v1;
-            e1 = first ? e : e1;
+            v3 = max(v3, min(v2, key[i]));
+            v2 = max(v2, min(v1, key[i]));
+            v1 = max(v1, key[i]);
         }
-        held = 2;
+        held = 3;
     }
 };
+
+// Choice number `lane` of a token by comparisons of the values themselves: numbers in descending order, then NaN, equal ones in the order of
+// the experts; -inf never.  One pass over a lane's logits per choice: for the rare tokens.
+template <typename T, int NV>
+__device__ __noinline__ void choose_exactly(const T* row, int E, int K, int lane, int& my_idx)
+{
+    float x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = lane + 32 * i < E ? to_f32(row[lane + 32 * i]) : kNegInf;
+    my_idx = -1;
+    float last = __builtin_huge_valf();
+    int last_e = -1;
+    bool nan = false;  // the numbers are used up
+    for (int j = 0; j < K; ++j) {
+        float v = kNegInf;
+        int e = kMaxExperts;
+        if (!nan) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {  // (comparisons with a NaN are false)
+                const int f = lane + 32 * i;
+                if ((x[i] < last || (x[i] == last && f > last_e)) && x[i] > v) v = x[i], e = f;
+            }
+            const float top = warp_max(v);
+            nan = top == kNegInf;
+            if (!nan) {
+                e = __reduce_min_sync(kAll, v == top ? e : kMaxExperts);
+                last = top;
+            } else {
+                last_e = -1;
+            }
+        }
+        if (nan) {
+            e = kMaxExperts;
+#pragma unroll
+            for (int i = NV - 1; i >= 0; --i)
+                if (x[i] != x[i] && lane + 32 * i > last_e) e = lane + 32 * i;
+            e = __reduce_min_sync(kAll, e);
+            if (e == kMaxExperts) break;
+        }
+        if (lane == j) my_idx = e;
+        last_e = e;
+    }
+}
 
 struct RouteArgs {
     const void* logits;
@@ -149,6 +197,7 @@ route_kernel(const RouteArgs p)
     int used = 0;
     const long long step = static_cast<long long>(gridDim.x) * kRouteWarps;
     long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + w;
+    constexpr int low_bits = 32 * NV - 1;  // at most 1023; the numbers of all lanes' experts fit
     constexpr bool AHEAD = NV <= 16;  // the next token's logits are requested before this one's are worked on
     T raw[NV], ahead[NV];
     uint8_t open = 1, open_ahead = 1;
@@ -173,57 +222,59 @@ route_kernel(const RouteArgs p)
         int my_idx = -1;
         float my_w = 0.0f;
         if (open) {
+            const T* row = static_cast<const T*>(p.logits) + t * p.ld;
             float x[NV];
-            bool nan = false;
+            int key[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 x[i] = lane + 32 * i < E ? to_f32(raw[i]) : kNegInf;
-                nan |= x[i] != x[i];
+                key[i] = order_key(x[i], lane + 32 * i, low_bits);
             }
-            const bool any_nan = __any_sync(kAll, nan);
-            LaneBest<NV> best;
-            best.scan(x, lane);
-            float top = warp_max(best.v1);
-            if (top != kNegInf || any_nan) {  // at least one expert to choose
+            Best3 best;
+            best.scan(key);
+            int top = __reduce_max_sync(kAll, best.v1);
+            float m;  // the largest logit, exactly: a low bit of 1e6 less would make exp(x - m) overflow
+            if constexpr (sizeof(T) == 2) {
+                m = key_value(top, low_bits);
+            } else {
+                m = kNegInf;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) m = fmaxf(m, x[i]);
+                m = warp_max(m);
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                x[i] = exp2_approx((x[i] - m) * kLog2e);
+                sum += x[i];
+            }
+            sum = warp_sum(sum);
+            const bool not_a_number = sum != sum;  // a NaN or +inf among the logits, or all of them masked (-inf less -inf)
+            int my_key = kNoChoice;
+            int chosen = 0;
+            for (; chosen < K && top >= kLowest; ++chosen) {
+                if (lane == chosen) my_key = top;
+                if (best.v1 == top) {
+                    best.v1 = best.v2, best.v2 = best.v3, best.v3 = kNoChoice;
+                    if (--best.held == 0) best.scan(key, top);  // one token in twenty with 8 choices among 32 lanes
+                }
+                top = __reduce_max_sync(kAll, best.v1);
+            }
+            if (my_key != kNoChoice) my_idx = low_bits - (my_key & low_bits);
+            bool again = not_a_number;
+            if constexpr (sizeof(T) == 4) {
+                const int next = __shfl_down_sync(kAll, my_key, 1);
+                const int behind = lane == chosen - 1 ? top : next;  // what was left behind the last choice
+                again |= __any_sync(kAll, lane < chosen && (my_key & ~low_bits) == (behind & ~low_bits));
+            }
+            if (again) choose_exactly<T, NV>(row, E, K, lane, my_idx);
+            if (__any_sync(kAll, my_idx >= 0)) {
                 ++used;
-                const float mx = top;
-                float my_logit = 0.0f;
-                int chosen = 0;
-                while (top != kNegInf) {
-                    const int e = __reduce_min_sync(kAll, best.v1 == top ? best.e1 : kMaxExperts);  // of equal logits the first expert
-                    if (lane == chosen) my_idx = e, my_logit = top;
-                    if (++chosen == K) break;
-                    if (best.e1 == e) {
-                        best.v1 = best.v2, best.e1 = best.e2, best.v2 = kNegInf;
-                        if (--best.held == 0) best.scan(x, lane, top, e);
-                    }
-                    top = warp_max(best.v1);
-                }
-                if (any_nan) {  // after every number, in the order of the experts
-                    int last = -1;
-                    while (chosen < K) {
-                        int e = kMaxExperts;
-#pragma unroll
-                        for (int i = NV - 1; i >= 0; --i)
-                            if (x[i] != x[i] && lane + 32 * i > last) e = lane + 32 * i;
-                        e = __reduce_min_sync(kAll, e);
-                        if (e == kMaxExperts) break;
-                        if (lane == chosen) my_idx = e, my_logit = __uint_as_float(0x7FC00000u);
-                        last = e;
-                        ++chosen;
-                    }
-                }
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    x[i] = exp2_approx((x[i] - mx) * kLog2e);
-                    sum += x[i];
-                }
-                const float inv = __frcp_rn(warp_sum(sum));
+                const float inv = __frcp_rn(sum);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
                 if (my_idx >= 0) {
-                    my_w = exp2_approx((my_logit - mx) * kLog2e) * inv;
+                    my_w = exp2_approx((to_f32(row[my_idx]) - m) * kLog2e) * inv;
                     atomicAdd(&s_count[my_idx], 1);
                 }
                 if (p.renorm) {
@@ -350,78 +401,95 @@ struct RouteGradArgs {
     int tokens, experts, top_k, renorm;
 };
 
+// One token per warp.  With E_i = exp(x_i - max) and S their sum: p_i = E_i / S, and sum_e p dp = (sum_i E_i base_i) / S + sum_j p_j g_j with
+// base_e = dloss E counts[e] / (N^2 top_k) and g_j what the weights' gradient gives choice j: every sum over experts is made from
+// values in registers.  The lanes write p (base - sum) for their experts, and after that the choices' own lanes write theirs again with
+// g_j in it.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256)
 route_grad_kernel(const RouteGradArgs p)
 {
-    extern __shared__ float s_given[];  // [8][experts]: what the weights' gradient gives the chosen experts of a warp's token, else 0
+    extern __shared__ float s_base[];  // [experts]
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int E = p.experts, K = p.top_k;
-    float* given = s_given + w * E;
-    for (int e = lane; e < E; e += 32) given[e] = 0.0f;
-    __syncwarp();
     grid_dependency_wait();
     float coef = 0.0f;
     if (p.dloss) {
         const float n = static_cast<float>(max(*p.num_tokens, 1ll));
         coef = *p.dloss * static_cast<float>(E) / (n * n * static_cast<float>(K));
     }
-    float base[NV];  // dloss * E * counts[e] / (N^2 top_k)
+    for (int e = threadIdx.x; e < E; e += 256) s_base[e] = p.dloss ? coef * static_cast<float>(p.counts[e]) : 0.0f;
+    __syncthreads();
+    float base[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) base[i] = (p.dloss && lane + 32 * i < E) ? coef * static_cast<float>(p.counts[lane + 32 * i]) : 0.0f;
-    for (long long t = static_cast<long long>(blockIdx.x) * 8 + w; t < p.tokens; t += gridDim.x * 8) {
+    for (int i = 0; i < NV; ++i) base[i] = lane + 32 * i < E ? s_base[lane + 32 * i] : 0.0f;
+    const long long step = static_cast<long long>(gridDim.x) * 8;
+    long long t = static_cast<long long>(blockIdx.x) * 8 + w;
+    constexpr bool AHEAD = NV <= 16;  // the next token is requested before this one is worked on
+    T raw[NV], raw_ahead[NV];
+    int my = -1, my_ahead = -1;
+    float gw = 0.0f, gw_ahead = 0.0f;
+    auto load = [&](long long token, T (&to)[NV], int& idx, float& g) {
+        if (token >= p.tokens) return;
+        const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + 32 * i < E) to[i] = row[lane + 32 * i];
+        if (lane < K) {
+            idx = p.idx[token * K + lane];
+            if (p.dweights) g = p.dweights[token * K + lane];
+        }
+    };
+    if constexpr (AHEAD) load(t, raw_ahead, my_ahead, gw_ahead);
+    for (; t < p.tokens; t += step) {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) raw[i] = raw_ahead[i];
+            my = my_ahead, gw = gw_ahead;
+            load(t + step, raw_ahead, my_ahead, gw_ahead);
+        } else {
+            load(t, raw, my, gw);
+        }
         const T* row = static_cast<const T*>(p.logits) + t * p.ld;
         T* out = static_cast<T*>(p.dlogits) + t * p.ld_out;
-        int my = lane < K ? p.idx[t * K + lane] : -1;
-        if (my >= E) my = -1;
-        const float gw = (p.dweights && my >= 0) ? p.dweights[t * K + lane] : 0.0f;
-        const bool in_use = __any_sync(kAll, my >= 0);
-        if (!in_use) {
+        const bool mine = my >= 0 && my < E;
+        if (!__any_sync(kAll, mine)) {  // not in use
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(0.0f);
             continue;
         }
-        float x[NV], mx = -__builtin_huge_valf();
+        const float my_logit = mine ? to_f32(row[my]) : 0.0f;
+        __syncwarp();  // dlogits may be the logits: every lane has read what it needs before the first one writes
+        float x[NV], mx = kNegInf;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            x[i] = lane + 32 * i < E ? to_f32(row[lane + 32 * i]) : -__builtin_huge_valf();
+            x[i] = lane + 32 * i < E ? to_f32(raw[i]) : kNegInf;
             mx = fmaxf(mx, x[i]);
         }
-        const float mine = my >= 0 ? to_f32(row[my]) : 0.0f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
-        float sum = 0.0f;
+        mx = warp_max(mx);
+        float sum = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             x[i] = exp2_approx((x[i] - mx) * kLog2e);
             sum += x[i];
+            dot = fmaf(x[i], base[i], dot);
         }
         const float inv = __frcp_rn(warp_sum(sum));
-        float g = gw;
-        if (p.dweights && p.renorm) {
-            // weights = p / S over the chosen: d/dp = (gw - sum gw * weights) / S
-            const float pj = my >= 0 ? exp2_approx((mine - mx) * kLog2e) * inv : 0.0f;
-            const float s = warp_sum(pj), dot = warp_sum(gw * pj);
+        const float pj = mine ? exp2_approx((my_logit - mx) * kLog2e) * inv : 0.0f;
+        float g = mine ? gw : 0.0f;
+        if (p.renorm && p.dweights) {
+            // weights = p / S over the choices: d/dp = (gw - sum gw * weights) / S
+            const float s = warp_sum(pj), gp = warp_sum(g * pj);
             const float inv_s = __frcp_rn(s);
-            g = (gw - dot * inv_s) * inv_s;
+            g = (g - gp * inv_s) * inv_s;
         }
-        if (my >= 0) atomicAdd(&given[my], g);
-        __syncwarp();
-        float dp[NV], dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            x[i] *= inv;
-            dp[i] = base[i] + (lane + 32 * i < E ? given[lane + 32 * i] : 0.0f);
-            dot = fmaf(x[i], dp[i], dot);
-        }
-        dot = warp_sum(dot);
+        dot = warp_sum(fmaf(dot, inv, mine ? pj * g : 0.0f));
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(x[i] * (dp[i] - dot));
+            if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(x[i] * inv * (base[i] - dot));
         __syncwarp();
-        if (my >= 0) given[my] = 0.0f;
-        __syncwarp();
+        if (mine) out[my] = from_f32<T>(pj * (s_base[my] + g - dot));
     }
 }
 
@@ -468,7 +536,7 @@ template <typename T, int NV>
 int launch_route_grad_as(const RouteGradArgs& p, int sms, cudaStream_t st)
 {
     const int blocks = static_cast<int>(std::min((p.tokens + 7ll) / 8, 8ll * sms));
-    ASCB200_CUDA(launch_pdl(route_grad_kernel<T, NV>, blocks, 256, 8 * static_cast<size_t>(p.experts) * 4, st, p));
+    ASCB200_CUDA(launch_pdl(route_grad_kernel<T, NV>, blocks, 256, static_cast<size_t>(p.experts) * 4, st, p));
     return ASCB200_OK;
 }
 template <typename T>

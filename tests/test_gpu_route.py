@@ -306,3 +306,21 @@ def test_captured_and_replayed():
         near(l, torch.tensor([want[5]]), 200 * F * want[5], "loss")
     graph.destroy()
     ab.lib().ascb200_stream_destroy(side)
+
+
+@pytest.mark.parametrize("e", [8, 60, 256, 1000])
+def test_close_and_large_logits(e):
+    """fp32 logits that agree in all but their last bits, among few and among many; values whose last bit is large."""
+    x = torch.randn(300, e, generator=gen(e))
+    near_one = (torch.ones(300, e).view(torch.int32) + torch.randint(0, 40, (300, e), generator=gen(e + 1), dtype=torch.int32)).view(torch.float32)
+    pick = torch.rand(300, e, generator=gen(e + 2)) < 0.3
+    x[:150] = torch.where(pick[:150], 2 * near_one[:150], x[:150])   # ties and near ties at the top
+    x[150:200] = -near_one[150:200]                                  # everywhere, negative
+    x[200:250] = 0.25                                                # all equal
+    for renorm in (0, 1):
+        _, out = forward(x, torch.float32, min(8, e), renorm)
+        check(x, out, None, min(8, e), renorm)
+    big = torch.randn(64, e, generator=gen(e + 3)) * torch.tensor([1e3, 1e6, 1e12, 1e30]).repeat(16)[:, None]
+    _, out = forward(big, torch.float32, min(8, e), 1)
+    idx, w, counts, n, _, _, _ = reference(big, None, min(8, e), 1)
+    assert torch.equal(out["idx"].t.cpu().long(), idx) and torch.isfinite(out["w"].t).all() and torch.equal(out["counts"].t[0].cpu(), counts)
