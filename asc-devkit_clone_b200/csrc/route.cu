@@ -32,6 +32,12 @@ __device__ __forceinline__ float exp2_approx(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float rcp_approx(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll
@@ -178,56 +184,88 @@ __device__ __forceinline__ float loss_of(const RouteArgs& p, float total, float 
     return total * inv_n * (static_cast<float>(p.experts) / static_cast<float>(p.top_k));
 }
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+// A block has a run of consecutive tokens, which it takes in tiles of one token per thread: it first writes down which of the tile's tokens
+// are valid (and closes the others), then its warps share those evenly.  FULL: the experts are 32 NV exactly.
+template <typename T, int NV, bool FULL>
+__global__ void __launch_bounds__(kRouteWarps * 32, NV <= 8 ? 2 : 1)
 route_kernel(const RouteArgs p)
 {
-    extern __shared__ float s_prob[];  // [kRouteWarps][experts], then int [experts] counts
+    constexpr int TILE = kRouteWarps * 32;
+    constexpr int low_bits = 32 * NV - 1;  // at most 1023; the numbers of all lanes' experts fit
+    constexpr bool AHEAD = NV <= 16;       // the next token's logits are requested before this one's are worked on
+    extern __shared__ float s_prob[];      // [kRouteWarps][experts], then int [experts] counts
     __shared__ int s_tokens[kRouteWarps];
     __shared__ float s_part[kRouteWarps];
+    __shared__ uint16_t s_list[TILE];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int E = p.experts, K = p.top_k;
+    const int E = FULL ? 32 * NV : p.experts, K = p.top_k;
     int* s_count = reinterpret_cast<int*>(s_prob + kRouteWarps * E);
     for (int e = threadIdx.x; e < E; e += kRouteWarps * 32) s_count[e] = 0;
-    __syncthreads();
     grid_dependency_wait();
     float acc[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) acc[i] = 0.0f;
     int used = 0;
-    const long long step = static_cast<long long>(gridDim.x) * kRouteWarps;
-    long long t = static_cast<long long>(blockIdx.x) * kRouteWarps + w;
-    constexpr int low_bits = 32 * NV - 1;  // at most 1023; the numbers of all lanes' experts fit
-    constexpr bool AHEAD = NV <= 16;  // the next token's logits are requested before this one's are worked on
-    T raw[NV], ahead[NV];
-    uint8_t open = 1, open_ahead = 1;
-    auto load = [&](long long token, T (&to)[NV], uint8_t& valid) {
-        if (token >= p.tokens) return;
-        if (p.valid) valid = p.valid[token];
-        const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+    const int run = static_cast<int>((p.tokens + static_cast<long long>(gridDim.x) - 1) / gridDim.x);
+    const long long first = static_cast<long long>(blockIdx.x) * run;
+    const int mine = static_cast<int>(max(0ll, min(static_cast<long long>(run), p.tokens - first)));
+    for (int tile = 0; tile < mine; tile += TILE) {
+        const long long token0 = first + tile;
+        int count = min(TILE, mine - tile);
+        __syncthreads();  // the zeroed counts; the list of the tile before
+        if (p.valid) {
+            const bool inside = static_cast<int>(threadIdx.x) < count;
+            const bool open = inside && p.valid[token0 + threadIdx.x] != 0;
+            const unsigned votes = __ballot_sync(kAll, open);
+            if (lane == 0) s_tokens[w] = __popc(votes);
+            __syncthreads();
+            int before = 0, all = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (lane + 32 * i < E) to[i] = row[lane + 32 * i];
-    };
-    if constexpr (AHEAD) load(t, ahead, open_ahead);
-    for (; t < p.tokens; t += step) {
-        if constexpr (AHEAD) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) raw[i] = ahead[i];
-            open = open_ahead;
-            load(t + step, ahead, open_ahead);
-        } else {
-            load(t, raw, open);
+            for (int i = 0; i < kRouteWarps; ++i) {
+                before += i < w ? s_tokens[i] : 0;
+                all += s_tokens[i];
+            }
+            if (open) {
+                s_list[before + __popc(votes & ((1u << lane) - 1))] = static_cast<uint16_t>(threadIdx.x);
+            } else if (inside) {
+                for (int j = 0; j < K; ++j) {
+                    p.idx[(token0 + threadIdx.x) * K + j] = -1;
+                    p.weights[(token0 + threadIdx.x) * K + j] = 0.0f;
+                }
+            }
+            count = all;
+            __syncthreads();
         }
-        int my_idx = -1;
-        float my_w = 0.0f;
-        if (open) {
-            const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+        const T* rows = static_cast<const T*>(p.logits) + token0 * p.ld + lane;
+        int* idx_out = p.idx + token0 * K + lane;
+        float* weights_out = p.weights + token0 * K + lane;
+        auto load = [&](int j, const T*& row, T (&to)[NV]) {
+            const int t = p.valid ? s_list[min(j, TILE - 1)] : j;
+            row = rows + t * p.ld;
+            if (j >= count) return t;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (FULL || lane + 32 * i < E) to[i] = row[32 * i];
+            return t;
+        };
+        T raw[NV], ahead[NV];
+        const T *row, *row_ahead;
+        int t, t_ahead = 0;
+        if constexpr (AHEAD) t_ahead = load(w, row_ahead, ahead);
+        for (int j = w; j < count; j += kRouteWarps) {
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) raw[i] = ahead[i];
+                row = row_ahead, t = t_ahead;
+                t_ahead = load(j + kRouteWarps, row_ahead, ahead);
+            } else {
+                t = load(j, row, raw);
+            }
             float x[NV];
             int key[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                x[i] = lane + 32 * i < E ? to_f32(raw[i]) : kNegInf;
+                x[i] = FULL || lane + 32 * i < E ? to_f32(raw[i]) : kNegInf;
                 key[i] = order_key(x[i], lane + 32 * i, low_bits);
             }
             Best3 best;
@@ -260,34 +298,36 @@ route_kernel(const RouteArgs p)
                 }
                 top = __reduce_max_sync(kAll, best.v1);
             }
-            if (my_key != kNoChoice) my_idx = low_bits - (my_key & low_bits);
+            int my_idx = my_key != kNoChoice ? low_bits - (my_key & low_bits) : -1;
             bool again = not_a_number;
             if constexpr (sizeof(T) == 4) {
                 const int next = __shfl_down_sync(kAll, my_key, 1);
                 const int behind = lane == chosen - 1 ? top : next;  // what was left behind the last choice
-                again |= __any_sync(kAll, lane < chosen && (my_key & ~low_bits) == (behind & ~low_bits));
+                again |= __any_sync(kAll, lane < chosen && ((my_key ^ behind) & ~low_bits) == 0);
             }
-            if (again) choose_exactly<T, NV>(row, E, K, lane, my_idx);
+            if (again) choose_exactly<T, NV>(row - lane, E, K, lane, my_idx);
+            float my_w = 0.0f;
             if (__any_sync(kAll, my_idx >= 0)) {
                 ++used;
-                const float inv = __frcp_rn(sum);
+                const float inv = rcp_approx(sum);
 #pragma unroll
                 for (int i = 0; i < NV; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
                 if (my_idx >= 0) {
-                    my_w = exp2_approx((to_f32(row[my_idx]) - m) * kLog2e) * inv;
+                    my_w = exp2_approx((to_f32(row[my_idx - lane]) - m) * kLog2e) * inv;
                     atomicAdd(&s_count[my_idx], 1);
                 }
                 if (p.renorm) {
                     const float total = warp_sum(my_w);  // lanes without a choice hold 0
-                    if (my_idx >= 0) my_w = __fdiv_rn(my_w, total);
+                    if (my_idx >= 0) my_w *= rcp_approx(total);
                 }
             }
-        }
-        if (lane < K) {
-            p.idx[t * K + lane] = my_idx;
-            p.weights[t * K + lane] = my_w;
+            if (lane < K) {
+                idx_out[static_cast<long long>(t) * K] = my_idx;
+                weights_out[static_cast<long long>(t) * K] = my_w;
+            }
         }
     }
+    __syncthreads();  // every count is in; s_tokens is free again
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (lane + 32 * i < E) s_prob[w * E + lane + 32 * i] = acc[i];
@@ -405,13 +445,13 @@ struct RouteGradArgs {
 // base_e = dloss E counts[e] / (N^2 top_k) and g_j what the weights' gradient gives choice j: every sum over experts is made from
 // values in registers.  The lanes write p (base - sum) for their experts, and after that the choices' own lanes write theirs again with
 // g_j in it.
-template <typename T, int NV>
+template <typename T, int NV, bool FULL>
 __global__ void __launch_bounds__(256)
 route_grad_kernel(const RouteGradArgs p)
 {
     extern __shared__ float s_base[];  // [experts]
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int E = p.experts, K = p.top_k;
+    const int E = FULL ? 32 * NV : p.experts, K = p.top_k;
     grid_dependency_wait();
     float coef = 0.0f;
     if (p.dloss) {
@@ -422,7 +462,7 @@ route_grad_kernel(const RouteGradArgs p)
     __syncthreads();
     float base[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) base[i] = lane + 32 * i < E ? s_base[lane + 32 * i] : 0.0f;
+    for (int i = 0; i < NV; ++i) base[i] = FULL || lane + 32 * i < E ? s_base[lane + 32 * i] : 0.0f;
     const long long step = static_cast<long long>(gridDim.x) * 8;
     long long t = static_cast<long long>(blockIdx.x) * 8 + w;
     constexpr bool AHEAD = NV <= 16;  // the next token is requested before this one is worked on
@@ -434,7 +474,7 @@ route_grad_kernel(const RouteGradArgs p)
         const T* row = static_cast<const T*>(p.logits) + token * p.ld;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (lane + 32 * i < E) to[i] = row[lane + 32 * i];
+            if (FULL || lane + 32 * i < E) to[i] = row[lane + 32 * i];
         if (lane < K) {
             idx = p.idx[token * K + lane];
             if (p.dweights) g = p.dweights[token * K + lane];
@@ -456,7 +496,7 @@ route_grad_kernel(const RouteGradArgs p)
         if (!__any_sync(kAll, mine)) {  // not in use
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(0.0f);
+                if (FULL || lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(0.0f);
             continue;
         }
         const float my_logit = mine ? to_f32(row[my]) : 0.0f;
@@ -464,7 +504,7 @@ route_grad_kernel(const RouteGradArgs p)
         float x[NV], mx = kNegInf;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            x[i] = lane + 32 * i < E ? to_f32(raw[i]) : kNegInf;
+            x[i] = FULL || lane + 32 * i < E ? to_f32(raw[i]) : kNegInf;
             mx = fmaxf(mx, x[i]);
         }
         mx = warp_max(mx);
@@ -475,19 +515,19 @@ route_grad_kernel(const RouteGradArgs p)
             sum += x[i];
             dot = fmaf(x[i], base[i], dot);
         }
-        const float inv = __frcp_rn(warp_sum(sum));
+        const float inv = rcp_approx(warp_sum(sum));
         const float pj = mine ? exp2_approx((my_logit - mx) * kLog2e) * inv : 0.0f;
         float g = mine ? gw : 0.0f;
         if (p.renorm && p.dweights) {
             // weights = p / S over the choices: d/dp = (gw - sum gw * weights) / S
             const float s = warp_sum(pj), gp = warp_sum(g * pj);
-            const float inv_s = __frcp_rn(s);
+            const float inv_s = rcp_approx(s);
             g = (g - gp * inv_s) * inv_s;
         }
         dot = warp_sum(fmaf(dot, inv, mine ? pj * g : 0.0f));
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(x[i] * inv * (base[i] - dot));
+            if (FULL || lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(x[i] * inv * (base[i] - dot));
         __syncwarp();
         if (mine) out[my] = from_f32<T>(pj * (s_base[my] + g - dot));
     }
@@ -504,39 +544,46 @@ size_t route_workspace(int tokens, int experts)
     return blocks == 1 ? 0 : static_cast<size_t>(blocks) * (2 * static_cast<size_t>(experts) + 1) * 4;
 }
 
-template <typename T, int NV>
+template <typename T, int NV, bool FULL>
 int launch_route_as(const RouteArgs& p, int blocks, cudaStream_t st)
 {
     const size_t smem = (kRouteWarps + 1) * static_cast<size_t>(p.experts) * 4;
-    if (smem > 48 * 1024) {  // more than 722 experts
+    if (smem > 46 * 1024) {  // more than 692 experts: beyond what a launch may take unasked
         static bool configured[16] = {};
         int dev = 0;
         ASCB200_CUDA(cudaGetDevice(&dev));
         if (!configured[dev & 15]) {
-            ASCB200_CUDA(cudaFuncSetAttribute(route_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kRouteWarps + 1) * kMaxExperts * 4));
+            ASCB200_CUDA(cudaFuncSetAttribute(route_kernel<T, NV, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kRouteWarps + 1) * kMaxExperts * 4));
             configured[dev & 15] = true;
         }
     }
-    ASCB200_CUDA(launch_pdl(route_kernel<T, NV>, blocks, kRouteWarps * 32, smem, st, p));
+    ASCB200_CUDA(launch_pdl(route_kernel<T, NV, FULL>, blocks, kRouteWarps * 32, smem, st, p));
     if (blocks > 1) ASCB200_CUDA(launch_pdl(route_finish_kernel, kFinishBlocks, kFinishWarps * 32, 0, st, p, blocks));
     return ASCB200_OK;
+}
+template <typename T, int NV>
+int launch_route_nv(const RouteArgs& p, int blocks, cudaStream_t st)
+{
+    return p.experts == 32 * NV ? launch_route_as<T, NV, true>(p, blocks, st) : launch_route_as<T, NV, false>(p, blocks, st);
 }
 template <typename T>
 int launch_route(const RouteArgs& p, int blocks, cudaStream_t st)
 {
-    if (p.experts <= 32) return launch_route_as<T, 1>(p, blocks, st);
-    if (p.experts <= 64) return launch_route_as<T, 2>(p, blocks, st);
-    if (p.experts <= 128) return launch_route_as<T, 4>(p, blocks, st);
-    if (p.experts <= 256) return launch_route_as<T, 8>(p, blocks, st);
-    if (p.experts <= 512) return launch_route_as<T, 16>(p, blocks, st);
-    return launch_route_as<T, 32>(p, blocks, st);
+    if (p.experts <= 32) return launch_route_nv<T, 1>(p, blocks, st);
+    if (p.experts <= 64) return launch_route_nv<T, 2>(p, blocks, st);
+    if (p.experts <= 128) return launch_route_nv<T, 4>(p, blocks, st);
+    if (p.experts <= 256) return launch_route_nv<T, 8>(p, blocks, st);
+    if (p.experts <= 512) return launch_route_nv<T, 16>(p, blocks, st);
+    return launch_route_nv<T, 32>(p, blocks, st);
 }
 
 template <typename T, int NV>
 int launch_route_grad_as(const RouteGradArgs& p, int sms, cudaStream_t st)
 {
     const int blocks = static_cast<int>(std::min((p.tokens + 7ll) / 8, 8ll * sms));
-    ASCB200_CUDA(launch_pdl(route_grad_kernel<T, NV>, blocks, 256, static_cast<size_t>(p.experts) * 4, st, p));
+    const size_t smem = static_cast<size_t>(p.experts) * 4;
+    if (p.experts == 32 * NV) ASCB200_CUDA(launch_pdl(route_grad_kernel<T, NV, true>, blocks, 256, smem, st, p));
+    else ASCB200_CUDA(launch_pdl(route_grad_kernel<T, NV, false>, blocks, 256, smem, st, p));
     return ASCB200_OK;
 }
 template <typename T>
