@@ -875,6 +875,66 @@ __device__ __forceinline__ void add_residual(const EpiParams& e, const ResidualC
     }
 }
 
+// 32 x 32 outputs of a warp whose rows do not start on 16 bytes (an odd n, packed rows): through the warp's staging buffer, so that the
+// lanes write runs of 32 columns of a row instead of one element of 32 rows each.  Two-byte types take the chunk at once, fp32 in two
+// halves of 16 columns.
+template <int DT>
+__device__ __forceinline__ void store_chunk_by_runs(void* base, long long ld, uint32_t smem, int lane, int row_base, int rows, int col0, int ncols, const float (&f)[32])
+{
+    const uint32_t sw = (lane >> 1) & 3;  // 16-byte pieces of a 64-byte row, XOR-swizzled: neither side collides on banks
+    if constexpr (DT == OUT_F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                st_shared_v4(smem + lane * 64 + ((j ^ sw) << 4), __float_as_uint(f[h * 16 + 4 * j]), __float_as_uint(f[h * 16 + 4 * j + 1]),
+                             __float_as_uint(f[h * 16 + 4 * j + 2]), __float_as_uint(f[h * 16 + 4 * j + 3]));
+            __syncwarp();
+            const int c = lane & 15, col = h * 16 + c;
+            for (int r = lane >> 4; r < rows; r += 2) {
+                uint32_t v;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(smem + r * 64 + (((c >> 2) ^ ((r >> 1) & 3)) << 4) + (c & 3) * 4) : "memory");
+                if (col < ncols) static_cast<uint32_t*>(base)[static_cast<size_t>(row_base + r) * static_cast<size_t>(ld) + col0 + col] = v;
+            }
+        }
+    } else {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = DT == OUT_F16 ? pack_f16x2_sat(f[2 * j], f[2 * j + 1]) : pack_bf16x2(f[2 * j], f[2 * j + 1]);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) st_shared_v4(smem + lane * 64 + ((j ^ sw) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        __syncwarp();
+        uint16_t* out = static_cast<uint16_t*>(base) + static_cast<size_t>(row_base) * static_cast<size_t>(ld) + col0 + lane;
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r, out += ld) {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(smem + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2) : "memory");
+            if (lane < ncols) *out = v;
+        }
+    }
+}
+// The same way for a two-byte residual: the lanes read runs of a row, every lane then has its own row.
+__device__ __forceinline__ void load_residual_by_runs(const EpiParams& e, uint32_t smem, int lane, int row_base, int rows, int col0, int ncols, ResidualChunk& r)
+{
+    __syncwarp();
+    const uint16_t* src = static_cast<const uint16_t*>(e.residual) + static_cast<size_t>(row_base) * static_cast<size_t>(e.ld_residual) + col0 + lane;
+#pragma unroll 8
+    for (int i = 0; i < rows; ++i) {
+        const uint16_t v = lane < ncols ? src[static_cast<size_t>(i) * static_cast<size_t>(e.ld_residual)] : static_cast<uint16_t>(0);
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(smem + i * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2), "h"(v) : "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float a, b, c, d;
+        ld_shared_v4(smem + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), a, b, c, d);
+        r.v[j] = make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+    }
+    __syncwarp();
+}
+
 struct LinearPre {
     float tok;
     float4 ch, bias;
@@ -918,7 +978,7 @@ __device__ __forceinline__ LinearPre linear_preload(const GemmParams& p, const T
             r.bias = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
-    if (p.epi.c_dtype != OUT_F32) load_residual16(p.epi, row_ok, row, first, end - first, r.res);
+    if (p.epi.c_dtype != OUT_F32 && p.epi.vec_residual) load_residual16(p.epi, row_ok, row, first, end - first, r.res);
     return r;
 }
 
@@ -937,13 +997,23 @@ __device__ __forceinline__ void linear_tile(const GemmParams& p, const TileInfo&
     __syncwarp();
     const int row_base = t.row0 + quad * 32, n_end = min(p.n, t.n_end);
     const bool stage_c = (DT == OUT_F16 || DT == OUT_BF16) && e.tma_c && !t.m64;
+    // rows that do not start on 16 bytes go through the staging buffer where no bulk store of y may still be reading it, else lane by lane
+    const bool by_runs = !stage_c;
+    const int base_row = t.m64 ? t.row0 + quad * 16 : row_base, rows = max(0, min(t.m64 ? 16 : 32, t.row_end - base_row));
 #pragma unroll 1
     for (int c = chunk0; c < chunk1; ++c) {
         const int col0 = t.n0 + c * 32;
         if (col0 >= n_end) break;  // uniform across the warp
         const int ncols = min(32, n_end - col0);
         ResidualChunk ahead;
-        if constexpr (DT != OUT_F32) load_residual16(e, row_ok && c + 1 < chunk1, row, col0 + 32, n_end - col0 - 32, ahead);
+        if constexpr (DT != OUT_F32) {
+            if (e.vec_residual) {
+                load_residual16(e, row_ok && c + 1 < chunk1, row, col0 + 32, n_end - col0 - 32, ahead);
+            } else if (e.residual) {
+                if (by_runs) load_residual_by_runs(e, stage_smem, lane, base_row, rows, col0, ncols, pre.res);
+                else load_residual16(e, row_ok, row, col0, ncols, pre.res);
+            }
+        }
         uint32_t r[32];
         tmem_ld_32x32(t_addr + c * 32, r);
         tmem_ld_wait();
@@ -982,7 +1052,10 @@ __device__ __forceinline__ void linear_tile(const GemmParams& p, const TileInfo&
         }
         const int unused[32] = {};
         if constexpr (!ACC_INT) {
-            if (e.c2 && row_ok) store_row32<DT>(e.c2, e.ldc2, e.vec_c2, row, col0, ncols, f, unused);
+            if (e.c2) {
+                if (by_runs && !e.vec_c2) store_chunk_by_runs<DT>(e.c2, e.ldc2, stage_smem, lane, base_row, rows, col0, ncols, f);
+                else if (row_ok) store_row32<DT>(e.c2, e.ldc2, e.vec_c2, row, col0, ncols, f, unused);
+            }
         }
         ASCB200_ACT_SWITCH(e.lin_act, {
 #pragma unroll
@@ -990,14 +1063,15 @@ __device__ __forceinline__ void linear_tile(const GemmParams& p, const TileInfo&
         })
         if (e.residual) add_residual<DT>(e, pre.res, row_ok, row, col0, ncols, f);
         if constexpr (DT != OUT_F32) {
-            pre.res = ahead;
+            if (e.vec_residual) pre.res = ahead;
             // a chunk that the tile or the matrix only half owns is stored from registers (see epilogue_tile)
             if (stage_c && ncols == 32) {
                 stage_store32<DT>(&outs.c, stage_smem, false, lane, row_base, col0, f, unused);
                 continue;
             }
         }
-        if (row_ok) store_row32<DT>(e.c, e.ldc, e.vec_c, row, col0, ncols, f, unused);
+        if (by_runs && !e.vec_c) store_chunk_by_runs<DT>(e.c, e.ldc, stage_smem, lane, base_row, rows, col0, ncols, f);
+        else if (row_ok) store_row32<DT>(e.c, e.ldc, e.vec_c, row, col0, ncols, f, unused);
     }
 }
 

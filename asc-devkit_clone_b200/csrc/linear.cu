@@ -20,11 +20,15 @@ namespace {
 // memory is used by one instruction for all tokens.  A sum over k does not care for the order of k as long as both operands agree,
 // so a lane feeds the instructions straight from 16 contiguous bytes of a weight row (its first two words are the lane's k slots of
 // one instruction, the last two those of the next): 64 bytes of a row per pair of instructions, no shuffles and no shared memory.
-// A block owns 16 weight rows; its warps take 256-byte pieces of them in turn and add their sums in warp order through shared memory.
+//
+// Two or three blocks per SM, all resident, each with an equal run of weight rows, one to three tiles of 16 in a pass: what is loaded of
+// the tokens serves every tile of the pass.  A block's eight warps take 256-byte pieces of the rows in turn and add their sums in warp
+// order through shared memory at the end of the pass.
 constexpr int kRowsMaxTokens = 16;
-constexpr int kRowsTile = 16;   // weight rows per block
+constexpr int kRowsTile = 16;
 constexpr int kRowsWarps = 8;
-constexpr int kRowsUnroll = 4;  // 64-byte chunks per warp and step
+constexpr int kRowsUnroll = 4;        // 64-byte chunks per warp and step
+constexpr int kRowsBlocksPerSm(int groups) { return groups == 1 ? 3 : 2; }  // by groups of eight tokens: what registers allow
 
 struct RowsArgs {
     const uint8_t* x;
@@ -45,23 +49,29 @@ template <int KIND>
 __device__ __forceinline__ void mma_16x8(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
     if constexpr (KIND == ASCB200_KIND_S8) {
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     } else {
         float* f = reinterpret_cast<float*>(c);
         if constexpr (KIND == ASCB200_KIND_F16)
-            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                          : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3])
                          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
         else
-            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                          : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3])
                          : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
 }
 
-// 16 bytes at `off` of a row of `bytes` bytes; what lies behind its end reads as zero and is not touched.
+template <int KIND>
+__device__ __forceinline__ uint32_t add_bits(uint32_t a, uint32_t b)
+{
+    return KIND == ASCB200_KIND_S8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+
+// 16 bytes at `off` of a row of `bytes` bytes; what lies behind its end reads as zero and is not touched.  STREAM: read once.
 template <bool STREAM>
 __device__ __forceinline__ uint4 load_piece(const uint8_t* row, int off, int bytes)
 {
@@ -90,84 +100,118 @@ __device__ __forceinline__ float as_f32<__half>(__half v) { return __half2float(
 template <>
 __device__ __forceinline__ float as_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-template <int KIND, int NT, typename OT>  // NT: groups of eight tokens
-__global__ void __launch_bounds__(kRowsWarps * 32)
+template <int KIND, int NT, int R, typename OT>  // NT: groups of eight tokens; R: tiles of 16 rows per pass
+__global__ void __launch_bounds__(kRowsWarps * 32, kRowsBlocksPerSm(NT))
 linear_rows_kernel(const RowsArgs p)
 {
-    __shared__ uint32_t part[kRowsWarps][NT * 8][kRowsTile + 1];
+    constexpr int STEP = kRowsUnroll * 64;
+    constexpr int CHAINS = NT == 1 ? 2 : 1;  // independent chains of instructions per tile: two in either case
+    __shared__ uint32_t part[kRowsWarps][NT * 8][R * kRowsTile + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, q = lane & 3;
-    const int n0 = blockIdx.x * kRowsTile;
-    const uint8_t* w0 = p.w + min(n0 + g, p.n - 1) * p.ldw;
-    const uint8_t* w1 = p.w + min(n0 + g + 8, p.n - 1) * p.ldw;
-    grid_dependency_wait();
-    uint32_t acc[NT][4] = {};
-    for (int base = warp * (kRowsUnroll * 64); base < p.k_bytes; base += kRowsWarps * kRowsUnroll * 64) {
-        uint4 a[kRowsUnroll], b[kRowsUnroll], x[NT][kRowsUnroll];
-#pragma unroll
-        for (int u = 0; u < kRowsUnroll; ++u) {
-            const int off = base + u * 64 + q * 16;
-            a[u] = load_piece<true>(w0, off, p.k_bytes);
-            b[u] = load_piece<true>(w1, off, p.k_bytes);
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int u = 0; u < kRowsUnroll; ++u) {
-                x[t][u] = make_uint4(0u, 0u, 0u, 0u);
-                if (t * 8 + g < p.m) x[t][u] = load_piece<false>(p.x + (t * 8 + g) * p.ldx, base + u * 64 + q * 16, p.k_bytes);
-            }
-#pragma unroll
-        for (int u = 0; u < kRowsUnroll; ++u)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                mma_16x8<KIND>(acc[t], a[u].x, b[u].x, a[u].y, b[u].y, x[t][u].x, x[t][u].y);
-                mma_16x8<KIND>(acc[t], a[u].z, b[u].z, a[u].w, b[u].w, x[t][u].z, x[t][u].w);
-            }
+    const int row0 = static_cast<int>(static_cast<long long>(blockIdx.x) * p.n / gridDim.x);
+    const int row1 = static_cast<int>((static_cast<long long>(blockIdx.x) + 1) * p.n / gridDim.x);
+    // While the kernel before this one drains, ask L2 for the warp's first pieces (hints: nothing is read into the program yet).
+    if (row0 + lane < row1 && warp * STEP < p.k_bytes) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.w + (row0 + lane) * p.ldw + warp * STEP));
+        if (warp * STEP + 128 < p.k_bytes) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.w + (row0 + lane) * p.ldw + warp * STEP + 128));
     }
-    // accumulators: rows g and g + 8, tokens 2 q and 2 q + 1
+    grid_dependency_wait();
+    for (int n0 = row0; n0 < row1; n0 += R * kRowsTile) {
+        const int tiles = min(R, (row1 - n0 + kRowsTile - 1) / kRowsTile);
+        uint32_t acc[R][NT][CHAINS][4] = {};
+        for (int base = warp * STEP; base < p.k_bytes; base += kRowsWarps * STEP) {
+            uint4 x[NT][kRowsUnroll];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+            for (int r = 0; r < R; ++r) {
+                if (r >= tiles) break;  // the same for the whole block
+                const int n = n0 + r * kRowsTile + g;
+                const uint8_t* w0 = p.w + n * p.ldw;
+                const uint8_t* w1 = w0 + 8 * p.ldw;
+                const int bytes0 = n < row1 ? p.k_bytes : 0, bytes1 = n + 8 < row1 ? p.k_bytes : 0;  // rows behind the run count as empty
+                uint4 a[kRowsUnroll], b[kRowsUnroll];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) part[warp][t * 8 + 2 * q + (j & 1)][g + (j >> 1) * 8] = acc[t][j];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NT * 8 * kRowsTile; i += kRowsWarps * 32) {
-        const int token = i / kRowsTile, col = i % kRowsTile, n = n0 + col;
-        if (token >= p.m || n >= p.n) continue;
-        float f;
-        if constexpr (KIND == ASCB200_KIND_S8) {
-            int s = 0;
+                for (int u = 0; u < kRowsUnroll; ++u) {
+                    const int off = base + u * 64 + q * 16;
+                    a[u] = load_piece<true>(w0, off, bytes0);
+                    b[u] = load_piece<true>(w1, off, bytes1);
+                }
+                if (r == 0) {
 #pragma unroll
-            for (int v = 0; v < kRowsWarps; ++v) s += static_cast<int>(part[v][token][col]);
-            f = static_cast<float>(s) * p.ch[n];
-            if (p.tok) f *= p.tok[token];
-        } else {
-            f = 0.0f;
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int v = 0; v < kRowsWarps; ++v) f += __uint_as_float(part[v][token][col]);
+                        for (int u = 0; u < kRowsUnroll; ++u) {
+                            x[t][u] = make_uint4(0u, 0u, 0u, 0u);
+                            if (t * 8 + g < p.m) x[t][u] = load_piece<false>(p.x + (t * 8 + g) * p.ldx, base + u * 64 + q * 16, p.k_bytes);
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < kRowsUnroll; ++u)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        mma_16x8<KIND>(acc[r][t][0], a[u].x, b[u].x, a[u].y, b[u].y, x[t][u].x, x[t][u].y);
+                        mma_16x8<KIND>(acc[r][t][CHAINS - 1], a[u].z, b[u].z, a[u].w, b[u].w, x[t][u].z, x[t][u].w);
+                    }
+            }
         }
-        if (p.bias) f += p.bias_f32 ? static_cast<const float*>(p.bias)[n] : as_f32(static_cast<const OT*>(p.bias)[n]);
-        if (p.z) static_cast<OT*>(p.z)[token * p.ldz + n] = rounded<OT>(f);
-        ASCB200_ACT_SWITCH(p.act, { f = act::value<ACT>(f); })
-        if (p.residual) f += as_f32(static_cast<const OT*>(p.residual)[token * p.ld_residual + n]);
-        static_cast<OT*>(p.y)[token * p.ldy + n] = rounded<OT>(f);
+        // accumulators: rows g and g + 8, tokens 2 q and 2 q + 1
+        if (n0 > row0) __syncthreads();  // the pass before has been read
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[warp][t * 8 + 2 * q + (j & 1)][r * kRowsTile + g + (j >> 1) * 8] = CHAINS == 2 ? add_bits<KIND>(acc[r][t][0][j], acc[r][t][CHAINS - 1][j]) : acc[r][t][0][j];
+        __syncthreads();
+        constexpr int cols = R * kRowsTile;
+        for (int i = threadIdx.x; i < NT * 8 * cols; i += kRowsWarps * 32) {
+            const int token = i / cols, col = i % cols, n = n0 + col;
+            if (token >= p.m || n >= row1) continue;
+            float f;
+            if constexpr (KIND == ASCB200_KIND_S8) {
+                int s = 0;
+#pragma unroll
+                for (int v = 0; v < kRowsWarps; ++v) s += static_cast<int>(part[v][token][col]);
+                f = static_cast<float>(s) * p.ch[n];
+                if (p.tok) f *= p.tok[token];
+            } else {
+                f = 0.0f;
+#pragma unroll
+                for (int v = 0; v < kRowsWarps; ++v) f += __uint_as_float(part[v][token][col]);
+            }
+            if (p.bias) f += p.bias_f32 ? static_cast<const float*>(p.bias)[n] : as_f32(static_cast<const OT*>(p.bias)[n]);
+            if (p.z) static_cast<OT*>(p.z)[token * p.ldz + n] = rounded<OT>(f);
+            ASCB200_ACT_SWITCH(p.act, { f = act::value<ACT>(f); })
+            if (p.residual) f += as_f32(static_cast<const OT*>(p.residual)[token * p.ld_residual + n]);
+            static_cast<OT*>(p.y)[token * p.ldy + n] = rounded<OT>(f);
+        }
     }
 }
 
-template <int KIND, typename OT>
-int launch_rows_as(const RowsArgs& p, cudaStream_t st)
+template <int KIND, int NT, int R, typename OT>
+int launch_rows_as(const RowsArgs& p, unsigned grid, cudaStream_t st)
 {
-    const unsigned grid = static_cast<unsigned>((p.n + kRowsTile - 1) / kRowsTile);
-    if (p.m <= 8) ASCB200_CUDA(launch_pdl(linear_rows_kernel<KIND, 1, OT>, grid, kRowsWarps * 32, 0, st, p));
-    else ASCB200_CUDA(launch_pdl(linear_rows_kernel<KIND, 2, OT>, grid, kRowsWarps * 32, 0, st, p));
+    ASCB200_CUDA(launch_pdl(linear_rows_kernel<KIND, NT, R, OT>, grid, kRowsWarps * 32, 0, st, p));
     return ASCB200_OK;
 }
-template <int KIND>
-int launch_rows(const RowsArgs& p, int y_dtype, cudaStream_t st)
+template <int KIND, typename OT>
+int launch_rows_of(const RowsArgs& p, int sms, cudaStream_t st)
 {
-    if (y_dtype == ASCB200_F16) return launch_rows_as<KIND, __half>(p, st);
-    if (y_dtype == ASCB200_BF16) return launch_rows_as<KIND, __nv_bfloat16>(p, st);
-    return launch_rows_as<KIND, float>(p, st);
+    // a run of at least as many rows as there may be tokens: with fewer, the tokens would be read more often than the weights
+    const int groups = p.m <= 8 ? 1 : 2;
+    const int grid = std::max(1, std::min(p.n / (8 * groups), kRowsBlocksPerSm(groups) * sms));
+    // One tile per pass for runs that have no more: the registers of the others would spill (16 x 4096 x 4096 bf16 8.9 against 10.3 us, 1 x 4096 x
+    // 11008 17.0 against 18.1); longer runs share the tokens' loads between tiles (16 x 11008 x 4096: 30.9 us with one, 19.4 with three).
+    const bool one = (p.n + grid - 1) / grid <= kRowsTile;
+    if (groups == 1) return one ? launch_rows_as<KIND, 1, 1, OT>(p, grid, st) : launch_rows_as<KIND, 1, 2, OT>(p, grid, st);
+    return one ? launch_rows_as<KIND, 2, 1, OT>(p, grid, st) : launch_rows_as<KIND, 2, 3, OT>(p, grid, st);
+}
+template <int KIND>
+int launch_rows(const RowsArgs& p, int y_dtype, int sms, cudaStream_t st)
+{
+    if (y_dtype == ASCB200_F16) return launch_rows_of<KIND, __half>(p, sms, st);
+    if (y_dtype == ASCB200_BF16) return launch_rows_of<KIND, __nv_bfloat16>(p, sms, st);
+    return launch_rows_of<KIND, float>(p, sms, st);
 }
 
 bool element_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -177,7 +221,8 @@ bool is_float_type(int dtype) { return dtype == ASCB200_F32 || dtype == ASCB200_
 
 int run_linear(const ascb200_linear_desc* desc, cudaStream_t stream)
 {
-    if (!current_state()) return ASCB200_ENODEV;
+    DeviceState* state = current_state();
+    if (!state) return ASCB200_ENODEV;
     if (!desc) return ASCB200_EINVAL;
     ascb200_linear_desc d = *desc;
     if (d.m < 0 || d.n < 0 || d.k <= 0 || d.reserved != 0 || (d.trans_w != 0 && d.trans_w != 1)) return ASCB200_EINVAL;
@@ -210,9 +255,9 @@ int run_linear(const ascb200_linear_desc* desc, cudaStream_t stream)
         p.bias = d.bias_dev, p.residual = d.residual_dev, p.y = d.y_dev, p.z = d.z_dev;
         p.ldx = d.ldx * esz, p.ldw = d.ldw * esz, p.ld_residual = d.ld_residual, p.ldy = d.ldy, p.ldz = d.ldz;
         p.m = d.m, p.n = d.n, p.k_bytes = d.k * esz, p.bias_f32 = d.bias_dtype == ASCB200_F32, p.act = d.act;
-        if (s8) return launch_rows<ASCB200_KIND_S8>(p, d.y_dtype, stream);
-        if (d.kind == ASCB200_KIND_F16) return launch_rows<ASCB200_KIND_F16>(p, d.y_dtype, stream);
-        return launch_rows<ASCB200_KIND_BF16>(p, d.y_dtype, stream);
+        if (s8) return launch_rows<ASCB200_KIND_S8>(p, d.y_dtype, state->sm_count, stream);
+        if (d.kind == ASCB200_KIND_F16) return launch_rows<ASCB200_KIND_F16>(p, d.y_dtype, state->sm_count, stream);
+        return launch_rows<ASCB200_KIND_BF16>(p, d.y_dtype, state->sm_count, stream);
     }
 
     ascb200_gemm_desc q = {};
@@ -382,6 +427,13 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
     if (!element_aligned(d.dy_dev, 2) || !element_aligned(d.z_dev, 2) || !element_aligned(d.dx_dev, 2)) return ASCB200_EALIGN;
     if ((d.dx_dev && !operand_aligned(d.w_dev, d.ldw, 2)) || (d.dw_dev && !operand_aligned(d.x_dev, d.ldx, 2))) return ASCB200_EALIGN;
 
+    // A product whose rows do not start on 16 bytes is stored by the linear build's output stage, which writes runs of a row through shared
+    // memory (dx and dw of 777 x 1000 x 515 fp16: 39.1 us in all with the plain build's element stores; see the table of figures).
+    const gemm::LinearArgs nothing = {nullptr, 0, ASCB200_ACT_NONE, nullptr, 0};
+    auto product = [&](const ascb200_gemm_desc& q) {
+        const bool aligned = aligned_to(q.c_dev, 16) && (q.ldc * float_bytes(q.c_dtype)) % 16 == 0;
+        return gemm::run_gemm(&q, nullptr, 0, stream, nullptr, aligned ? nullptr : &nothing);
+    };
     const bool products = d.dx_dev || d.dw_dev;
     // dy itself is the operand where there is no activation and it can be one
     const bool make_dz = products && (d.act != ASCB200_ACT_NONE || !operand_aligned(d.dy_dev, d.ld_dy, 2));
@@ -412,7 +464,7 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
         q.kind = d.kind, q.m = d.m, q.n = d.k, q.k = d.n;
         q.a_dev = dz, q.lda = ld_dz, q.b_dev = d.w_dev, q.ldb = d.ldw, q.trans_b = !d.trans_w;
         q.c_dev = d.dx_dev, q.ldc = d.ld_dx, q.c_dtype = own;
-        const int rc = gemm::run_gemm(&q, nullptr, 0, stream);
+        const int rc = product(q);
         if (rc != ASCB200_OK) return rc;
     }
     if (d.dw_dev) {  // [n, k] = dz^T x, or [k, n] = x^T dz
@@ -421,7 +473,7 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
         q.a_dev = d.trans_w ? dz : d.x_dev, q.lda = d.trans_w ? ld_dz : d.ldx;
         q.b_dev = d.trans_w ? d.x_dev : dz, q.ldb = d.trans_w ? d.ldx : ld_dz;
         q.c_dev = d.dw_dev, q.ldc = d.ld_dw, q.c_dtype = d.dw_dtype;
-        const int rc = gemm::run_gemm(&q, nullptr, 0, stream);
+        const int rc = product(q);
         if (rc != ASCB200_OK) return rc;
     }
     return ASCB200_OK;

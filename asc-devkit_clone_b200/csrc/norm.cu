@@ -331,6 +331,12 @@ rms_norm_kernel(const NormArgs p)
             if (r) load_chunk<T, VEC>(r, c, k, rr[i]);
         }
     }
+    constexpr bool EARLY = NCHUNK == 1;  // gamma is requested with the row: where few rows leave latency to count
+    float2 early[4];
+    if constexpr (EARLY) {
+        const int c = first_column<TPR, VEC>(t, 0);
+        if (c < k) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, early);
+    }
     float2 hg[NCHUNK][4], ss2 = both(0.0f);
     float amax = 0.0f;
 #pragma unroll
@@ -346,9 +352,10 @@ rms_norm_kernel(const NormArgs p)
                 for (int j = 0; j < 4; ++j) hg[i][j] = add2(hg[i][j], v[j]);
             }
             if (p.sum) store_chunk<T, VEC>(static_cast<T*>(p.sum) + row * p.ld_sum, c, k, hg[i]);
-            load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
+            if constexpr (!EARLY) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                if constexpr (EARLY) g[j] = early[j];
                 ss2 = fma2(hg[i][j], hg[i][j], ss2);
                 hg[i][j] = mul2(hg[i][j], g[j]);
                 amax = max_abs(amax, hg[i][j]);
@@ -443,7 +450,14 @@ int launch_norm(const NormArgs& p, int sms, cudaStream_t st)
     const int chunks = (p.k + 7) / 8;
 #define ASCB200_NORM_WARP(NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, 32, NC, VEC>, static_cast<unsigned>((p.m + 3ll) / 4), 128, 0, st, p))
 #define ASCB200_NORM_BLOCK(TPR, NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, TPR, NC, VEC>, p.m, TPR, 0, st, p))
-    if (chunks <= 32) ASCB200_NORM_WARP(1);
+    // Up to a row per SM: one chunk per thread, so that a row's loads are all in flight at once (1 x 4096 bf16 in a stream of such calls:
+    // see the table of figures).  More rows: two to four chunks per thread, whose reductions cost less per element.
+    if (chunks > 32 && chunks <= 1024 && p.m <= sms) {
+        if (chunks <= 128) ASCB200_NORM_BLOCK(128, 1);
+        else if (chunks <= 256) ASCB200_NORM_BLOCK(256, 1);
+        else if (chunks <= 512) ASCB200_NORM_BLOCK(512, 1);
+        else ASCB200_NORM_BLOCK(1024, 1);
+    } else if (chunks <= 32) ASCB200_NORM_WARP(1);
     else if (chunks <= 64) ASCB200_NORM_WARP(2);
     else if (chunks <= 128) ASCB200_NORM_WARP(4);
     else if (chunks <= 256) ASCB200_NORM_BLOCK(128, 2);
@@ -453,7 +467,6 @@ int launch_norm(const NormArgs& p, int sms, cudaStream_t st)
     else ASCB200_NORM_BLOCK(1024, 4);
 #undef ASCB200_NORM_WARP
 #undef ASCB200_NORM_BLOCK
-    (void)sms;
     return ASCB200_OK;
 }
 
