@@ -24,7 +24,7 @@ namespace {
 // Two or three blocks per SM, all resident, each with an equal run of weight rows, one to three tiles of 16 in a pass: what is loaded of
 // the tokens serves every tile of the pass.  A block's eight warps take 256-byte pieces of the rows in turn and add their sums in warp
 // order through shared memory at the end of the pass.
-constexpr int kRowsMaxTokens = 16;
+constexpr int kRowsTokens = 16;       // per block
 constexpr int kRowsTile = 16;
 constexpr int kRowsWarps = 8;
 constexpr int kRowsUnroll = 4;        // 64-byte chunks per warp and step
@@ -109,6 +109,8 @@ linear_rows_kernel(const RowsArgs p)
     __shared__ uint32_t part[kRowsWarps][NT * 8][R * kRowsTile + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, q = lane & 3;
+    const int token0 = blockIdx.y * kRowsTokens, tokens = min(kRowsTokens, p.m - token0);
+    const uint8_t* xs = p.x + token0 * p.ldx;
     const int row0 = static_cast<int>(static_cast<long long>(blockIdx.x) * p.n / gridDim.x);
     const int row1 = static_cast<int>((static_cast<long long>(blockIdx.x) + 1) * p.n / gridDim.x);
     // While the kernel before this one drains, ask L2 for the warp's first pieces (hints: nothing is read into the program yet).
@@ -142,7 +144,7 @@ linear_rows_kernel(const RowsArgs p)
 #pragma unroll
                         for (int u = 0; u < kRowsUnroll; ++u) {
                             x[t][u] = make_uint4(0u, 0u, 0u, 0u);
-                            if (t * 8 + g < p.m) x[t][u] = load_piece<false>(p.x + (t * 8 + g) * p.ldx, base + u * 64 + q * 16, p.k_bytes);
+                            if (t * 8 + g < tokens) x[t][u] = load_piece<false>(xs + (t * 8 + g) * p.ldx, base + u * 64 + q * 16, p.k_bytes);
                         }
                 }
 #pragma unroll
@@ -165,19 +167,19 @@ linear_rows_kernel(const RowsArgs p)
         __syncthreads();
         constexpr int cols = R * kRowsTile;
         for (int i = threadIdx.x; i < NT * 8 * cols; i += kRowsWarps * 32) {
-            const int token = i / cols, col = i % cols, n = n0 + col;
-            if (token >= p.m || n >= row1) continue;
+            const int local = i / cols, token = token0 + local, col = i % cols, n = n0 + col;
+            if (local >= tokens || n >= row1) continue;
             float f;
             if constexpr (KIND == ASCB200_KIND_S8) {
                 int s = 0;
 #pragma unroll
-                for (int v = 0; v < kRowsWarps; ++v) s += static_cast<int>(part[v][token][col]);
+                for (int v = 0; v < kRowsWarps; ++v) s += static_cast<int>(part[v][local][col]);
                 f = static_cast<float>(s) * p.ch[n];
                 if (p.tok) f *= p.tok[token];
             } else {
                 f = 0.0f;
 #pragma unroll
-                for (int v = 0; v < kRowsWarps; ++v) f += __uint_as_float(part[v][token][col]);
+                for (int v = 0; v < kRowsWarps; ++v) f += __uint_as_float(part[v][local][col]);
             }
             if (p.bias) f += p.bias_f32 ? static_cast<const float*>(p.bias)[n] : as_f32(static_cast<const OT*>(p.bias)[n]);
             if (p.z) static_cast<OT*>(p.z)[token * p.ldz + n] = rounded<OT>(f);
@@ -189,22 +191,48 @@ linear_rows_kernel(const RowsArgs p)
 }
 
 template <int KIND, int NT, int R, typename OT>
-int launch_rows_as(const RowsArgs& p, unsigned grid, cudaStream_t st)
+int launch_rows_as(const RowsArgs& p, dim3 grid, cudaStream_t st)
 {
     ASCB200_CUDA(launch_pdl(linear_rows_kernel<KIND, NT, R, OT>, grid, kRowsWarps * 32, 0, st, p));
     return ASCB200_OK;
 }
+// How a call is cut for the kernel above: blocks of 16 tokens (grid.y) times runs of weight rows.  A run has at least as many rows as a block
+// has tokens: with fewer, the tokens would be read more often than the weights.
+struct RowsCut {
+    int groups, by_tokens, runs, tiles, steps;  // tiles of 16 rows per run; 2048-byte steps of a block along k
+};
+RowsCut cut_rows(int m, int n, int64_t k_bytes, int sms)
+{
+    RowsCut c;
+    c.groups = m <= 8 ? 1 : 2;
+    c.by_tokens = (m + kRowsTokens - 1) / kRowsTokens;
+    c.runs = std::max(1, std::min(n / (8 * c.groups), kRowsBlocksPerSm(c.groups) * sms / c.by_tokens));
+    c.tiles = ((n + c.runs - 1) / c.runs + kRowsTile - 1) / kRowsTile;
+    c.steps = static_cast<int>((k_bytes + kRowsWarps * kRowsUnroll * 64 - 1) / (kRowsWarps * kRowsUnroll * 64));
+    return c;
+}
+// Up to 16 tokens the kernel above is the faster one at every size measured (us, bf16, m x n x k: 1 x 4096 x 4096 6.8, 16 x 4096 x 4096 8.8 against
+// 12.4 on the GEMM kernels at 17 rows, 16 x 11008 x 4096 20.2 against 21.4, 16 x 512 x 512 2.4 against 5.8).  Up to 256, while every block has one
+// or two tiles and a short k, it still is: 128 x 512 x 512 2.7 against 5.9, 256 x 256 x 4096 8.0 against 10.3, 32 x 4096 x 1024 5.6 against
+// 9.4, 64 x 2048 x 2048 8.1 against 9.0; but 32 x 4096 x 4096 (two tiles, four steps) 13.8 against 12.5, 64 x 4096 x 256 (four tiles) 8.7 against 5.7.
+bool rows_suit(int m, int n, int64_t k_bytes, int sms)
+{
+    if (k_bytes > (1ll << 30)) return false;  // offsets within a row are 32-bit
+    if (m <= kRowsTokens) return true;
+    if (m > 256) return false;
+    const RowsCut c = cut_rows(m, n, k_bytes, sms);
+    return c.tiles <= 2 && c.tiles * c.tiles * c.steps <= 8;
+}
+
 template <int KIND, typename OT>
 int launch_rows_of(const RowsArgs& p, int sms, cudaStream_t st)
 {
-    // a run of at least as many rows as there may be tokens: with fewer, the tokens would be read more often than the weights
-    const int groups = p.m <= 8 ? 1 : 2;
-    const int grid = std::max(1, std::min(p.n / (8 * groups), kRowsBlocksPerSm(groups) * sms));
+    const RowsCut c = cut_rows(p.m, p.n, p.k_bytes, sms);
+    const dim3 grid(c.runs, c.by_tokens);
     // One tile per pass for runs that have no more: the registers of the others would spill (16 x 4096 x 4096 bf16 8.9 against 10.3 us, 1 x 4096 x
-    // 11008 17.0 against 18.1); longer runs share the tokens' loads between tiles (16 x 11008 x 4096: 30.9 us with one, 19.4 with three).
-    const bool one = (p.n + grid - 1) / grid <= kRowsTile;
-    if (groups == 1) return one ? launch_rows_as<KIND, 1, 1, OT>(p, grid, st) : launch_rows_as<KIND, 1, 2, OT>(p, grid, st);
-    return one ? launch_rows_as<KIND, 2, 1, OT>(p, grid, st) : launch_rows_as<KIND, 2, 3, OT>(p, grid, st);
+    // 11008 17.0 against 18.1); longer runs share the tokens' loads between tiles (16 x 11008 x 4096: 30.9 us with one, 20.2 with three).
+    if (c.groups == 1) return c.tiles == 1 ? launch_rows_as<KIND, 1, 1, OT>(p, grid, st) : launch_rows_as<KIND, 1, 2, OT>(p, grid, st);
+    return c.tiles == 1 ? launch_rows_as<KIND, 2, 1, OT>(p, grid, st) : launch_rows_as<KIND, 2, 3, OT>(p, grid, st);
 }
 template <int KIND>
 int launch_rows(const RowsArgs& p, int y_dtype, int sms, cudaStream_t st)
@@ -248,8 +276,7 @@ int run_linear(const ascb200_linear_desc* desc, cudaStream_t stream)
         !element_aligned(d.ch_scale_dev, 4) || (d.bias_dev && !element_aligned(d.bias_dev, float_bytes(d.bias_dtype))))
         return ASCB200_EALIGN;
 
-    // k * esz has to fit the 32-bit offsets within a row
-    if (d.m <= kRowsMaxTokens && d.trans_w && d.k <= (1 << 29)) {
+    if (d.trans_w && rows_suit(d.m, d.n, static_cast<int64_t>(d.k) * esz, state->sm_count)) {
         RowsArgs p = {};
         p.x = static_cast<const uint8_t*>(d.x_dev), p.w = static_cast<const uint8_t*>(d.w_dev), p.tok = d.tok_scale_dev, p.ch = d.ch_scale_dev;
         p.bias = d.bias_dev, p.residual = d.residual_dev, p.y = d.y_dev, p.z = d.z_dev;

@@ -514,8 +514,8 @@ enum { ASCB200_ACT_NONE = 0, ASCB200_ACT_FASTER_GELU = 1, ASCB200_ACT_RELU = 2, 
  * F16 / BF16 operands).  y (and z, residual): the operands' type or F32; F32 / F16 / BF16 for S8.  bias [n]: F32 or y's type.
  * F16 outputs saturate at +-65504.  x and w as for ascb200_gemm: 16-byte aligned, leading dimensions a multiple of 16 bytes (k and n of
  * any size); the other tensors whole elements, fastest with rows on 16 bytes.  k >= 1.  y may be the residual itself (same leading dimension).
- * Up to 16 rows with trans_w = 1 run a kernel that streams the weights once (a token at a time, or a few); the others the GEMM kernels.
- * The order of the fp32 sums depends on which, and within each on the sizes alone. */
+ * Few rows (up to 16, and up to 256 of small layers) with trans_w = 1 run a kernel that streams the weights; the others the GEMM kernels.  The order
+ * of the fp32 sums depends on which, and within each on the sizes and the device alone. */
 typedef struct ascb200_linear_desc {
     int32_t kind;               /* ASCB200_KIND_F16 / BF16 / S8 */
     int32_t m, n, k;

@@ -110,6 +110,13 @@ def test_sizes(m, n, k, dtype):
     forward(m, n, k, dtype, "silu", z=dtype != torch.int8)
 
 
+@pytest.mark.parametrize("m,n,k", [(17, 40, 70), (31, 512, 500), (100, 77, 1030), (128, 1024, 512), (200, 16, 2100), (256, 100, 300), (257, 100, 300)])
+def test_blocks_of_tokens(m, n, k):
+    """Several blocks of tokens over the weights' rows, up to where the GEMM kernels take over."""
+    forward(m, n, k, torch.bfloat16, "gelu_tanh", z=True, bias="out")
+    forward(m, n, k, torch.int8, "silu")
+
+
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.int8])
 @pytest.mark.parametrize("m", [5, 200])
