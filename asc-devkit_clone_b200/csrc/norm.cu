@@ -67,6 +67,19 @@ __device__ __forceinline__ uint4 ld_v4(const void* p)
     return r;
 }
 
+// One element where `inside`, else zero: a predicated load, so that the eight of a chunk go out back to back.
+template <int BYTES>
+__device__ __forceinline__ uint32_t ld_element(const void* p, bool inside)
+{
+    uint32_t r = 0u;
+    if constexpr (BYTES == 4)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}" : "+r"(r) : "l"(p), "r"(static_cast<uint32_t>(inside)));
+    else
+        asm volatile("{\n\t.reg .pred q;\n\t.reg .u16 h;\n\tmov.u16 h, 0;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+                     : "=r"(r) : "l"(p), "r"(static_cast<uint32_t>(inside)));
+    return r;
+}
+
 // A thread's i-th eight columns.  VEC (every row of every tensor starts on 16 bytes and k is a multiple of 8): neighbours, starting at
 // `first_column`.  Else: 32 columns apart, so that a warp's accesses of one element each are contiguous whatever the alignment (gradients of
 // fp32 1000 x 1111: 16 us with neighbouring columns, 10.5 so).  Either way a warp owns 256 contiguous columns.
@@ -89,13 +102,7 @@ __device__ __forceinline__ void load_chunk(const T* row, int c, int k, Raw8<T>& 
     }
     uint32_t u[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        u[j] = 0u;
-        if (c + j * kColumnStep<VEC> < k) {
-            if constexpr (sizeof(T) == 4) u[j] = *reinterpret_cast<const volatile uint32_t*>(row + c + j * kColumnStep<VEC>);
-            else u[j] = *reinterpret_cast<const volatile uint16_t*>(row + c + j * kColumnStep<VEC>);
-        }
-    }
+    for (int j = 0; j < 8; ++j) u[j] = ld_element<sizeof(T)>(row + c + j * kColumnStep<VEC>, c + j * kColumnStep<VEC> < k);
     if constexpr (sizeof(T) == 4) {
         r.v = make_uint4(u[0], u[1], u[2], u[3]);
         r.w = make_uint4(u[4], u[5], u[6], u[7]);
@@ -241,14 +248,16 @@ struct NormArgs {
 // Largest magnitude that a code stands for, in units of the scale.
 constexpr float kTopS8 = 127.0f, kTopE4M3 = 448.0f;
 
-// scale = amax / top and its reciprocal.  A scale under the smallest normal number counts as zero: its reciprocal would not
-// be finite, and codes times scale are then below 2^-117 anyway.  NaN stays NaN.
+// scale = amax / top and its reciprocal, each within a unit in the last place.  A scale under the smallest normal number counts as zero:
+// its reciprocal would not be finite, and codes times scale are then below 2^-117 anyway.  NaN stays NaN.
 __device__ __forceinline__ void scale_of(float amax, bool s8, float& scale, float& inv)
 {
-    const float s = s8 ? __fdiv_rn(amax, kTopS8) : __fdiv_rn(amax, kTopE4M3);
+    const float s = amax * (s8 ? 1.0f / kTopS8 : 1.0f / kTopE4M3);
     const bool none = s < 1.1754943508222875e-38f;
     scale = none ? 0.0f : s;
-    inv = none ? 0.0f : __frcp_rn(s);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    inv = none ? 0.0f : r;
 }
 // MX: the shared exponent floor(log2 amax) - 8 (the exponent of the largest e4m3 power of two), biased by 127; 255 marks a block
 // that holds an infinity or a NaN.
@@ -392,16 +401,17 @@ rms_norm_kernel(const NormArgs p)
         if (t == 0) static_cast<float*>(p.scale)[row] = scale;
     }
     const int lanes = p.group_lanes;
-    const long long groups = (k + lanes * 8 - 1) / (lanes * 8);
+    const int shift = 31 - __clz(lanes * 8);  // columns per group: a power of two
+    const long long group0 = row * ((k + lanes * 8 - 1) >> shift);
     auto scale_group = [&](float g, int column, bool writes) {  // the group's largest magnitude -> its scale, stored, and the reciprocal
         float r;
         if (p.scale_mode == ASCB200_SCALE_MX) {
             const uint32_t byte = mx_scale_byte(g, r);
-            if (writes) static_cast<uint8_t*>(p.scale)[row * groups + column / (lanes * 8)] = static_cast<uint8_t>(byte);
+            if (writes) static_cast<uint8_t*>(p.scale)[group0 + (column >> shift)] = static_cast<uint8_t>(byte);
         } else {
             float scale;
             scale_of(g, s8, scale, r);
-            if (writes) static_cast<float*>(p.scale)[row * groups + column / (lanes * 8)] = scale;
+            if (writes) static_cast<float*>(p.scale)[group0 + (column >> shift)] = scale;
         }
         return r;
     };
@@ -450,9 +460,11 @@ int launch_norm(const NormArgs& p, int sms, cudaStream_t st)
     const int chunks = (p.k + 7) / 8;
 #define ASCB200_NORM_WARP(NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, 32, NC, VEC>, static_cast<unsigned>((p.m + 3ll) / 4), 128, 0, st, p))
 #define ASCB200_NORM_BLOCK(TPR, NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, TPR, NC, VEC>, p.m, TPR, 0, st, p))
-    // Up to a row per SM: one chunk per thread, so that a row's loads are all in flight at once (1 x 4096 bf16 in a stream of such calls:
-    // see the table of figures).  More rows: two to four chunks per thread, whose reductions cost less per element.
-    if (chunks > 32 && chunks <= 1024 && p.m <= sms) {
+    // While all rows fit the machine at once with one chunk per thread: that, so that a row's loads are all in flight (us, bf16 with residual and e4m3
+    // codes, rows x k: 1 x 4096 2.0, 300 x 1024 2.3 against 3.4 with four chunks per lane, 1200 x 1024 3.3 against 4.8, 300 x 4096 3.3
+    // against 4.1).  More rows: two to four chunks per thread, whose reductions cost less per element (600 x 4096 4.3 against 4.8,
+    // 5000 x 4096 24.8 against 30.7, 5000 x 8192 47 against 85).
+    if (chunks > 32 && chunks <= 1024 && static_cast<long long>(p.m) * chunks <= 1536ll * sms) {
         if (chunks <= 128) ASCB200_NORM_BLOCK(128, 1);
         else if (chunks <= 256) ASCB200_NORM_BLOCK(256, 1);
         else if (chunks <= 512) ASCB200_NORM_BLOCK(512, 1);
@@ -547,13 +559,20 @@ struct NormGradArgs {
     const void* gamma;
     const void* dh;
     void* dx;
-    float* partial;  // [blocks][k]
+    float* partial;  // [blocks][k], or nullptr
+    void* dgamma;    // a single block writes it itself
+    int dgamma_dtype;
     long long ld_dy, ldh, ld_dh, ld_dx;
     int m, k;
     int gamma_f32;
 };
 
-constexpr int kMaxGradBlocks = 296;  // rows of the workspace
+
+// Blocks that have to fit an SM: 64 registers per thread with one chunk of a 16-bit row, 128 in warp rows.
+constexpr int grad_blocks_per_sm(int tpr, int nchunk, int bytes)
+{
+    return bytes == 4 ? 1 : tpr == 32 ? 2 : nchunk == 1 ? 1024 / tpr : 1;
+}
 
 template <typename T, int NCHUNK>
 struct GradRow {
@@ -583,12 +602,12 @@ __device__ __forceinline__ void load_grad_row(const NormGradArgs& p, long long r
 // dy * gamma and hat in registers from the reduction to the output, and (16-bit types) request the next row before the current one is
 // worked on; more chunks read gamma and unpack dy and h twice.
 template <typename T, int TPR, int NCHUNK, bool VEC>
-__global__ void __launch_bounds__(TPR > 32 ? TPR : 256, TPR > 32 && NCHUNK == 1 && sizeof(T) == 2 && VEC ? 1024 / TPR : 1)
+__global__ void __launch_bounds__(TPR > 32 ? TPR : 256, grad_blocks_per_sm(TPR, NCHUNK, sizeof(T)))
 rms_norm_grad_kernel(const NormGradArgs p)
 {
     constexpr int ROWS = TPR > 32 ? 1 : 8;
-    constexpr bool AHEAD = NCHUNK * sizeof(T) <= 4;
-    constexpr bool KEEP = NCHUNK <= 2;
+    constexpr bool AHEAD = VEC && NCHUNK * sizeof(T) <= 4;  // (single elements are put together as they come, which waits for them)
+    constexpr bool KEEP = NCHUNK == 1 || (NCHUNK == 2 && TPR > 32);
     constexpr int HELD = KEEP ? NCHUNK : 1;
     __shared__ float2 red[2][32];
     extern __shared__ float warp_acc[];  // warp rows: [8][TPR * NCHUNK * 8]
@@ -671,13 +690,18 @@ rms_norm_grad_kernel(const NormGradArgs p)
     }
     if (!p.partial) return;
     float* out = p.partial + static_cast<size_t>(blockIdx.x) * k;
+    auto put = [&](int col, float v) {
+        if (gridDim.x > 1) out[col] = v;
+        else if (p.dgamma_dtype == ASCB200_F32) static_cast<float*>(p.dgamma)[col] = v;
+        else static_cast<T*>(p.dgamma)[col] = rounded<T>(v);
+    };
     if constexpr (TPR > 32) {
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int col = first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>;
-                if (col < k) out[col] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
+                if (col < k) put(col, j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
             }
     } else {
         constexpr int W = TPR * NCHUNK * 8;
@@ -690,40 +714,48 @@ rms_norm_grad_kernel(const NormGradArgs p)
             float v = 0.0f;
 #pragma unroll
             for (int w = 0; w < ROWS; ++w) v += warp_acc[w * W + col];
-            out[col] = v;
+            put(col, v);
         }
     }
 }
 
-template <typename T, int TPR, int NCHUNK, bool VEC>
-int launch_norm_grad_as(const NormGradArgs& p, int sms, cudaStream_t st, int* blocks)
+// Blocks of the gradient kernel, at most: rows of the workspace.  By k alone: as many as fill the machine at 64 registers per thread (16-bit rows of up
+// to 4096), which more than pays for the longer second sum (16384 x 2048 bf16: 80 us with 296 blocks, 56 with 592).
+int grad_blocks(int m, int k)
 {
-    constexpr int rows = TPR > 32 ? 1 : 8;
+    const int chunks = (k + 7) / 8;
+    const long long most = chunks <= 64 ? 592 : chunks <= 128 ? 888 : chunks <= 256 ? 592 : 296;
+    const long long rows = chunks <= 64 ? (m + 7ll) / 8 : m;
+    return static_cast<int>(std::min(most, std::min(rows, std::max(148ll, rows / 4))));  // four rows at a time before a second block per SM
+}
+
+template <typename T, int TPR, int NCHUNK, bool VEC>
+int launch_norm_grad_as(const NormGradArgs& p, cudaStream_t st, int* blocks)
+{
     constexpr size_t smem = TPR > 32 ? 0 : 8 * TPR * NCHUNK * 8 * sizeof(float);
-    *blocks = static_cast<int>(std::min<long long>((p.m + rows - 1ll) / rows, std::min(2 * sms, kMaxGradBlocks)));
+    *blocks = grad_blocks(p.m, p.k);
     ASCB200_CUDA(launch_pdl(rms_norm_grad_kernel<T, TPR, NCHUNK, VEC>, *blocks, TPR > 32 ? TPR : 256, smem, st, p));
     return ASCB200_OK;
 }
 template <typename T, bool VEC>
-int launch_norm_grad(const NormGradArgs& p, int sms, cudaStream_t st, int* blocks)
+int launch_norm_grad(const NormGradArgs& p, cudaStream_t st, int* blocks)
 {
     const int chunks = (p.k + 7) / 8;
-    if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, VEC>(p, sms, st, blocks);
-    if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, VEC>(p, sms, st, blocks);
-    if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, VEC>(p, sms, st, blocks);
-    if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, VEC>(p, sms, st, blocks);
-    if (chunks <= 512) return launch_norm_grad_as<T, 512, 1, VEC>(p, sms, st, blocks);
-    if (chunks <= 1024) return launch_norm_grad_as<T, 512, 2, VEC>(p, sms, st, blocks);
-    if (chunks <= 2048) return launch_norm_grad_as<T, 512, 4, VEC>(p, sms, st, blocks);
-    return launch_norm_grad_as<T, 1024, 4, VEC>(p, sms, st, blocks);
+    if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, VEC>(p, st, blocks);
+    if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, VEC>(p, st, blocks);
+    if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, VEC>(p, st, blocks);
+    if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, VEC>(p, st, blocks);
+    if (chunks <= 512) return launch_norm_grad_as<T, 512, 1, VEC>(p, st, blocks);
+    if (chunks <= 1024) return launch_norm_grad_as<T, 512, 2, VEC>(p, st, blocks);
+    if (chunks <= 2048) return launch_norm_grad_as<T, 512, 4, VEC>(p, st, blocks);
+    return launch_norm_grad_as<T, 1024, 4, VEC>(p, st, blocks);
 }
 
-size_t grad_workspace(int m, int k) { return m <= 0 || k <= 0 ? 0 : static_cast<size_t>(std::min(m, kMaxGradBlocks)) * k * sizeof(float); }
+size_t grad_workspace(int m, int k) { return m <= 0 || k <= 0 ? 0 : static_cast<size_t>(grad_blocks(m, k)) * k * sizeof(float); }
 
 int run_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, cudaStream_t stream)
 {
-    DeviceState* st = current_state();
-    if (!st) return ASCB200_ENODEV;
+    if (!current_state()) return ASCB200_ENODEV;
     if (!desc) return ASCB200_EINVAL;
     ascb200_rms_norm_grad_desc d = *desc;
     if (d.m < 0 || d.k <= 0 || d.reserved != 0) return ASCB200_EINVAL;
@@ -752,16 +784,16 @@ int run_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, cudaStream_t strea
     p.ld_dy = d.ld_dy, p.ldh = d.ldh, p.ld_dh = d.ld_dh, p.ld_dx = d.ld_dx, p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32;
     const bool vec = d.k % 8 == 0 && rows_aligned(d.dy_dev, d.ld_dy, esz, 16) && rows_aligned(d.h_dev, d.ldh, esz, 16) && rows_aligned(d.dh_dev, d.ld_dh, esz, 16) &&
                      rows_aligned(d.dx_dev, d.ld_dx, esz, 16) && (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
+    p.dgamma = d.dgamma_dev, p.dgamma_dtype = d.dgamma_dtype;
     int blocks = 0, rc;
-    const int sms = st->sm_count;
     switch (d.dtype) {
-        case ASCB200_F16: rc = vec ? launch_norm_grad<__half, true>(p, sms, stream, &blocks) : launch_norm_grad<__half, false>(p, sms, stream, &blocks); break;
+        case ASCB200_F16: rc = vec ? launch_norm_grad<__half, true>(p, stream, &blocks) : launch_norm_grad<__half, false>(p, stream, &blocks); break;
         case ASCB200_BF16:
-            rc = vec ? launch_norm_grad<__nv_bfloat16, true>(p, sms, stream, &blocks) : launch_norm_grad<__nv_bfloat16, false>(p, sms, stream, &blocks);
+            rc = vec ? launch_norm_grad<__nv_bfloat16, true>(p, stream, &blocks) : launch_norm_grad<__nv_bfloat16, false>(p, stream, &blocks);
             break;
-        default: rc = vec ? launch_norm_grad<float, true>(p, sms, stream, &blocks) : launch_norm_grad<float, false>(p, sms, stream, &blocks);
+        default: rc = vec ? launch_norm_grad<float, true>(p, stream, &blocks) : launch_norm_grad<float, false>(p, stream, &blocks);
     }
-    if (rc != ASCB200_OK || !d.dgamma_dev) return rc;
+    if (rc != ASCB200_OK || !d.dgamma_dev || blocks == 1) return rc;
     return sum_partials(p.partial, d.dgamma_dev, d.dgamma_dtype, blocks, d.k, stream);
 }
 
