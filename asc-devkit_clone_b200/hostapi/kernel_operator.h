@@ -268,3 +268,4 @@ inline uint8_t* GetSysWorkSpacePtr()
 }
 
 #include "adv_api_ops.h"
+#include "feed_forward_ops.h"
