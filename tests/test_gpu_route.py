@@ -83,6 +83,7 @@ def check(x, out, valid, top_k, renorm):
 
 @pytest.mark.parametrize("renorm", [0, 1])
 @pytest.mark.parametrize("t,e,k,dtype", [(1, 1, 1, "f32"), (1, 8, 2, "bf16"), (16, 60, 4, "f32"), (17, 64, 6, "f16"), (3, 33, 32, "f32"), (300, 128, 8, "bf16"), (65, 257, 8, "f32"),
+                                         (129, 5, 3, "f32"), (256, 1024, 4, "f16"), (257, 20, 2, "bf16"),
                                          (40, 512, 3, "f16"), (33, 1000, 8, "f32"), (20, 1024, 32, "bf16"), (5000, 16, 2, "f32")])
 def test_sizes(t, e, k, dtype, renorm):
     g = gen(t + e)
@@ -251,13 +252,13 @@ def test_optional_outputs():
 
 def test_refusals():
     dev()
-    x = torch.zeros(100, 8, device="cuda")
-    idx, w, c = torch.zeros(100, 2, device="cuda", dtype=torch.int32), torch.zeros(100, 2, device="cuda"), torch.zeros(8, device="cuda", dtype=torch.int64)
-    room = torch.zeros(ab.route_workspace_bytes(100, 8), device="cuda", dtype=torch.uint8)
+    x = torch.zeros(300, 8, device="cuda")
+    idx, w, c = torch.zeros(300, 2, device="cuda", dtype=torch.int32), torch.zeros(300, 2, device="cuda"), torch.zeros(8, device="cuda", dtype=torch.int64)
+    room = torch.zeros(ab.route_workspace_bytes(300, 8), device="cuda", dtype=torch.uint8)
     assert room.numel() > 0 and ab.route_workspace_bytes(16, 8) == 0 and ab.route_workspace_bytes(0, 8) == 0 and ab.route_workspace_bytes(-1, 8) == 0
 
     def rc(**kw):
-        f = dict(tokens=100, experts=8, top_k=2, logits_dev=ptr(x), idx_dev=ptr(idx), weights_dev=ptr(w), counts_dev=ptr(c), workspace_dev=ptr(room), workspace_bytes=room.numel())
+        f = dict(tokens=300, experts=8, top_k=2, logits_dev=ptr(x), idx_dev=ptr(idx), weights_dev=ptr(w), counts_dev=ptr(c), workspace_dev=ptr(room), workspace_bytes=room.numel())
         return ab.route(ab.RouteDesc(**(f | kw)), stream())
 
     assert rc() == 0
@@ -271,7 +272,7 @@ def test_refusals():
     n, l = torch.ones(1, device="cuda", dtype=torch.int64), torch.zeros(1, device="cuda")
 
     def grad(**kw):
-        f = dict(tokens=100, experts=8, top_k=2, logits_dev=ptr(x), idx_dev=ptr(idx), counts_dev=ptr(c), num_tokens_dev=ptr(n), dloss_dev=ptr(l), dlogits_dev=ptr(x))
+        f = dict(tokens=300, experts=8, top_k=2, logits_dev=ptr(x), idx_dev=ptr(idx), counts_dev=ptr(c), num_tokens_dev=ptr(n), dloss_dev=ptr(l), dlogits_dev=ptr(x))
         return ab.route_grad(ab.RouteGradDesc(**(f | kw)), stream())
 
     assert grad() == 0
