@@ -270,6 +270,7 @@ int run_linear(const ascb200_linear_desc* desc, cudaStream_t stream)
     if (d.ldx < d.k || d.ldw < (d.trans_w ? d.k : d.n) || d.ld_residual < d.n || d.ldy < d.n || d.ldz < d.n) return ASCB200_EINVAL;
     if (d.m == 0 || d.n == 0) return ASCB200_OK;
     if (!d.x_dev || !d.w_dev || !d.y_dev || (s8 && !d.ch_scale_dev) || d.y_dev == d.z_dev) return ASCB200_EINVAL;
+    if (d.residual_dev && ((d.y_dev == d.residual_dev && d.ldy != d.ld_residual) || d.z_dev == d.residual_dev)) return ASCB200_EINVAL;
     const int esz = s8 ? 1 : 2, osz = float_bytes(d.y_dtype);
     if (!operand_aligned(d.x_dev, d.ldx, esz) || !operand_aligned(d.w_dev, d.ldw, esz)) return ASCB200_EALIGN;
     if (!element_aligned(d.y_dev, osz) || !element_aligned(d.z_dev, osz) || !element_aligned(d.residual_dev, osz) || !element_aligned(d.tok_scale_dev, 4) ||
@@ -455,7 +456,7 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
     if ((d.dx_dev && !operand_aligned(d.w_dev, d.ldw, 2)) || (d.dw_dev && !operand_aligned(d.x_dev, d.ldx, 2))) return ASCB200_EALIGN;
 
     // A product whose rows do not start on 16 bytes is stored by the linear build's output stage, which writes runs of a row through shared
-    // memory (dx and dw of 777 x 1000 x 515 fp16: 39.1 us in all with the plain build's element stores; see the table of figures).
+    // memory (gradients of 777 x 1000 x 515 fp16: 39.1 us in all with the plain build's element stores, 21.7 so).
     const gemm::LinearArgs nothing = {nullptr, 0, ASCB200_ACT_NONE, nullptr, 0};
     auto product = [&](const ascb200_gemm_desc& q) {
         const bool aligned = aligned_to(q.c_dev, 16) && (q.ldc * float_bytes(q.c_dtype)) % 16 == 0;
@@ -468,7 +469,7 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
     int64_t ld_dz = d.ld_dy;
     if (make_dz || d.dbias_dev) {
         if (!d.workspace_dev || d.workspace_bytes < linear_grad_workspace(d.m, d.n)) return ASCB200_EINVAL;
-        if (!aligned_to(d.workspace_dev, 256)) return ASCB200_EALIGN;
+        if (!aligned_to(d.workspace_dev, 16)) return ASCB200_EALIGN;
         ActGradArgs p = {};
         p.dy = d.dy_dev, p.z = d.z_dev, p.ld_dy = d.ld_dy, p.ldz = d.ldz, p.m = d.m, p.n = d.n;
         if (make_dz) {

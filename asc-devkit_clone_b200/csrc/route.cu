@@ -659,7 +659,7 @@ int run_route_grad(const ascb200_route_grad_desc* desc, cudaStream_t stream)
     if (d.ld_dlogits == 0) d.ld_dlogits = d.experts;
     if (d.ld_dlogits < d.experts || d.reserved != 0) return ASCB200_EINVAL;
     if (d.tokens == 0) return ASCB200_OK;
-    if (!d.logits_dev || !d.idx_dev || !d.dlogits_dev) return ASCB200_EINVAL;
+    if (!d.logits_dev || !d.idx_dev || !d.dlogits_dev || (d.dlogits_dev == d.logits_dev && d.ld_dlogits != d.ld_logits)) return ASCB200_EINVAL;
     if (d.dloss_dev && (!d.counts_dev || !d.num_tokens_dev)) return ASCB200_EINVAL;
     const int esz = d.dtype == ASCB200_F32 ? 4 : 2;
     if (!element_aligned(d.logits_dev, esz) || !element_aligned(d.dlogits_dev, esz) || !element_aligned(d.idx_dev, 4) || !element_aligned(d.counts_dev, 8) ||

@@ -447,7 +447,7 @@ enum { ASCB200_SCALE_PER_TOKEN = 0, ASCB200_SCALE_PER_GROUP = 1, ASCB200_SCALE_M
  *   MX: e = floor(log2(max|y|)) - 8 over 32 columns, scale byte = e + 127 (at least 0), q = e4m3(y / 2^e) saturating.
  * With S8 and PER_TOKEN, q and scale are a_dev and tok_scale_dev of an A8W8 ascb200_gemm / ascb200_linear; with MX, a_dev and
  * scale_a_dev of KIND_MXFP8_E4M3 (k a multiple of 64 there).
- * All-zero rows and groups (and those whose scale would be under 2^-126) get scale 0 and codes 0.  A NaN or an infinity in a row
+ * All-zero rows and groups (and those whose scale would be under 2^-126) get scale 0 and codes 0 (with eps > 0; eps = 0 makes them NaN).  A NaN or an infinity in a row
  * makes its rstd, y and scales NaN (0 where only finite values meet an infinity's rstd of 0; MX scale byte 255); int8 codes are 0 there.
  * F16 outputs saturate at +-65504.  Squares are summed in fp32: rows of |h| above 1e18 overflow.
  * dtype (x, residual, sum, y): F32 / F16 / BF16; gamma: the same or F32, NULL for ones.  k up to 32768; any alignment of whole
@@ -544,7 +544,7 @@ ASCB200_API int ascb200_linear(const ascb200_linear_desc* desc, void* stream);
  *   dz = dy * act'(z);  dbias = sum over rows of dz;  dx = dz w;  dw = dz^T x ([n, k], or [k, n] with trans_w = 0).
  * z as the forward call wrote it in the operands' type (not read for ACT_NONE).  dz is rounded to the operands' type for the two products, dbias
  * is summed in fp32 from the values before.  dx, dw and dbias may each be NULL (not wanted); dw and dbias: the operands' type or F32.
- * The workspace (256-byte aligned) holds dz and the partial sums of dbias; without activation and dbias it is not needed when dy is
+ * The workspace holds dz and the partial sums of dbias; without activation and dbias it is not needed when dy is
  * aligned like x.  m = 0 gives dw = 0 and dbias = 0. */
 typedef struct ascb200_linear_grad_desc {
     int32_t kind;

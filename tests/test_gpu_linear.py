@@ -153,6 +153,43 @@ def test_split_k(m, n, k):
     forward(m, n, k, torch.int8, "silu")
 
 
+@pytest.mark.parametrize("m,n,k", [(40, 1100, 4100), (64, 2100, 2100), (65, 1101, 4100), (130, 3001, 1000), (200, 4096, 264), (300, 515, 1000), (1025, 65, 300)])
+def test_gemm_kernels(m, n, k):
+    """Sizes that the GEMM kernels take: tiles of 64 rows and less, ragged ones, odd widths through the staging buffer, every output type."""
+    for dtype in (torch.bfloat16, torch.float16):
+        forward(m, n, k, dtype, "gelu", z=True, bias="out")
+        forward(m, n, k, dtype, "silu", z=True, out=torch.float32, y_pad=3, offset=1)
+        forward(m, n, k, dtype, "relu", residual=True, z=True, y_pad=-n % 8 + 8, offset=8, pad=1)
+        forward(m, n, k, dtype, "none", in_place=True, trans_w=0)
+    for out in (torch.bfloat16, torch.float32):
+        forward(m, n, k, torch.int8, "gelu_tanh", out=out, pad=1, tok=out == torch.float32)
+        forward(m, n, k, torch.int8, "faster_gelu", out=out, residual=False, bias=None, y_pad=5)
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 512, 16384), (300, 256, 4096), (20, 300, 20000), (60, 128, 18000)])
+def test_gemm_kernels_split_k(m, n, k):
+    forward(m, n, k, torch.bfloat16, "gelu", z=True)
+    forward(m, n + 1, k, torch.float16, "silu", z=True, out=torch.float32)
+    forward(m, n, k, torch.int8, "silu")
+
+
+def test_unaligned_residual_beside_aligned_output():
+    """y's rows on 16 bytes, the residual's not, and the other way round."""
+    dev()
+    m, n, k = 300, 515, 1000
+    x, w, xs, ws = operands(m, n, k, torch.bfloat16, 1, 0)
+    r = torch.randn(m, n, generator=gen(21)).bfloat16()
+    want = (x.cuda().double() @ w.cuda().double().t()) + r.cuda().double()
+    tol = (k / 16 + 32) * 2 * F * (x.cuda().double().abs() @ w.cuda().double().abs().t()) + (2.0**-8 + 4 * F) * want.abs() + TINY[torch.bfloat16]
+    for y_pad, r_pad in ((5, 0), (0, 5), (5, 13)):
+        y, rs = Out(m, n, torch.bfloat16, y_pad), rows_in(r, torch.bfloat16, r_pad)
+        ab.check(ab.linear(ab.LinearDesc(kind=ab.KIND_BF16, m=m, n=n, k=k, x_dev=ptr(xs), ldx=xs.stride(0), w_dev=ptr(ws), ldw=ws.stride(0), trans_w=1, residual_dev=ptr(rs), ld_residual=n + r_pad,
+                                         y_dev=y.ptr(), ldy=y.ld, y_dtype=ab.BF16), stream()))
+        torch.cuda.synchronize()
+        y.check()
+        near(y.t, want, tol, "y")
+
+
 @pytest.mark.parametrize("width", [64, 112, 160, 256])
 def test_pair_tiles(width, monkeypatch):
     monkeypatch.setenv("ASCB200_PAIR_N", str(width))
@@ -310,7 +347,7 @@ def test_refusals():
 
     assert rc() == 0
     for bad in (dict(m=-1), dict(n=-1), dict(k=0), dict(x_dev=None), dict(w_dev=None), dict(y_dev=None), dict(ldx=56), dict(ldw=56), dict(ldy=63), dict(ldz=63), dict(ld_residual=63), dict(act=6),
-                dict(act=-1), dict(trans_w=2), dict(reserved=1), dict(tok_scale_dev=ptr(s)), dict(z_dev=ptr(y)), dict(kind=ab.KIND_S8, y_dtype=ab.BF16)):
+                dict(act=-1), dict(trans_w=2), dict(reserved=1), dict(tok_scale_dev=ptr(s)), dict(z_dev=ptr(y)), dict(residual_dev=ptr(y), ld_residual=72), dict(residual_dev=ptr(f), z_dev=ptr(f)), dict(kind=ab.KIND_S8, y_dtype=ab.BF16)):
         assert rc(**bad) == ab.EINVAL, bad
     for bad in (dict(kind=ab.KIND_MXFP4), dict(kind=9), dict(y_dtype=ab.BF16), dict(y_dtype=ab.S8), dict(bias_dev=ptr(s), bias_dtype=ab.BF16),
                 dict(kind=ab.KIND_S8, y_dtype=ab.BF16, ch_scale_dev=ptr(s), z_dev=ptr(f))):
@@ -332,7 +369,7 @@ def test_refusals():
         assert grad(**bad) == ab.EINVAL, bad
     for bad in (dict(kind=ab.KIND_S8), dict(dw_dtype=ab.BF16), dict(dbias_dev=ptr(s), dbias_dtype=ab.BF16)):
         assert grad(**bad) == ab.EUNSUPPORTED, bad
-    for bad in (dict(x_dev=ptr(x) + 2), dict(w_dev=ptr(w) + 8), dict(workspace_dev=ptr(room) + 16), dict(dy_dev=ptr(y) + 1), dict(dbias_dev=ptr(s) + 1)):
+    for bad in (dict(x_dev=ptr(x) + 2), dict(w_dev=ptr(w) + 8), dict(workspace_dev=ptr(room) + 8), dict(dy_dev=ptr(y) + 1), dict(dbias_dev=ptr(s) + 1)):
         assert grad(**bad) == ab.EALIGN, bad
     assert ab.linear_grad_workspace_bytes(0, 4) == 0 and ab.linear_grad_workspace_bytes(-1, 4) == 0
     assert ab.lib().ascb200_linear_grad(None, None) == ab.EINVAL

@@ -287,6 +287,7 @@ def test_refusals():
 
     assert rc() == 0
     assert rc(m=-1) == ab.EINVAL and rc(k=0) == ab.EINVAL and rc(x_dev=None) == ab.EINVAL and rc(y_dev=None) == ab.EINVAL and rc(ldx=63) == ab.EINVAL
+    assert rc(ldy=72) == ab.EINVAL and rc(residual_dev=ptr(x), sum_dev=ptr(x), y_dev=ptr(q), ld_sum=72) == ab.EINVAL
     assert rc(eps=-1.0) == ab.EINVAL and rc(eps=float("nan")) == ab.EINVAL and rc(reserved=1) == ab.EINVAL and rc(sum_dev=ptr(x)) == ab.EINVAL
     assert rc(dtype=ab.S8) == ab.EUNSUPPORTED and rc(gamma_dev=ptr(x), gamma_dtype=ab.F16) == ab.EUNSUPPORTED
     assert rc(k=32769, ldx=0) == ab.ETOOBIG and rc(x_dev=ptr(x) + 1) == ab.EALIGN and rc(rstd_dev=ptr(s) + 2) == ab.EALIGN
@@ -309,7 +310,7 @@ def test_refusals():
     assert grad() == 0
     for name in ("dy_dev", "h_dev", "rstd_dev", "dx_dev", "workspace_dev"):
         assert grad(**{name: None}) == ab.EINVAL
-    assert grad(workspace_bytes=room.numel() - 1) == ab.EINVAL and grad(workspace_dev=ptr(room) + 4) == ab.EALIGN and grad(ld_dx=63) == ab.EINVAL
+    assert grad(ld_dx=72) == ab.EINVAL and grad(workspace_bytes=room.numel() - 1) == ab.EINVAL and grad(workspace_dev=ptr(room) + 4) == ab.EALIGN and grad(ld_dx=63) == ab.EINVAL
     assert grad(k=40000) == ab.ETOOBIG and grad(dgamma_dtype=ab.F16) == ab.EUNSUPPORTED and grad(reserved=1) == ab.EINVAL and grad(dtype=ab.S32) == ab.EUNSUPPORTED
     assert ab.lib().ascb200_rms_norm_grad(None, None) == ab.EINVAL
     torch.cuda.synchronize()

@@ -276,7 +276,7 @@ def test_refusals():
         return ab.route_grad(ab.RouteGradDesc(**(f | kw)), stream())
 
     assert grad() == 0
-    for bad in (dict(logits_dev=None), dict(idx_dev=None), dict(dlogits_dev=None), dict(counts_dev=None), dict(num_tokens_dev=None), dict(ld_dlogits=7), dict(reserved=1),
+    for bad in (dict(logits_dev=None), dict(idx_dev=None), dict(dlogits_dev=None), dict(counts_dev=None), dict(num_tokens_dev=None), dict(ld_dlogits=7), dict(ld_dlogits=16), dict(reserved=1),
                 dict(top_k=9), dict(renorm=-1)):
         assert grad(**bad) == ab.EINVAL, bad
     assert grad(dtype=ab.S32) == ab.EUNSUPPORTED and grad(dloss_dev=ptr(l) + 1) == ab.EALIGN
