@@ -80,34 +80,90 @@ __device__ __forceinline__ uint32_t ld_element(const void* p, bool inside)
     return r;
 }
 
-// A thread's i-th eight columns.  VEC (every row of every tensor starts on 16 bytes and k is a multiple of 8): neighbours, starting at
-// `first_column`.  Else: 32 columns apart, so that a warp's accesses of one element each are contiguous whatever the alignment (gradients of
-// fp32 1000 x 1111: 16 us with neighbouring columns, 10.5 so).  Either way a warp owns 256 contiguous columns.
-template <bool VEC>
-constexpr int kColumnStep = VEC ? 1 : 32;
-template <int TPR, bool VEC>
-__device__ __forceinline__ int first_column(int t, int i)
+// How a thread's i-th eight columns lie; a warp owns 256 neighbouring columns in either case.
+//   kVec       neighbours, one 16-byte access: every row of every tensor starts on 16 bytes and k is a multiple of 8;
+//   kPairs     16-bit rows else, where all tensors' rows have the same parity: pairs, 64 columns apart, that start on 4 bytes (in a row that does
+//              not, the pairs begin one column to the left: the first pair then has only its second column);
+//   kElements  single elements, 32 columns apart, so that a warp's accesses are contiguous whatever the alignment.
+// (us, bf16 with residual and int8 codes, 65536 x 511: neighbouring columns one by one 174, kElements 71, kPairs 57, and the aligned 65536 x 512
+// 38; gradients of 8192 x 4095 / 4096: kElements 117, kPairs 69, kVec 54.)
+enum Mode : int { kElements = 0, kVec = 1, kPairs = 2 };
+// `shift`: kPairs, 1 where the row's pairs begin to the left of its first column.  The column may then be -1.
+template <int TPR, int MODE>
+__device__ __forceinline__ int first_column(int t, int i, int shift)
 {
-    return VEC ? (t + i * TPR) * 8 : (i * TPR + (t & ~31)) * 8 + (t & 31);
+    if constexpr (MODE == kVec) return (t + i * TPR) * 8;
+    else if constexpr (MODE == kPairs) return (i * TPR + (t & ~31)) * 8 + 2 * (t & 31) - shift;
+    else return (i * TPR + (t & ~31)) * 8 + (t & 31);
+}
+template <int MODE>
+__device__ __forceinline__ int column(int c, int j)  // the j-th of the eight that start at c
+{
+    return MODE == kVec ? c + j : MODE == kPairs ? c + 64 * (j >> 1) + (j & 1) : c + 32 * j;
+}
+__device__ __forceinline__ bool in_row(int col, int k) { return static_cast<unsigned>(col) < static_cast<unsigned>(k); }
+template <int MODE>
+__device__ __forceinline__ int row_shift(const void* row) { return MODE == kPairs ? static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1 : 0; }
+// kPairs: whether all of the warp's pairs are whole; the same for its lanes.
+__device__ __forceinline__ bool whole_pairs(int c, int k)
+{
+    const int warp_first = c - 2 * (threadIdx.x & 31);
+    return warp_first >= 0 && warp_first + 256 <= k;
 }
 
-// The eight elements at column c < k; elements past the row's end read as zero and are not touched.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_chunk(const T* row, int c, int k, Raw8<T>& r)
+// kPairs: which pairs of a row (by their first column) are read as a whole.  The pair that begins at -1 holds the element before the row, the one
+// that begins at k - 1 the element behind it: these belong to the neighbouring rows, or to what lies between rows, and are thrown
+// away, except before the first row and behind the last, where they would not belong to the tensor.
+struct PairRange {
+    int first, last;
+};
+template <int MODE>
+__device__ __forceinline__ PairRange pair_range(long long row, int m, int k)
 {
-    if constexpr (VEC) {
+    if constexpr (MODE != kPairs) return {0, 0};
+    return {row == 0 ? 0 : -1, row == m - 1 ? k - 2 : k - 1};
+}
+
+// The eight elements at column c < k; elements outside the row are not touched and read as zero (kPairs: see finish_chunk).
+template <typename T, int MODE>
+__device__ __forceinline__ void load_chunk(const T* row, int c, int k, const PairRange& range, Raw8<T>& r)
+{
+    if constexpr (MODE == kVec) {
         r.v = ld_v4(row + c);
         if constexpr (sizeof(T) == 4) r.w = ld_v4(row + c + 4);
-        return;
-    }
-    uint32_t u[8];
+    } else if constexpr (MODE == kPairs) {
+        uint32_t u[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = ld_element<sizeof(T)>(row + c + j * kColumnStep<VEC>, c + j * kColumnStep<VEC> < k);
-    if constexpr (sizeof(T) == 4) {
+        for (int j = 0; j < 4; ++j) u[j] = ld_element<4>(row + c + 64 * j, static_cast<unsigned>(c + 64 * j - range.first) <= static_cast<unsigned>(range.last - range.first) && range.last >= range.first);
         r.v = make_uint4(u[0], u[1], u[2], u[3]);
-        r.w = make_uint4(u[4], u[5], u[6], u[7]);
     } else {
-        r.v = make_uint4(u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16));
+        uint32_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = ld_element<sizeof(T)>(row + column<MODE>(c, j), in_row(column<MODE>(c, j), k));
+        if constexpr (sizeof(T) == 4) {
+            r.v = make_uint4(u[0], u[1], u[2], u[3]);
+            r.w = make_uint4(u[4], u[5], u[6], u[7]);
+        } else {
+            r.v = make_uint4(u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16));
+        }
+    }
+}
+// Before the first use of a loaded chunk.  kPairs, where the warp has a pair that the row only half owns: takes the other half out, and fetches the
+// element of a pair that was not read.  (Here and not at the load, which would then be waited for.)
+template <typename T, int MODE>
+__device__ __forceinline__ void finish_chunk(const T* row, int c, int k, const PairRange& range, Raw8<T>& r)
+{
+    if constexpr (MODE == kPairs) {
+        if (whole_pairs(c, k)) return;
+        uint32_t u[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int col = c + 64 * j;
+            if (col == -1) u[j] = range.first == 0 ? (k > 0 ? static_cast<uint32_t>(e[0]) << 16 : 0u) : u[j] & 0xFFFF0000u;
+            if (col == k - 1 && col >= 0) u[j] = range.last < col ? static_cast<uint32_t>(e[col]) : u[j] & 0xFFFFu;
+        }
+        r.v = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
 __device__ __forceinline__ void unpack8(const Raw8<float>& r, float2 (&f)[4])
@@ -139,53 +195,66 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16)
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __device__ __forceinline__ void store_chunk(T* row, int c, int k, const float2 (&f)[4])
 {
     if constexpr (sizeof(T) == 4) {
-        if constexpr (VEC) {
+        if constexpr (MODE == kVec) {
             *reinterpret_cast<float4*>(row + c) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
             *reinterpret_cast<float4*>(row + c + 4) = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + j * kColumnStep<VEC> < k) row[c + j * kColumnStep<VEC>] = j & 1 ? f[j / 2].y : f[j / 2].x;
+                if (in_row(column<MODE>(c, j), k)) row[column<MODE>(c, j)] = j & 1 ? f[j / 2].y : f[j / 2].x;
         }
     } else {
         const uint4 v = make_uint4(pack2(f[0].x, f[0].y, T()), pack2(f[1].x, f[1].y, T()), pack2(f[2].x, f[2].y, T()), pack2(f[3].x, f[3].y, T()));
-        if constexpr (VEC) {
+        if constexpr (MODE == kVec) {
             *reinterpret_cast<uint4*>(row + c) = v;
         } else {
             const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            if constexpr (MODE == kPairs) {
+                if (whole_pairs(c, k)) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(row + c + 64 * j) = u[j];
+                    return;
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + j * kColumnStep<VEC> < k) reinterpret_cast<uint16_t*>(row)[c + j * kColumnStep<VEC>] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+                if (in_row(column<MODE>(c, j), k)) reinterpret_cast<uint16_t*>(row)[column<MODE>(c, j)] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
         }
     }
 }
 // gamma: NULL (ones), fp32, or the rows' type.
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __device__ __forceinline__ void load_gamma(const void* __restrict__ gamma, int gamma_f32, int c, int k, float2 (&g)[4])
 {
     if (!gamma) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) g[j] = both(1.0f);
     } else if (sizeof(T) == 4 || gamma_f32) {
-        const float* src = static_cast<const float*>(gamma) + c;
-        if constexpr (VEC) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(src)), b = __ldg(reinterpret_cast<const float4*>(src) + 1);
+        const float* src = static_cast<const float*>(gamma);
+        if constexpr (MODE == kVec) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(src + c)), b = __ldg(reinterpret_cast<const float4*>(src + c) + 1);
             g[0] = make_float2(a.x, a.y), g[1] = make_float2(a.z, a.w), g[2] = make_float2(b.x, b.y), g[3] = make_float2(b.z, b.w);
         } else {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c + j * kColumnStep<VEC> < k ? __ldg(src + j * kColumnStep<VEC>) : 0.0f;
+            for (int j = 0; j < 8; ++j) v[j] = in_row(column<MODE>(c, j), k) ? __ldg(src + column<MODE>(c, j)) : 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) g[j] = make_float2(v[2 * j], v[2 * j + 1]);
         }
     } else {
         Raw8<T> r;
-        if constexpr (VEC) r.v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(gamma) + c));
-        else load_chunk<T, VEC>(static_cast<const T*>(gamma), c, k, r);
+        if constexpr (MODE == kVec) r.v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(gamma) + c));
+        else {
+            const uint16_t* src = static_cast<const uint16_t*>(gamma);  // (its pairs need not lie like the rows')
+            uint32_t u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = in_row(column<MODE>(c, j), k) ? __ldg(src + column<MODE>(c, j)) : 0u;
+            r.v = make_uint4(u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16));
+        }
         unpack8(r, g);
     }
 }
@@ -288,7 +357,7 @@ __device__ __forceinline__ uint32_t pack_bytes(float2 a, float2 b)
 // Eight codes of y * mul (mul: the reciprocals of the scales).  int8: |y * mul| is at most 127 and a bit, so adding 1.5 * 2^23 in the
 // same instruction rounds it once, to the nearest even integer, which is then the sum's low byte in two's complement; values whose
 // scale is NaN give 0.
-template <bool VEC>
+template <int MODE>
 __device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8, const float2 (&y)[4], const float2 (&mul)[4])
 {
     uint32_t a, b;
@@ -298,28 +367,35 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8,
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             v[j] = fma2(y[j], mul[j], magic);
-            if constexpr (!VEC) {  // the eight values may have different scales
+            if constexpr (MODE == kElements) {  // the eight values may have different scales
                 if (mul[j].x != mul[j].x) v[j].x = 0.0f;
                 if (mul[j].y != mul[j].y) v[j].y = 0.0f;
             }
         }
         a = pack_bytes(v[0], v[1]), b = pack_bytes(v[2], v[3]);
-        if (VEC && mul[0].x != mul[0].x) a = b = 0u;
+        if (MODE != kElements && mul[0].x != mul[0].x) a = b = 0u;
     } else {
         a = e4m3x2_of(mul2(y[0], mul[0])) | (e4m3x2_of(mul2(y[1], mul[1])) << 16);
         b = e4m3x2_of(mul2(y[2], mul[2])) | (e4m3x2_of(mul2(y[3], mul[3])) << 16);
     }
-    if constexpr (VEC) {
+    if constexpr (MODE == kVec) {
         *reinterpret_cast<uint2*>(row + c) = make_uint2(a, b);
     } else {
+        if constexpr (MODE == kPairs) {
+            if (whole_pairs(c, k)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<uint16_t*>(row + c + 64 * j) = static_cast<uint16_t>((j < 2 ? a : b) >> (16 * (j & 1)));
+                return;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (c + j * kColumnStep<VEC> < k) row[c + j * kColumnStep<VEC>] = static_cast<uint8_t>((j < 4 ? a : b) >> (8 * (j & 3)));
+            if (in_row(column<MODE>(c, j), k)) row[column<MODE>(c, j)] = static_cast<uint8_t>((j < 4 ? a : b) >> (8 * (j & 3)));
     }
 }
 
 // One row per TPR threads: a warp (blocks of 128 threads hold four rows) or the whole block.  Thread t owns chunks t, t + TPR, ...
-template <typename T, int TPR, int NCHUNK, bool VEC>
+template <typename T, int TPR, int NCHUNK, int MODE>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 128)
 rms_norm_kernel(const NormArgs p)
 {
@@ -330,38 +406,42 @@ rms_norm_kernel(const NormArgs p)
     if (row >= p.m) return;  // whole warps; never with a block per row
     const int k = p.k;
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const int shift = row_shift<MODE>(x);
+    const PairRange range = pair_range<MODE>(row, p.m, k);
     const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.ld_residual : nullptr;
     Raw8<T> xr[NCHUNK], rr[NCHUNK];
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, VEC>(t, i);
+        const int c = first_column<TPR, MODE>(t, i, shift);
         if (c < k) {
-            load_chunk<T, VEC>(x, c, k, xr[i]);
-            if (r) load_chunk<T, VEC>(r, c, k, rr[i]);
+            load_chunk<T, MODE>(x, c, k, range, xr[i]);
+            if (r) load_chunk<T, MODE>(r, c, k, range, rr[i]);
         }
     }
     constexpr bool EARLY = NCHUNK == 1;  // gamma is requested with the row: where few rows leave latency to count
     float2 early[4];
     if constexpr (EARLY) {
-        const int c = first_column<TPR, VEC>(t, 0);
-        if (c < k) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, early);
+        const int c = first_column<TPR, MODE>(t, 0, shift);
+        if (c < k) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, early);
     }
     float2 hg[NCHUNK][4], ss2 = both(0.0f);
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, VEC>(t, i);
+        const int c = first_column<TPR, MODE>(t, i, shift);
         if (c < k) {
             float2 g[4];
+            finish_chunk<T, MODE>(x, c, k, range, xr[i]);
             unpack8(xr[i], hg[i]);
             if (r) {
                 float2 v[4];
+                finish_chunk<T, MODE>(r, c, k, range, rr[i]);
                 unpack8(rr[i], v);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) hg[i][j] = add2(hg[i][j], v[j]);
             }
-            if (p.sum) store_chunk<T, VEC>(static_cast<T*>(p.sum) + row * p.ld_sum, c, k, hg[i]);
-            if constexpr (!EARLY) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, g);
+            if (p.sum) store_chunk<T, MODE>(static_cast<T*>(p.sum) + row * p.ld_sum, c, k, hg[i]);
+            if constexpr (!EARLY) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (EARLY) g[j] = early[j];
@@ -382,12 +462,12 @@ rms_norm_kernel(const NormArgs p)
         T* y = static_cast<T*>(p.y) + row * p.ldy;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = first_column<TPR, VEC>(t, i);
+            const int c = first_column<TPR, MODE>(t, i, shift);
             if (c < k) {
                 float2 v[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = mul2(hg[i][j], both(rstd));
-                store_chunk<T, VEC>(y, c, k, v);
+                store_chunk<T, MODE>(y, c, k, v);
             }
         }
     }
@@ -401,29 +481,29 @@ rms_norm_kernel(const NormArgs p)
         if (t == 0) static_cast<float*>(p.scale)[row] = scale;
     }
     const int lanes = p.group_lanes;
-    const int shift = 31 - __clz(lanes * 8);  // columns per group: a power of two
-    const long long group0 = row * ((k + lanes * 8 - 1) >> shift);
-    auto scale_group = [&](float g, int column, bool writes) {  // the group's largest magnitude -> its scale, stored, and the reciprocal
+    const int group_bits = 31 - __clz(lanes * 8);  // columns per group: a power of two
+    const long long group0 = row * ((k + lanes * 8 - 1) >> group_bits);
+    auto scale_group = [&](float g, int col, bool writes) {  // the group's largest magnitude -> its scale, stored, and the reciprocal
         float r;
         if (p.scale_mode == ASCB200_SCALE_MX) {
             const uint32_t byte = mx_scale_byte(g, r);
-            if (writes) static_cast<uint8_t*>(p.scale)[group0 + (column >> shift)] = static_cast<uint8_t>(byte);
+            if (writes) static_cast<uint8_t*>(p.scale)[group0 + (col >> group_bits)] = static_cast<uint8_t>(byte);
         } else {
             float scale;
             scale_of(g, s8, scale, r);
-            if (writes) static_cast<float*>(p.scale)[group0 + (column >> shift)] = scale;
+            if (writes) static_cast<float*>(p.scale)[group0 + (col >> group_bits)] = scale;
         }
         return r;
     };
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, VEC>(t, i);
+        const int c = first_column<TPR, MODE>(t, i, shift);
         float2 y[4], mul[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = mul2(hg[i][j], both(rstd)), mul[j] = both(inv);
         if (p.scale_mode != ASCB200_SCALE_PER_TOKEN) {
             // the whole warp takes part in a group's maximum, columns past the row's end with zeros
-            if constexpr (VEC) {  // a group is `lanes` neighbouring lanes
+            if constexpr (MODE == kVec) {  // a group is `lanes` neighbouring lanes
                 float g = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) g = max_abs(g, y[j]);
@@ -431,7 +511,7 @@ rms_norm_kernel(const NormArgs p)
                 const float r = scale_group(g, c, (c / 8 & (lanes - 1)) == 0 && c < k);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) mul[j] = both(r);
-            } else {  // a group is one, two, four or eight of the warp's 32-column runs
+            } else if constexpr (MODE == kElements) {  // a group is one, two, four or eight of the warp's 32-column runs
                 float g[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g[j] = warp_max_abs(fabsf(j & 1 ? y[j / 2].y : y[j / 2].x));
@@ -448,18 +528,18 @@ rms_norm_kernel(const NormArgs p)
                 for (int j = 0; j < 4; ++j) mul[j] = make_float2(g[2 * j], g[2 * j + 1]);
             }
         }
-        if (c < k) store_codes<VEC>(q, c, k, s8, y, mul);
+        if (c < k) store_codes<MODE>(q, c, k, s8, y, mul);
     }
 }
 
 constexpr int kMaxNormK = 32768;
 
-template <typename T, bool VEC>
+template <typename T, int MODE>
 int launch_norm(const NormArgs& p, int sms, cudaStream_t st)
 {
-    const int chunks = (p.k + 7) / 8;
-#define ASCB200_NORM_WARP(NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, 32, NC, VEC>, static_cast<unsigned>((p.m + 3ll) / 4), 128, 0, st, p))
-#define ASCB200_NORM_BLOCK(TPR, NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, TPR, NC, VEC>, p.m, TPR, 0, st, p))
+    const int chunks = (p.k + (MODE == kPairs) + 7) / 8;  // pairs may begin one column early
+#define ASCB200_NORM_WARP(NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, 32, NC, MODE>, static_cast<unsigned>((p.m + 3ll) / 4), 128, 0, st, p))
+#define ASCB200_NORM_BLOCK(TPR, NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, TPR, NC, MODE>, p.m, TPR, 0, st, p))
     // While all rows fit the machine at once with one chunk per thread: that, so that a row's loads are all in flight (us, bf16 with residual and e4m3
     // codes, rows x k: 1 x 4096 2.0, 300 x 1024 2.3 against 3.4 with four chunks per lane, 1200 x 1024 3.3 against 4.8, 300 x 4096 3.3
     // against 4.1).  More rows: two to four chunks per thread, whose reductions cost less per element (600 x 4096 4.3 against 4.8,
@@ -493,6 +573,28 @@ bool resolve_ld(int64_t& ld, int k)
 }
 bool element_aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool rows_aligned(const void* p, int64_t ld, int bytes, int to) { return !p || (aligned_to(p, to) && (ld * bytes) % to == 0); }
+
+// Where elements of `bytes` lie to pairs of them: the parity of the first row's place and of the leading dimension.  kPairs needs the same of
+// every tensor, so that their rows' pairs begin at the same column; absent tensors agree with all.
+struct PairPlace {
+    int first = -1, step = -1;
+    bool same = true;
+    void add(const void* p, int64_t ld, int bytes)
+    {
+        if (!p) return;
+        const int f = static_cast<int>((reinterpret_cast<uintptr_t>(p) / bytes) & 1), s = static_cast<int>(ld & 1);
+        same = same && (first < 0 || (first == f && step == s));
+        first = f, step = s;
+    }
+};
+template <typename T>
+int launch_norm_mode(const NormArgs& p, int mode, int sms, cudaStream_t st)
+{
+    if (mode == kVec) return launch_norm<T, kVec>(p, sms, st);
+    if constexpr (sizeof(T) == 2)
+        if (mode == kPairs) return launch_norm<T, kPairs>(p, sms, st);
+    return launch_norm<T, kElements>(p, sms, st);
+}
 
 int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
 {
@@ -545,14 +647,19 @@ int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
     p.rstd = d.rstd_dev;
     p.ldx = d.ldx, p.ld_residual = d.ld_residual, p.ld_sum = d.ld_sum, p.ldy = d.ldy, p.ldq = d.ldq;
     p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32, p.q_s8 = d.q_dtype == ASCB200_S8, p.scale_mode = d.scale_mode, p.eps = d.eps;
-    // 16-byte accesses where every row of every tensor allows them, element by element otherwise (see first_column)
-    const bool vec = d.k % 8 == 0 && rows_aligned(d.x_dev, d.ldx, esz, 16) && rows_aligned(d.residual_dev, d.ld_residual, esz, 16) && rows_aligned(d.sum_dev, d.ld_sum, esz, 16) &&
-                     rows_aligned(d.y_dev, d.ldy, esz, 16) && rows_aligned(d.q_dev, d.ldq, 1, 8) && (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
+    const bool vec = d.k % 8 == 0 && rows_aligned(d.x_dev, d.ldx, esz, 16) && rows_aligned(d.residual_dev, d.ld_residual, esz, 16) &&
+                     rows_aligned(d.sum_dev, d.ld_sum, esz, 16) && rows_aligned(d.y_dev, d.ldy, esz, 16) && rows_aligned(d.q_dev, d.ldq, 1, 8) &&
+                     (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
+    PairPlace pairs;
+    pairs.add(d.x_dev, d.ldx, esz), pairs.add(d.residual_dev, d.ld_residual, esz), pairs.add(d.sum_dev, d.ld_sum, esz), pairs.add(d.y_dev, d.ldy, esz);
+    pairs.add(d.q_dev, d.ldq, 1);
+    // (groups of columns end inside pairs that begin one column early)
+    const int mode = vec ? kVec : esz == 2 && pairs.same && (!d.q_dev || d.scale_mode == ASCB200_SCALE_PER_TOKEN) ? kPairs : kElements;
     const int sms = st->sm_count;
     switch (d.dtype) {
-        case ASCB200_F16: return vec ? launch_norm<__half, true>(p, sms, stream) : launch_norm<__half, false>(p, sms, stream);
-        case ASCB200_BF16: return vec ? launch_norm<__nv_bfloat16, true>(p, sms, stream) : launch_norm<__nv_bfloat16, false>(p, sms, stream);
-        default: return vec ? launch_norm<float, true>(p, sms, stream) : launch_norm<float, false>(p, sms, stream);
+        case ASCB200_F16: return launch_norm_mode<__half>(p, mode, sms, stream);
+        case ASCB200_BF16: return launch_norm_mode<__nv_bfloat16>(p, mode, sms, stream);
+        default: return launch_norm_mode<float>(p, mode, sms, stream);
     }
 }
 
@@ -584,21 +691,38 @@ struct GradRow {
     Raw8<T> dy[NCHUNK], h[NCHUNK], dh[NCHUNK];
     float rstd;
 };
-template <typename T, int TPR, int NCHUNK, bool VEC>
-__device__ __forceinline__ void load_grad_row(const NormGradArgs& p, long long row, int t, GradRow<T, NCHUNK>& r)
+template <typename T, int TPR, int NCHUNK, int MODE>
+__device__ __forceinline__ void load_grad_row(const NormGradArgs& p, long long row, int t, int shift, GradRow<T, NCHUNK>& r)
 {
     if (row >= p.m) return;
     r.rstd = __ldg(p.rstd + row);
     const T* dy = static_cast<const T*>(p.dy) + row * p.ld_dy;
     const T* h = static_cast<const T*>(p.h) + row * p.ldh;
     const T* dh = static_cast<const T*>(p.dh) + row * p.ld_dh;
+    const PairRange range = pair_range<MODE>(row, p.m, p.k);
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, VEC>(t, i);
+        const int c = first_column<TPR, MODE>(t, i, shift);
         if (c < p.k) {
-            load_chunk<T, VEC>(dy, c, p.k, r.dy[i]);
-            load_chunk<T, VEC>(h, c, p.k, r.h[i]);
-            if (p.dh) load_chunk<T, VEC>(dh, c, p.k, r.dh[i]);
+            load_chunk<T, MODE>(dy, c, p.k, range, r.dy[i]);
+            load_chunk<T, MODE>(h, c, p.k, range, r.h[i]);
+            if (p.dh) load_chunk<T, MODE>(dh, c, p.k, range, r.dh[i]);
+        }
+    }
+}
+template <typename T, int TPR, int NCHUNK, int MODE>
+__device__ __forceinline__ void finish_grad_row(const NormGradArgs& p, long long row, int t, int shift, GradRow<T, NCHUNK>& r)
+{
+    if constexpr (MODE == kPairs) {
+        const PairRange range = pair_range<MODE>(row, p.m, p.k);
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i) {
+            const int c = first_column<TPR, MODE>(t, i, shift);
+            if (c < p.k) {
+                finish_chunk<T, MODE>(static_cast<const T*>(p.dy) + row * p.ld_dy, c, p.k, range, r.dy[i]);
+                finish_chunk<T, MODE>(static_cast<const T*>(p.h) + row * p.ldh, c, p.k, range, r.h[i]);
+                if (p.dh) finish_chunk<T, MODE>(static_cast<const T*>(p.dh) + row * p.ld_dh, c, p.k, range, r.dh[i]);
+            }
         }
     }
 }
@@ -606,12 +730,12 @@ __device__ __forceinline__ void load_grad_row(const NormGradArgs& p, long long r
 // TPR threads per row as above; a block holds ROWS rows at a time (blocks of 256 threads for warp rows).  Up to two chunks per thread keep gamma,
 // dy * gamma and hat in registers from the reduction to the output, and (16-bit types) request the next row before the current one is
 // worked on; more chunks read gamma and unpack dy and h twice.
-template <typename T, int TPR, int NCHUNK, bool VEC>
+template <typename T, int TPR, int NCHUNK, int MODE>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 256, grad_blocks_per_sm(TPR, NCHUNK, sizeof(T)))
 rms_norm_grad_kernel(const NormGradArgs p)
 {
     constexpr int ROWS = TPR > 32 ? 1 : 8;
-    constexpr bool AHEAD = VEC && NCHUNK * sizeof(T) <= 4;  // (single elements are put together as they come, which waits for them)
+    constexpr bool AHEAD = MODE != kElements && NCHUNK * sizeof(T) <= 4;  // (single elements are put together as they come, which waits for them)
     constexpr bool KEEP = NCHUNK == 1 || (NCHUNK == 2 && TPR > 32);
     constexpr int HELD = KEEP ? NCHUNK : 1;
     __shared__ float2 red[2][32];
@@ -621,39 +745,42 @@ rms_norm_grad_kernel(const NormGradArgs p)
     const int sub = TPR > 32 ? 0 : threadIdx.x >> 5;
     const int k = p.k;
     const float inv_k = __frcp_rn(static_cast<float>(k));
+    const long long step = static_cast<long long>(gridDim.x) * ROWS;
+    long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
+    // A thread's columns are the same in all of its rows: kPairs' shift too, since the rows are an even number apart (see grad_blocks).
+    const int shift = row_shift<MODE>(static_cast<const T*>(p.dy) + row * p.ld_dy);
     float2 acc[NCHUNK][4], gamma[HELD][4], hat[HELD][4], g[HELD][4];
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = both(0.0f);
         if constexpr (KEEP) {
-            const int c = first_column<TPR, VEC>(t, i);
-            if (c < k) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, gamma[i]);
+            const int c = first_column<TPR, MODE>(t, i, shift);
+            if (c < k) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[i]);
         }
     }
     int parity = 0;
-    const long long step = static_cast<long long>(gridDim.x) * ROWS;
-    long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
     GradRow<T, NCHUNK> r, next;
-    if constexpr (AHEAD) load_grad_row<T, TPR, NCHUNK, VEC>(p, row, t, next);
+    if constexpr (AHEAD) load_grad_row<T, TPR, NCHUNK, MODE>(p, row, t, shift, next);
     for (; row < p.m; row += step, parity ^= 1) {
         if constexpr (AHEAD) {
             r = next;
-            load_grad_row<T, TPR, NCHUNK, VEC>(p, row + step, t, next);
+            load_grad_row<T, TPR, NCHUNK, MODE>(p, row + step, t, shift, next);
         } else {
-            load_grad_row<T, TPR, NCHUNK, VEC>(p, row, t, r);
+            load_grad_row<T, TPR, NCHUNK, MODE>(p, row, t, shift, r);
         }
+        finish_grad_row<T, TPR, NCHUNK, MODE>(p, row, t, shift, r);
         const float2 rstd = both(r.rstd);
         float2 dot2 = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = first_column<TPR, VEC>(t, i);
+            const int c = first_column<TPR, MODE>(t, i, shift);
             const int held = KEEP ? i : 0;
             if (c < k) {
                 float2 a[4];
                 unpack8(r.dy[i], a);
                 unpack8(r.h[i], hat[held]);
-                if constexpr (!KEEP) load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, gamma[held]);
+                if constexpr (!KEEP) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[held]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     hat[held][j] = mul2(hat[held][j], rstd);
@@ -669,7 +796,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
         T* dx = static_cast<T*>(p.dx) + row * p.ld_dx;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = first_column<TPR, VEC>(t, i);
+            const int c = first_column<TPR, MODE>(t, i, shift);
             const int held = KEEP ? i : 0;
             if (c < k) {
                 float2 e[4];
@@ -677,7 +804,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
                     float2 a[4];
                     unpack8(r.dy[i], a);
                     unpack8(r.h[i], hat[held]);
-                    load_gamma<T, VEC>(p.gamma, p.gamma_f32, c, k, gamma[held]);
+                    load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[held]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) hat[held][j] = mul2(hat[held][j], rstd), g[held][j] = mul2(a[j], gamma[held][j]);
                 }
@@ -689,7 +816,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) e[j] = fma2(fma2(hat[held][j], minus_mean, g[held][j]), rstd, e[j]);
-                store_chunk<T, VEC>(dx, c, k, e);
+                store_chunk<T, MODE>(dx, c, k, e);
             }
         }
     }
@@ -705,15 +832,18 @@ rms_norm_grad_kernel(const NormGradArgs p)
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int col = first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>;
-                if (col < k) put(col, j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
+                const int col = column<MODE>(first_column<TPR, MODE>(t, i, shift), j);
+                if (in_row(col, k)) put(col, j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
             }
     } else {
         constexpr int W = TPR * NCHUNK * 8;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) warp_acc[sub * W + first_column<TPR, VEC>(t, i) + j * kColumnStep<VEC>] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
+            for (int j = 0; j < 8; ++j) {
+                const int col = column<MODE>(first_column<TPR, MODE>(t, i, shift), j);
+                if (in_row(col, k)) warp_acc[sub * W + col] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
+            }
         __syncthreads();
         for (int col = threadIdx.x; col < k; col += 256) {
             float v = 0.0f;
@@ -731,29 +861,39 @@ int grad_blocks(int m, int k)
     const int chunks = (k + 7) / 8;
     const long long most = chunks <= 64 ? 592 : chunks <= 128 ? 888 : chunks <= 256 ? 592 : 296;
     const long long rows = chunks <= 64 ? (m + 7ll) / 8 : m;
-    return static_cast<int>(std::min(most, std::min(rows, std::max(148ll, rows / 4))));  // four rows at a time before a second block per SM
+    const int blocks = static_cast<int>(std::min(most, std::min(rows, std::max(148ll, rows / 4))));  // four rows at a time before a second block per SM
+    return blocks > 1 ? blocks & ~1 : blocks;
 }
 
-template <typename T, int TPR, int NCHUNK, bool VEC>
+template <typename T, int TPR, int NCHUNK, int MODE>
 int launch_norm_grad_as(const NormGradArgs& p, cudaStream_t st, int* blocks)
 {
     constexpr size_t smem = TPR > 32 ? 0 : 8 * TPR * NCHUNK * 8 * sizeof(float);
     *blocks = grad_blocks(p.m, p.k);
-    ASCB200_CUDA(launch_pdl(rms_norm_grad_kernel<T, TPR, NCHUNK, VEC>, *blocks, TPR > 32 ? TPR : 256, smem, st, p));
+    ASCB200_CUDA(launch_pdl(rms_norm_grad_kernel<T, TPR, NCHUNK, MODE>, *blocks, TPR > 32 ? TPR : 256, smem, st, p));
     return ASCB200_OK;
 }
-template <typename T, bool VEC>
+template <typename T, int MODE>
 int launch_norm_grad(const NormGradArgs& p, cudaStream_t st, int* blocks)
 {
     const int chunks = (p.k + 7) / 8;
-    if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, VEC>(p, st, blocks);
-    if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, VEC>(p, st, blocks);
-    if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, VEC>(p, st, blocks);
-    if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, VEC>(p, st, blocks);
-    if (chunks <= 512) return launch_norm_grad_as<T, 512, 1, VEC>(p, st, blocks);
-    if (chunks <= 1024) return launch_norm_grad_as<T, 512, 2, VEC>(p, st, blocks);
-    if (chunks <= 2048) return launch_norm_grad_as<T, 512, 4, VEC>(p, st, blocks);
-    return launch_norm_grad_as<T, 1024, 4, VEC>(p, st, blocks);
+    if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, MODE>(p, st, blocks);
+    if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, MODE>(p, st, blocks);
+    if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, MODE>(p, st, blocks);
+    if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, MODE>(p, st, blocks);
+    if (chunks <= 512) return launch_norm_grad_as<T, 512, 1, MODE>(p, st, blocks);
+    if (chunks <= 1024) return launch_norm_grad_as<T, 512, 2, MODE>(p, st, blocks);
+    if (chunks <= 2048) return launch_norm_grad_as<T, 512, 4, MODE>(p, st, blocks);
+    return launch_norm_grad_as<T, 1024, 4, MODE>(p, st, blocks);
+}
+
+template <typename T>
+int launch_norm_grad_mode(const NormGradArgs& p, int mode, cudaStream_t st, int* blocks)
+{
+    if (mode == kVec) return launch_norm_grad<T, kVec>(p, st, blocks);
+    if constexpr (sizeof(T) == 2)
+        if (mode == kPairs) return launch_norm_grad<T, kPairs>(p, st, blocks);
+    return launch_norm_grad<T, kElements>(p, st, blocks);
 }
 
 size_t grad_workspace(int m, int k) { return m <= 0 || k <= 0 ? 0 : static_cast<size_t>(grad_blocks(m, k)) * k * sizeof(float); }
@@ -790,14 +930,16 @@ int run_rms_norm_grad(const ascb200_rms_norm_grad_desc* desc, cudaStream_t strea
     p.ld_dy = d.ld_dy, p.ldh = d.ldh, p.ld_dh = d.ld_dh, p.ld_dx = d.ld_dx, p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32;
     const bool vec = d.k % 8 == 0 && rows_aligned(d.dy_dev, d.ld_dy, esz, 16) && rows_aligned(d.h_dev, d.ldh, esz, 16) && rows_aligned(d.dh_dev, d.ld_dh, esz, 16) &&
                      rows_aligned(d.dx_dev, d.ld_dx, esz, 16) && (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
+    PairPlace pairs;
+    pairs.add(d.dy_dev, d.ld_dy, esz), pairs.add(d.h_dev, d.ldh, esz), pairs.add(d.dh_dev, d.ld_dh, esz), pairs.add(d.dx_dev, d.ld_dx, esz);
+    // (k % 8: the early column must not change the number of chunks, by which the blocks are counted)
+    const int mode = vec ? kVec : esz == 2 && pairs.same && d.k % 8 != 0 ? kPairs : kElements;
     p.dgamma = d.dgamma_dev, p.dgamma_dtype = d.dgamma_dtype;
     int blocks = 0, rc;
     switch (d.dtype) {
-        case ASCB200_F16: rc = vec ? launch_norm_grad<__half, true>(p, stream, &blocks) : launch_norm_grad<__half, false>(p, stream, &blocks); break;
-        case ASCB200_BF16:
-            rc = vec ? launch_norm_grad<__nv_bfloat16, true>(p, stream, &blocks) : launch_norm_grad<__nv_bfloat16, false>(p, stream, &blocks);
-            break;
-        default: rc = vec ? launch_norm_grad<float, true>(p, stream, &blocks) : launch_norm_grad<float, false>(p, stream, &blocks);
+        case ASCB200_F16: rc = launch_norm_grad_mode<__half>(p, mode, stream, &blocks); break;
+        case ASCB200_BF16: rc = launch_norm_grad_mode<__nv_bfloat16>(p, mode, stream, &blocks); break;
+        default: rc = launch_norm_grad_mode<float>(p, mode, stream, &blocks);
     }
     if (rc != ASCB200_OK || !d.dgamma_dev || blocks == 1) return rc;
     return sum_partials(p.partial, d.dgamma_dev, d.dgamma_dtype, blocks, d.k, stream);

@@ -108,6 +108,28 @@ def test_forward_strides_and_alignment(dtype, k, pad, offset):
     check_codes(check_floats(x, r, w, out, TORCH[dtype]), out, torch.int8, ab.SCALE_PER_TOKEN, 0)
 
 
+@pytest.mark.parametrize("k", [1, 2, 7, 63, 250, 255, 257, 300, 509, 1022, 2047, 4098, 7167, 16383, 32767])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (0, 1), (1, 0), (1, 1), (2, 1), (5, 6)])
+def test_forward_in_pairs(k, pad, offset):
+    """Rows of every parity, alternating ones among them, with and without codes, whose own rows may lie otherwise."""
+    for dtype in (torch.bfloat16, torch.float16):
+        x, r, w, out = forward(5, k, dtype, pad=pad, offset=offset, gamma="f32" if k % 2 else "same", q=torch.int8 if k % 3 else torch.float8_e4m3fn)
+        check_codes(check_floats(x, r, w, out, dtype), out, torch.int8 if k % 3 else torch.float8_e4m3fn, ab.SCALE_PER_TOKEN, 0)
+
+
+def test_forward_with_rows_that_lie_differently():
+    """x and y on other parities: element by element."""
+    dev()
+    for ldx, ldy in ((100, 101), (101, 100), (101, 103), (102, 104)):
+        x = rows_in(torch.randn(9, 99, generator=gen(ldx)), torch.bfloat16, ldx - 99)
+        y = Out(9, 99, torch.bfloat16, ldy - 99)
+        ab.check(ab.rms_norm(ab.RmsNormDesc(m=9, k=99, dtype=ab.BF16, x_dev=ptr(x), ldx=ldx, y_dev=y.ptr(), ldy=ldy, eps=EPS), stream()))
+        torch.cuda.synchronize()
+        y.check()
+        want = reference(x.cpu(), None, None)[2]
+        near(y.t, want, (2.0**-8 + 48 * F) * want.abs(), "y")
+
+
 @pytest.mark.parametrize("residual,gamma,y", [(False, "same", True), (True, None, True), (False, "f32", False), (True, "f32", True)])
 def test_forward_without_residual_or_gamma(residual, gamma, y):
     for dtype in TORCH.values():
@@ -230,6 +252,13 @@ def test_gradient_sizes(m, k, dtype):
 @pytest.mark.parametrize("k", [104, 1027, 3000])
 def test_gradient_forms(k, gamma, dh, dgamma, pad, offset):
     backward(40, k, torch.bfloat16, gamma=gamma, dh=dh, dgamma=dgamma, pad=pad, offset=offset)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 9, 70, 601])
+@pytest.mark.parametrize("k,pad,offset", [(2, 0, 0), (255, 0, 1), (257, 0, 0), (509, 1, 1), (511, 0, 0), (511, 2, 3), (513, 0, 0), (1023, 0, 0), (1026, 1, 0), (3001, 0, 1), (512, 1, 0), (512, 1, 1)])
+def test_gradient_in_pairs(m, k, pad, offset):
+    backward(m, k, torch.bfloat16, gamma="f32" if m % 2 else "same", pad=pad, offset=offset)
+    backward(m, k, torch.float16, dh=False, pad=pad, offset=offset, dgamma=torch.float16)
 
 
 def test_gradient_against_differences():
