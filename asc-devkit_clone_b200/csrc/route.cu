@@ -115,12 +115,12 @@ struct Best3 {
 // Choice number `lane` of a token by comparisons of the values themselves: numbers in descending order, then NaN, equal ones in the order of
 // the experts; -inf never.  One pass over a lane's logits per choice: for the rare tokens.
 template <typename T, int NV>
-__device__ __noinline__ void choose_exactly(const T* row, int E, int K, int lane, int& my_idx)
+__device__ __noinline__ int choose_exactly(const T* row, int E, int K, int lane)
 {
     float x[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i] = lane + 32 * i < E ? to_f32(row[lane + 32 * i]) : kNegInf;
-    my_idx = -1;
+    int my_idx = -1;
     float last = __builtin_huge_valf();
     int last_e = -1;
     bool nan = false;  // the numbers are used up
@@ -153,6 +153,7 @@ __device__ __noinline__ void choose_exactly(const T* row, int E, int K, int lane
         if (lane == j) my_idx = e;
         last_e = e;
     }
+    return my_idx;
 }
 
 struct RouteArgs {
@@ -237,11 +238,12 @@ route_kernel(const RouteArgs p)
             __syncthreads();
         }
         const T* rows = static_cast<const T*>(p.logits) + token0 * p.ld + lane;
+        const long long ld = p.ld;
         int* idx_out = p.idx + token0 * K + lane;
         float* weights_out = p.weights + token0 * K + lane;
         auto load = [&](int j, const T*& row, T (&to)[NV]) {
             const int t = p.valid ? s_list[min(j, TILE - 1)] : j;
-            row = rows + t * p.ld;
+            row = rows + t * ld;
             if (j >= count) return t;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -305,7 +307,7 @@ route_kernel(const RouteArgs p)
                 const int behind = lane == chosen - 1 ? top : next;  // what was left behind the last choice
                 again |= __any_sync(kAll, lane < chosen && ((my_key ^ behind) & ~low_bits) == 0);
             }
-            if (again) choose_exactly<T, NV>(row - lane, E, K, lane, my_idx);
+            if (again) my_idx = choose_exactly<T, NV>(row - lane, E, K, lane);
             float my_w = 0.0f;
             if (__any_sync(kAll, my_idx >= 0)) {
                 ++used;
@@ -322,8 +324,8 @@ route_kernel(const RouteArgs p)
                 }
             }
             if (lane < K) {
-                idx_out[static_cast<long long>(t) * K] = my_idx;
-                weights_out[static_cast<long long>(t) * K] = my_w;
+                idx_out[t * K] = my_idx;  // less than TILE * kMaxTopK
+                weights_out[t * K] = my_w;
             }
         }
     }
