@@ -56,7 +56,7 @@ __device__ __forceinline__ float value(float z)
     } else if constexpr (ACT == ASCB200_ACT_GELU) {
         float e;
         const float tail = normal_tail(z, e);
-        return z > 0.0f ? fmaf(-z, tail, z) : z * tail;
+        return z > 0.0f ? fmaf(-fminf(z, 64.0f), tail, z) : z * tail;  // (the tail is 0 long before 64: infinity stays)
     } else if constexpr (ACT == ASCB200_ACT_GELU_TANH) return z * sigmoid(tanh_arg(z));
     else if constexpr (ACT == ASCB200_ACT_SILU) return z * sigmoid(z);
     else return z;
@@ -66,8 +66,8 @@ template <int ACT>
 __device__ __forceinline__ float slope(float z)
 {
     if constexpr (ACT == ASCB200_ACT_FASTER_GELU) {
-        const float g = sigmoid(1.702f * z);
-        return g * fmaf(1.702f * z, 1.0f - g, 1.0f);
+        const float a = 1.702f * z, g = sigmoid(a);
+        return g * fmaf(fminf(fmaxf(a, -256.0f), 256.0f), 1.0f - g, 1.0f);  // (a may be infinite where z is not; g or 1 - g is 0 long before)
     } else if constexpr (ACT == ASCB200_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
     else if constexpr (ACT == ASCB200_ACT_GELU) {
         float e;

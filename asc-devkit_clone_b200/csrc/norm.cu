@@ -318,7 +318,8 @@ struct NormArgs {
 constexpr float kTopS8 = 127.0f, kTopE4M3 = 448.0f;
 
 // scale = amax / top and its reciprocal, each within a unit in the last place.  A scale under the smallest normal number counts as zero:
-// its reciprocal would not be finite, and codes times scale are then below 2^-117 anyway.  NaN stays NaN.
+// its reciprocal would not be finite, and codes times scale are then below 2^-117 anyway.  NaN stays NaN.  An infinite scale (of an infinite gamma,
+// or a product beyond fp32) makes e4m3 codes 0 and NaN by y / inf, and int8 codes 0 as where the scale is NaN.
 __device__ __forceinline__ void scale_of(float amax, bool s8, float& scale, float& inv)
 {
     const float s = amax * (s8 ? 1.0f / kTopS8 : 1.0f / kTopE4M3);
@@ -326,7 +327,7 @@ __device__ __forceinline__ void scale_of(float amax, bool s8, float& scale, floa
     scale = none ? 0.0f : s;
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-    inv = none ? 0.0f : r;
+    inv = none ? 0.0f : s8 && s == __builtin_huge_valf() ? __uint_as_float(0x7FC00000u) : r;
 }
 // MX: the shared exponent floor(log2 amax) - 8 (the exponent of the largest e4m3 power of two), biased by 127; 255 marks a block
 // that holds an infinity or a NaN.
@@ -678,7 +679,6 @@ struct NormGradArgs {
     int m, k;
     int gamma_f32;
 };
-
 
 // Blocks that have to fit an SM: 64 registers per thread with one chunk of a 16-bit row, 128 in warp rows.
 constexpr int grad_blocks_per_sm(int tpr, int nchunk, int bytes)

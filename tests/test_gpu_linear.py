@@ -214,6 +214,32 @@ def test_infinite_and_nan_inputs_stay_in_their_rows():
         assert torch.isfinite(y[rows]).all()
 
 
+@pytest.mark.parametrize("name", ACTS)
+def test_activations_at_the_ends_of_the_range(name):
+    """z comes from the bias alone.  From |z| = 200 on every activation is z or 0 and every slope 1 or 0 to the last bit; the infinities as in
+    the formula (NaN where it has an infinity times 0)."""
+    dev()
+    z = torch.tensor([200.0, 1e10, 2.5e38, 3.3e38, -200.0, -1e10, -2.5e38, -3.3e38, math.inf] + ([] if name == "relu" else [math.nan]))
+    n = len(z)
+    code = ACTS[name] if isinstance(ACTS, dict) else getattr(ab, "ACT_" + name.upper())
+    want, slope, _ = act(z.bfloat16().double(), name)
+    for m in (2, 300):
+        x, w = torch.zeros(m, 16, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, 16, dtype=torch.bfloat16, device="cuda")
+        bias, y = z.bfloat16().float().cuda(), torch.empty(m, n, device="cuda")
+        ab.check(ab.linear(ab.LinearDesc(kind=ab.KIND_BF16, m=m, n=n, k=16, x_dev=ptr(x), w_dev=ptr(w), trans_w=1, act=code, bias_dev=ptr(bias), bias_dtype=ab.F32, y_dev=ptr(y),
+                                         y_dtype=ab.F32), stream()))
+        torch.cuda.synchronize()
+        near(y, want.expand(m, n), 1e-37, "y")
+    # the slope of finite z: dbias of one row with dy = 1
+    z, slope = z[:8].bfloat16(), slope[:8]
+    zs, dy, dbias = z[None].cuda(), torch.ones(1, 8, dtype=torch.bfloat16, device="cuda"), torch.empty(8, device="cuda")
+    work = torch.empty(ab.linear_grad_workspace_bytes(1, 8), dtype=torch.uint8, device="cuda")
+    ab.check(ab.linear_grad(ab.LinearGradDesc(kind=ab.KIND_BF16, m=1, n=8, k=16, act=code, trans_w=1, dy_dev=ptr(dy), z_dev=ptr(zs), dbias_dev=ptr(dbias), dbias_dtype=ab.F32,
+                                              workspace_dev=ptr(work), workspace_bytes=work.numel()), stream()))
+    torch.cuda.synchronize()
+    near(dbias, slope, 1e-37, "slope")
+
+
 # ---- gradients -----------------------------------------------------------------------------------------------------------------
 def backward(m, n, k, dtype, name="silu", trans_w=1, pad=0, dx=True, dw=True, dbias=True, dw_dtype=None, dbias_dtype=torch.float32, dy_pad=None, offset=0):
     dev()

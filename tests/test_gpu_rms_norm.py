@@ -5,6 +5,7 @@ additions per thread and ten more across threads: relative error under 64 * 2^-2
 fewer than 48 * 2^-24 of |y|.  On top comes half a step of the output type.
 """
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -175,6 +176,22 @@ def test_a_bad_value_shows_in_its_row_only(bad):
         for name in ("y", "q"):
             assert torch.equal(out[name].t[[0, 2]].float(), ref[name].t[[0, 2]].float())
         assert torch.equal(out["scale"][[0, 2]], ref["scale"][[0, 2]])
+
+
+@pytest.mark.parametrize("k", [1000, 1001])
+@pytest.mark.parametrize("mode,group", [(ab.SCALE_PER_TOKEN, 0), (ab.SCALE_PER_GROUP, 64)])
+def test_int8_codes_beside_an_infinite_product_are_zero(mode, group, k):
+    dev()
+    x, w = torch.ones(1, k, dtype=torch.bfloat16, device="cuda"), torch.ones(k, device="cuda")
+    w[3] = math.inf
+    q, scale = torch.full((1, k), 9, dtype=torch.int8, device="cuda"), torch.zeros(1, -(-k // (group or k)), device="cuda")
+    d = ab.RmsNormDesc(m=1, k=k, dtype=ab.BF16, gamma_dtype=ab.F32, x_dev=ptr(x), gamma_dev=ptr(w), q_dev=ptr(q), scale_dev=ptr(scale), q_dtype=ab.S8, scale_mode=mode,
+                       group_size=group, eps=EPS)
+    ab.check(ab.rms_norm(d, stream()))
+    torch.cuda.synchronize()
+    assert float(scale[0, 0]) == math.inf
+    assert (q[0, : group or k] == 0).all()
+    assert group == 0 or (q[0, group:] == 127).all()
 
 
 def test_extreme_magnitudes():
