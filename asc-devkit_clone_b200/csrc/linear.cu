@@ -7,6 +7,7 @@
 //
 // Gradients: dz = dy * act'(z) and dbias = sum over rows of dz in one pass over dy and z, then dx = dz w and dw = dz^T x as plain GEMMs.
 #include <algorithm>
+#include <type_traits>
 
 #include "activation.cuh"
 #include "gemm_host.cuh"
@@ -413,6 +414,360 @@ int launch_act_grad(const ActGradArgs& p, int act, bool vec, dim3 grid, cudaStre
     return vec ? launch_act_grad_as<T, true>(p, act, grid, st) : launch_act_grad_as<T, false>(p, act, grid, st);
 }
 
+// ---- gradients of a few rows ----------------------------------------------------------------------------------------------------
+// Up to 16 rows everything fits one launch, whose blocks have one of three jobs.  What bounds it is reading w once and writing dw once.
+//   dx    a strip of 64 columns of w; its rows are shared by the blocks of a cluster, and within a block by the warps, 16 at a time.  The sums
+//         meet in shared memory, of the block and then of the cluster, always in the same order.
+//   dw    tiles of 64 x 256: one instruction per 16 x 8 outputs sums all rows.
+//   dbias 256 columns.
+// Each job makes the dz that it needs itself, rounded to the operands' type like the dz of the other path.
+//
+// As in the kernel for a few tokens, the order of the summands and of the columns is free as long as the operands agree.  dx: lane (g, q) reads
+// 16 bytes, columns 8 g .. 8 g + 7, of rows 4 q .. 4 q + 3; the i-th of eight instructions takes the i-th of each lane's columns, two
+// rows packed by one byte permutation.  dw: the columns of an instruction are those that leave a lane with eight neighbours after four.
+constexpr int kGradRows = 16;
+constexpr int kGradThreads = 256, kGradWarps = 8;
+constexpr int kGradStrip = 64;                         // columns of dx per cluster
+constexpr int kGradTileRows = 64, kGradTileCols = 256;  // of dw
+constexpr int kPartLd = kGradStrip + 8;
+
+struct GradRowsArgs {
+    const void* dy;
+    const void* z;
+    const void* x;
+    const void* w;
+    void* dx;
+    void* dw;
+    void* dbias;
+    long long ld_dy, ldz, ldx, ldw, ld_dx, ld_dw;
+    int m, n, k;
+    int dw_f32, dbias_f32;
+    int quads;   // four elements of dy and z from a column that is a multiple of four start on 8 bytes
+    int dw_vec;  // eight elements of dw from a column that is a multiple of eight start on 16 bytes, and k is a multiple of eight
+    int splits;  // blocks per cluster
+    int dx_blocks, dw_blocks;
+};
+
+// Four neighbouring 16-bit elements from column c on, zeros from column n on.
+__device__ __forceinline__ uint2 load_quad(const uint16_t* row, int c, int n, bool aligned)
+{
+    if (aligned && c + 4 <= n) return __ldg(reinterpret_cast<const uint2*>(row + c));
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = c + j < n ? __ldg(row + c + j) : 0u;
+    return make_uint2(v[0] | (v[1] << 16), v[2] | (v[3] << 16));
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t v)
+{
+    T e[2];
+    *reinterpret_cast<uint32_t*>(e) = v;
+    return make_float2(as_f32(e[0]), as_f32(e[1]));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b)
+{
+    T e[2] = {rounded<T>(a), rounded<T>(b)};
+    return *reinterpret_cast<uint32_t*>(e);
+}
+struct RawQuad {
+    uint2 dy, z;
+};
+template <int ACT>
+__device__ __forceinline__ RawQuad load_dz(const GradRowsArgs& p, int t, int c)
+{
+    RawQuad r = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+    if (t < p.m) {
+        r.dy = load_quad(static_cast<const uint16_t*>(p.dy) + t * p.ld_dy, c, p.n, p.quads);
+        if constexpr (ACT != ASCB200_ACT_NONE) r.z = load_quad(static_cast<const uint16_t*>(p.z) + t * p.ldz, c, p.n, p.quads);
+    }
+    return r;
+}
+template <typename T, int ACT>
+__device__ __forceinline__ uint2 dz_of(const RawQuad& r)
+{
+    if constexpr (ACT == ASCB200_ACT_NONE) return r.dy;
+    const float2 a = unpack_pair<T>(r.dy.x), b = unpack_pair<T>(r.dy.y), za = unpack_pair<T>(r.z.x), zb = unpack_pair<T>(r.z.y);
+    return make_uint2(pack_pair<T>(a.x * act::slope<ACT>(za.x), a.y * act::slope<ACT>(za.y)), pack_pair<T>(b.x * act::slope<ACT>(zb.x), b.y * act::slope<ACT>(zb.y)));
+}
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+template <typename T>
+constexpr int kind_of() { return std::is_same<T, __half>::value ? ASCB200_KIND_F16 : ASCB200_KIND_BF16; }
+
+template <typename T, int ACT>
+__device__ __forceinline__ void grad_rows_dx(const GradRowsArgs& p, float (*part)[kGradRows][kPartLd])
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const int rank = blockIdx.x % p.splits, col0 = static_cast<int>(blockIdx.x / p.splits) * kGradStrip;
+    const int chunks = (p.n + 15) / 16, per = (chunks + p.splits - 1) / p.splits;
+    const int first = rank * per, last = min(chunks, first + per);
+    const uint8_t* w = static_cast<const uint8_t*>(p.w);
+    const long long ldw = p.ldw * 2;
+    uint32_t acc[8][4] = {};
+    struct Piece {  // 16 rows x 64 columns of w, with the dz that meets them
+        uint4 v[4];
+        RawQuad dz[2];
+    };
+    auto load = [&](int ch, Piece& to) {
+        const int row = ch * 16 + 4 * q, end = ch < last ? p.n : 0;
+        const uint8_t* at = w + row * ldw;
+#pragma unroll
+        for (int j = 0; j < 4; ++j, at += ldw) {  // (what a piece holds from column k on belongs to no output; behind the last row it is not read)
+            const int bytes = row + j < end ? (row + j < p.n - 1 ? (p.k + 7) / 8 * 16 : p.k * 2) : 0;
+            to.v[j] = load_piece<true>(at, (col0 + 8 * g) * 2, bytes);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) to.dz[h] = load_dz<ACT>(p, end > 0 ? g + 8 * h : kGradRows, row);
+    };
+    auto add = [&](const Piece& from) {
+        const uint2 lo = dz_of<T, ACT>(from.dz[0]), hi = dz_of<T, ACT>(from.dz[1]);
+        const uint32_t r0[4] = {from.v[0].x, from.v[0].y, from.v[0].z, from.v[0].w}, r1[4] = {from.v[1].x, from.v[1].y, from.v[1].z, from.v[1].w};
+        const uint32_t r2[4] = {from.v[2].x, from.v[2].y, from.v[2].z, from.v[2].w}, r3[4] = {from.v[3].x, from.v[3].y, from.v[3].z, from.v[3].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            mma_16x8<kind_of<T>()>(acc[2 * i], lo.x, hi.x, lo.y, hi.y, low_halves(r0[i], r1[i]), low_halves(r2[i], r3[i]));
+            mma_16x8<kind_of<T>()>(acc[2 * i + 1], lo.x, hi.x, lo.y, hi.y, high_halves(r0[i], r1[i]), high_halves(r2[i], r3[i]));
+        }
+    };
+    Piece even, odd;  // one is worked on while the other is on its way
+    load(first + warp, even);
+    for (int ch = first + warp; ch < last; ch += 2 * kGradWarps) {
+        load(ch + kGradWarps, odd);
+        add(even);
+        if (ch + kGradWarps >= last) break;
+        load(ch + 2 * kGradWarps, even);
+        add(odd);
+    }
+    // place i * 8 + s holds column 8 s + i
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float2*>(&part[warp][g + 8 * h][i * 8 + 2 * q]) = make_float2(__uint_as_float(acc[i][2 * h]), __uint_as_float(acc[i][2 * h + 1]));
+    __syncthreads();
+    for (int i = threadIdx.x; i < kGradRows * kGradStrip; i += kGradThreads) {
+        float* at = &part[0][i / kGradStrip][i % kGradStrip];
+        float s = at[0];
+#pragma unroll
+        for (int v = 1; v < kGradWarps; ++v) s += at[v * kGradRows * kPartLd];
+        at[0] = s;
+    }
+    if (p.splits > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+    const int share = (kGradRows * kGradStrip + p.splits - 1) / p.splits;
+    for (int i = rank * share + threadIdx.x; i < min(kGradRows * kGradStrip, (rank + 1) * share); i += kGradThreads) {
+        const int t = i / kGradStrip, c = i % kGradStrip, place = (c & 7) * 8 + (c >> 3);
+        float s = 0.0f;
+        if (p.splits > 1) {
+            const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(&part[0][t][place]));
+            for (int v = 0; v < p.splits; ++v) {
+                uint32_t there;
+                float f;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(v));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there) : "memory");
+                s += f;
+            }
+        } else {
+            s = part[0][t][place];
+        }
+        if (t < p.m && col0 + c < p.k) static_cast<T*>(p.dx)[t * p.ld_dx + col0 + c] = rounded<T>(s);
+    }
+    if (p.splits > 1) {  // a block's sums stay until every block of the cluster has read them
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
+
+constexpr int kALd = kGradTileRows + 8, kBLd = kGradTileCols + 2;  // words; so that a warp's reads fall into different banks
+constexpr int kRunBytes = 256, kRunLd = kRunBytes + 16;            // of a row that a warp writes at once where rows do not start on 16 bytes
+struct DwTile {
+    uint32_t a[kGradRows / 2][kALd];  // rows 2 i and 2 i + 1 of dz, packed
+    uint32_t b[kGradRows / 2][kBLd];  // and of x
+    alignas(16) uint8_t out[kGradWarps][16][kRunLd];
+};
+// A warp writes 16 runs of `count` elements (of E bytes) from shared memory to rows `ld` elements apart, `rows` of which are there: a half warp per row, a
+// lane per 16 bytes of the memory, the ends one by one.  (Element by element an SM's stores, each a partial 32-byte sector or three, took
+// as long as the rest: 15 x 5312 x 1199 15.7 us for dw alone against 6.8 for 15 x 5312 x 1200.)
+template <int E>
+__device__ __forceinline__ void store_runs(uint8_t* to, long long ld, int rows, int count, const uint8_t (*from)[kRunLd], int lane)
+{
+    constexpr int N = 16 / E;  // elements per piece
+#pragma unroll
+    for (int h = 0; h < 16; h += 2) {
+        const int r = h + (lane >> 4), l = lane & 15;
+        if (r >= rows) continue;
+        uint8_t* row = to + r * ld * E;
+        const int head = min(count, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / E);
+        const int pieces = (count - head) / N, tail = head + pieces * N;
+        if (l < pieces) {
+            const int e = (head + l * N) * E;  // its place in the run, a multiple of E
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(from[r]) + e / 4;
+            uint32_t v[4];
+            if (E == 4 || (e & 2) == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = words[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = __byte_perm(words[j], words[j + 1], 0x5432);
+            }
+            *reinterpret_cast<uint4*>(row + e) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        const int single = l < 8 ? l : tail + l - 8;
+        if (l < 8 ? single < head : single < count) {
+            if constexpr (E == 4) reinterpret_cast<uint32_t*>(row)[single] = reinterpret_cast<const uint32_t*>(from[r])[single];
+            else reinterpret_cast<uint16_t*>(row)[single] = reinterpret_cast<const uint16_t*>(from[r])[single];
+        }
+    }
+}
+// Two rows' quads -> four words, one per column.
+__device__ __forceinline__ void put_pairs(uint32_t* to, uint2 a, uint2 b)
+{
+    to[0] = low_halves(a.x, b.x), to[1] = high_halves(a.x, b.x), to[2] = low_halves(a.y, b.y), to[3] = high_halves(a.y, b.y);
+}
+template <typename T, int ACT>
+__device__ __forceinline__ void grad_rows_dw(const GradRowsArgs& p, DwTile& s)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    // A block has a run of tiles, along the columns first.  What a tile needs is requested while the one before it is made.
+    const int across = (p.k + kGradTileCols - 1) / kGradTileCols, tiles = (p.n + kGradTileRows - 1) / kGradTileRows * across;
+    const int block = blockIdx.x - p.dx_blocks;
+    const int first = static_cast<int>(static_cast<long long>(block) * tiles / p.dw_blocks), last = static_cast<int>((block + 1ll) * tiles / p.dw_blocks);
+    constexpr int kQuadsA = kGradTileRows / 4, kQuadsB = kGradTileCols / 4, kB = (kGradRows / 2) * kQuadsB / kGradThreads;
+    const bool has_a = threadIdx.x < (kGradRows / 2) * kQuadsA;
+    const int pair_a = threadIdx.x / kQuadsA, c_a = threadIdx.x % kQuadsA * 4;
+    RawQuad raw_a[2];
+    uint2 raw_b[kB][2];
+    auto fetch = [&](int tile) {
+        const int row0 = tile / across * kGradTileRows, col0 = tile % across * kGradTileCols;
+        if (has_a) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) raw_a[h] = load_dz<ACT>(p, 2 * pair_a + h, row0 + c_a);
+        }
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+            const int at = threadIdx.x + i * kGradThreads, pair = at / kQuadsB, c = at % kQuadsB * 4;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                raw_b[i][h] = 2 * pair + h < p.m ? load_quad(static_cast<const uint16_t*>(p.x) + (2 * pair + h) * p.ldx, col0 + c, p.k, true) : make_uint2(0u, 0u);
+        }
+    };
+    if (first < last) fetch(first);
+    for (int tile = first; tile < last; ++tile) {
+        const int row0 = tile / across * kGradTileRows, col0 = tile % across * kGradTileCols;
+        __syncthreads();  // the tile before has been read
+        if (has_a) put_pairs(&s.a[pair_a][c_a], dz_of<T, ACT>(raw_a[0]), dz_of<T, ACT>(raw_a[1]));
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+            const int at = threadIdx.x + i * kGradThreads;
+            put_pairs(&s.b[at / kQuadsB][at % kQuadsB * 4], raw_b[i][0], raw_b[i][1]);
+        }
+        __syncthreads();
+        if (tile + 1 < last) fetch(tile + 1);
+        const int r = (warp & 3) * 16, half = (warp >> 2) * 128;
+        const int run = p.dw_f32 ? 64 : 128;  // columns per run
+        const uint32_t a0 = s.a[q][r + g], a1 = s.a[q][r + g + 8], a2 = s.a[q + 4][r + g], a3 = s.a[q + 4][r + g + 8];
+#pragma unroll
+        for (int set = 0; set < 4; ++set) {  // 32 columns: the lane gets eight of rows g and g + 8
+            uint32_t d[4][4] = {};
+            const int c = half + set * 32;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = c + 8 * (g >> 1) + 2 * i + (g & 1);
+                mma_16x8<kind_of<T>()>(d[i], a0, a1, a2, a3, s.b[q][at], s.b[q + 4][at]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = row0 + r + g + 8 * h, col = col0 + c + 8 * q;
+                uint8_t* staged = s.out[warp][g + 8 * h];
+                if (p.dw_f32) {
+                    const uint4 v0 = make_uint4(d[0][2 * h], d[0][2 * h + 1], d[1][2 * h], d[1][2 * h + 1]), v1 = make_uint4(d[2][2 * h], d[2][2 * h + 1], d[3][2 * h], d[3][2 * h + 1]);
+                    uint4* out = p.dw_vec ? reinterpret_cast<uint4*>(static_cast<float*>(p.dw) + row * p.ld_dw + col) : reinterpret_cast<uint4*>(staged + ((set & 1) * 32 + 8 * q) * 4);
+                    if (!p.dw_vec || (row < p.n && col < p.k)) out[0] = v0, out[1] = v1;
+                } else {
+                    uint32_t v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = pack_pair<T>(__uint_as_float(d[i][2 * h]), __uint_as_float(d[i][2 * h + 1]));
+                    uint4* out = p.dw_vec ? reinterpret_cast<uint4*>(static_cast<T*>(p.dw) + row * p.ld_dw + col) : reinterpret_cast<uint4*>(staged + (set * 32 + 8 * q) * 2);
+                    if (!p.dw_vec || (row < p.n && col < p.k)) *out = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+            }
+            if (!p.dw_vec && (set == 3 || (p.dw_f32 && set == 1))) {  // a run of 256 bytes per row is together
+                __syncwarp();
+                const int col = col0 + half + (p.dw_f32 ? (set >> 1) * 64 : 0), count = min(run, p.k - col), rows = min(16, p.n - row0 - r);
+                const long long at = static_cast<long long>(row0 + r) * p.ld_dw + col;
+                if (count > 0 && rows > 0) {
+                    if (p.dw_f32) store_runs<4>(static_cast<uint8_t*>(p.dw) + at * 4, p.ld_dw, rows, count, s.out[warp], lane);
+                    else store_runs<2>(static_cast<uint8_t*>(p.dw) + at * 2, p.ld_dw, rows, count, s.out[warp], lane);
+                }
+                __syncwarp();
+            }
+        }
+    }
+}
+
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kGradThreads, 2)
+grad_rows_kernel(const GradRowsArgs p)
+{
+    __shared__ alignas(16) union {
+        float part[kGradWarps][kGradRows][kPartLd];
+        DwTile tile;
+    } s;
+    const int block = blockIdx.x;
+    if (block < p.dx_blocks) {  // while the kernel before this one drains, ask L2 for the first pieces of w (hints only)
+        const int chunks = (p.n + 15) / 16, per = (chunks + p.splits - 1) / p.splits;
+        const int row = (block % p.splits) * per * 16 + threadIdx.x;
+        if (row < p.n) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(p.w) + (row * p.ldw + block / p.splits * kGradStrip) * 2));
+    }
+    grid_dependency_wait();
+    if (block < p.dx_blocks) {
+        grad_rows_dx<T, ACT>(p, s.part);
+    } else if (block < p.dx_blocks + p.dw_blocks) {
+        grad_rows_dw<T, ACT>(p, s.tile);
+    } else {
+        const int c = (block - p.dx_blocks - p.dw_blocks) * kGradThreads + threadIdx.x;
+        if (!p.dbias || c >= p.n) return;
+        float v = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kGradRows; ++t) {
+            if (t >= p.m) break;
+            float f = as_f32(static_cast<const T*>(p.dy)[t * p.ld_dy + c]);
+            if constexpr (ACT != ASCB200_ACT_NONE) f *= act::slope<ACT>(as_f32(static_cast<const T*>(p.z)[t * p.ldz + c]));
+            v += f;
+        }
+        if (p.dbias_f32) static_cast<float*>(p.dbias)[c] = v;
+        else static_cast<T*>(p.dbias)[c] = rounded<T>(v);
+    }
+}
+
+template <typename T>
+int launch_grad_rows(GradRowsArgs p, int act, int sms, cudaStream_t st)
+{
+    const int strips = (p.k + kGradStrip - 1) / kGradStrip, chunks = (p.n + 15) / 16;
+    // w's rows are split while two blocks per SM hold all strips' parts at once and every warp still has a piece.
+    p.splits = p.dx ? std::max(1, std::min({8, 2 * sms / strips, chunks / kGradWarps})) : 1;
+    p.dx_blocks = p.dx ? strips * p.splits : 0;
+    const long long tiles = p.dw ? static_cast<long long>((p.n + kGradTileRows - 1) / kGradTileRows) * ((p.k + kGradTileCols - 1) / kGradTileCols) : 0;
+    p.dw_blocks = static_cast<int>(std::min(tiles, (p.dx ? 4ll : 2ll) * sms));  // (behind dx shorter runs fill the SMs more evenly: 16 x 4096 x 11008 50 against 60 us)
+    int blocks = p.dx_blocks + p.dw_blocks + (p.dbias ? (p.n + kGradThreads - 1) / kGradThreads : 0);
+    blocks = (blocks + p.splits - 1) / p.splits * p.splits;
+    switch (act) {
+#define ASCB200_GRAD_ROWS(A) case A: ASCB200_CUDA(launch_pdl_cluster(grad_rows_kernel<T, A>, blocks, kGradThreads, 0, st, p.splits, p)); return ASCB200_OK;
+        ASCB200_GRAD_ROWS(ASCB200_ACT_FASTER_GELU)
+        ASCB200_GRAD_ROWS(ASCB200_ACT_RELU)
+        ASCB200_GRAD_ROWS(ASCB200_ACT_GELU)
+        ASCB200_GRAD_ROWS(ASCB200_ACT_GELU_TANH)
+        ASCB200_GRAD_ROWS(ASCB200_ACT_SILU)
+        default: ASCB200_CUDA(launch_pdl_cluster(grad_rows_kernel<T, ASCB200_ACT_NONE>, blocks, kGradThreads, 0, st, p.splits, p)); return ASCB200_OK;
+#undef ASCB200_GRAD_ROWS
+    }
+}
+
 constexpr int kActGradBlocks = 592;  // blocks to aim for: four per SM
 int act_grad_row_blocks(int m, int n)
 {
@@ -427,7 +782,8 @@ size_t linear_grad_workspace(int m, int n)
 
 int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
 {
-    if (!current_state()) return ASCB200_ENODEV;
+    DeviceState* state = current_state();
+    if (!state) return ASCB200_ENODEV;
     if (!desc) return ASCB200_EINVAL;
     ascb200_linear_grad_desc d = *desc;
     if (d.m < 0 || d.n <= 0 || d.k <= 0 || (d.trans_w != 0 && d.trans_w != 1)) return ASCB200_EINVAL;
@@ -470,6 +826,17 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
     if (make_dz || d.dbias_dev) {
         if (!d.workspace_dev || d.workspace_bytes < linear_grad_workspace(d.m, d.n)) return ASCB200_EINVAL;
         if (!aligned_to(d.workspace_dev, 16)) return ASCB200_EALIGN;
+    }
+    if (d.m <= kGradRows && d.trans_w && products && d.k < (1 << 30)) {
+        GradRowsArgs p = {};
+        p.dy = d.dy_dev, p.z = d.z_dev, p.x = d.x_dev, p.w = d.w_dev, p.dx = d.dx_dev, p.dw = d.dw_dev, p.dbias = d.dbias_dev;
+        p.ld_dy = d.ld_dy, p.ldz = d.ldz, p.ldx = d.ldx, p.ldw = d.ldw, p.ld_dx = d.ld_dx, p.ld_dw = d.ld_dw, p.m = d.m, p.n = d.n, p.k = d.k;
+        p.dw_f32 = d.dw_dtype == ASCB200_F32, p.dbias_f32 = d.dbias_dtype == ASCB200_F32;
+        p.quads = aligned_to(d.dy_dev, 8) && d.ld_dy % 4 == 0 && (d.act == ASCB200_ACT_NONE || (aligned_to(d.z_dev, 8) && d.ldz % 4 == 0));
+        p.dw_vec = d.k % 8 == 0 && aligned_to(d.dw_dev, 16) && (d.ld_dw * dwsz) % 16 == 0;
+        return d.kind == ASCB200_KIND_F16 ? launch_grad_rows<__half>(p, d.act, state->sm_count, stream) : launch_grad_rows<__nv_bfloat16>(p, d.act, state->sm_count, stream);
+    }
+    if (make_dz || d.dbias_dev) {
         ActGradArgs p = {};
         p.dy = d.dy_dev, p.z = d.z_dev, p.ld_dy = d.ld_dy, p.ldz = d.ldz, p.m = d.m, p.n = d.n;
         if (make_dz) {

@@ -241,7 +241,7 @@ def test_activations_at_the_ends_of_the_range(name):
 
 
 # ---- gradients -----------------------------------------------------------------------------------------------------------------
-def backward(m, n, k, dtype, name="silu", trans_w=1, pad=0, dx=True, dw=True, dbias=True, dw_dtype=None, dbias_dtype=torch.float32, dy_pad=None, offset=0):
+def backward(m, n, k, dtype, name="silu", trans_w=1, pad=0, dx=True, dw=True, dbias=True, dw_dtype=None, dbias_dtype=torch.float32, dy_pad=None, offset=0, out_pads=(3, 5)):
     dev()
     x, w, xs, ws = operands(m, n, k, dtype, trans_w, pad)
     g = gen(m * n + k)
@@ -253,7 +253,7 @@ def backward(m, n, k, dtype, name="silu", trans_w=1, pad=0, dx=True, dw=True, db
     d = ab.LinearGradDesc(kind=KIND[dtype], m=m, n=n, k=k, act=ACTS[name], trans_w=trans_w, dy_dev=ptr(ds), ld_dy=n + dy_pad, z_dev=ptr(zs), ldz=n + dy_pad, x_dev=ptr(xs), ldx=xs.stride(0),
                           w_dev=ptr(ws), ldw=ws.stride(0), workspace_dev=ptr(room), workspace_bytes=size)
     dw_dtype = dw_dtype or dtype
-    gx, gw, gb = Out(m, k, dtype, 3), Out(n if trans_w else k, k if trans_w else n, dw_dtype, 5), Out(1, n, dbias_dtype)
+    gx, gw, gb = Out(m, k, dtype, out_pads[0]), Out(n if trans_w else k, k if trans_w else n, dw_dtype, out_pads[1]), Out(1, n, dbias_dtype)
     if dx:
         d.dx_dev, d.ld_dx = gx.ptr(), gx.ld
     if dw:
@@ -288,6 +288,20 @@ def backward(m, n, k, dtype, name="silu", trans_w=1, pad=0, dx=True, dw=True, db
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 64, 64), (3, 17, 33), (16, 100, 40), (65, 257, 130), (130, 1000, 72), (300, 130, 515), (1000, 64, 264), (2049, 300, 96)])
 def test_gradient_sizes(m, n, k, dtype):
     backward(m, n, k, dtype)
+
+
+@pytest.mark.parametrize("out_pads", [(0, 0), (8, 8), (1, 4)])
+@pytest.mark.parametrize("dtype,dw_dtype", [(torch.float16, None), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 8), (2, 15, 64), (1, 4000, 64), (5, 2050, 515), (16, 1000, 1000), (9, 257, 72), (15, 5312, 1200), (2, 300, 2048), (16, 64, 4096), (8, 16, 20000), (7, 3001, 129)])
+def test_gradient_of_few_rows(m, n, k, dtype, dw_dtype, out_pads):
+    backward(m, n, k, dtype, dw_dtype=dw_dtype, out_pads=out_pads)
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("kw", [dict(dx=False), dict(dw=False), dict(dbias=False), dict(dx=False, dbias=False), dict(dbias_dtype=torch.float16, dy_pad=3, offset=1), dict(dy_pad=0),
+                                dict(dy_pad=16, offset=8, dw=False, dbias=False)])
+def test_gradient_forms_of_few_rows(name, kw):
+    backward(13, 1030, 200, torch.float16, name, pad=1, **kw)
 
 
 @pytest.mark.parametrize("name", ACTS)
