@@ -5,7 +5,8 @@
 // Many rows run on the tensor-core GEMM kernels with the output stage of a linear layer (gemm_linear.cu).  A few tokens run here:
 // the product then reads every weight once and is memory bound.
 //
-// Gradients: dz = dy * act'(z) and dbias = sum over rows of dz in one pass over dy and z, then dx = dz w and dw = dz^T x as plain GEMMs.
+// Gradients: dz = dy * act'(z) and dbias = sum over rows of dz in one pass over dy and z, then dx = dz w and dw = dz^T x as plain GEMMs; of a few
+// rows all in one launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -308,8 +309,9 @@ struct ActGradArgs {
     const void* z;
     void* dz;
     float* partial;  // [row blocks][n], or nullptr
+    void* dbias;     // a single block of rows writes it itself
     long long ld_dy, ldz, ld_dz;
-    int m, n;
+    int m, n, dbias_f32;
 };
 
 template <typename T>
@@ -389,7 +391,9 @@ act_grad_kernel(const ActGradArgs p)
         float v = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v += part[i][threadIdx.x];
-        p.partial[static_cast<size_t>(blockIdx.y) * p.n + c] = v;
+        if (gridDim.y > 1) p.partial[static_cast<size_t>(blockIdx.y) * p.n + c] = v;
+        else if (p.dbias_f32) static_cast<float*>(p.dbias)[c] = v;
+        else static_cast<T*>(p.dbias)[c] = rounded<T>(v);
     }
 }
 
@@ -425,6 +429,11 @@ int launch_act_grad(const ActGradArgs& p, int act, bool vec, dim3 grid, cudaStre
 // As in the kernel for a few tokens, the order of the summands and of the columns is free as long as the operands agree.  dx: lane (g, q) reads
 // 16 bytes, columns 8 g .. 8 g + 7, of rows 4 q .. 4 q + 3; the i-th of eight instructions takes the i-th of each lane's columns, two
 // rows packed by one byte permutation.  dw: the columns of an instruction are those that leave a lane with eight neighbours after four.
+//
+// One launch instead of four, of which two are GEMMs of mostly empty tiles (us, bf16 silu with dbias, n x k, 16 rows here against 17 on the GEMMs: 320 x 481
+// 5.2 / 11.1, 1792 x 3864 14.5 / 25.6, 4096 x 4096 23.4 / 30.4, 11008 x 4096 54 / 61, 4096 x 11008 50 / 60; one row of the last two 46 and 47,
+// 3.9 TB/s).  What keeps it from the memory's rate is the latency of a block's loads: dx alone of 1 x 11008 x 4096 runs at 3.6 TB/s, dw
+// alone at 4.6; 128 registers per thread leave room for two blocks per SM.
 constexpr int kGradRows = 16;
 constexpr int kGradThreads = 256, kGradWarps = 8;
 constexpr int kGradStrip = 64;                         // columns of dx per cluster
@@ -772,6 +781,7 @@ constexpr int kActGradBlocks = 592;  // blocks to aim for: four per SM
 int act_grad_row_blocks(int m, int n)
 {
     const int cols = (n + 255) / 256;
+    if (m <= 32) return 1;  // a launch less (us, fp16 silu with dbias: 17 x 128 x 335 10.6 -> 9.8, 20 x 4096 x 1024 20.9 -> 20.2; 64 x 11008 x 1024 would take 34.0 for 31.6)
     return static_cast<int>(std::min<long long>((m + 7ll) / 8, std::max(1, std::min(296, kActGradBlocks / cols))));
 }
 size_t dz_bytes(int m, int n) { return (static_cast<size_t>(m) * ((static_cast<size_t>(n) + 7) / 8 * 8) * 2 + 255) / 256 * 256; }
@@ -843,13 +853,14 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
             dz = p.dz = d.workspace_dev;
             ld_dz = p.ld_dz = (static_cast<int64_t>(d.n) + 7) / 8 * 8;
         }
+        p.dbias = d.dbias_dev, p.dbias_f32 = d.dbias_dtype == ASCB200_F32;
         if (d.dbias_dev) p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(d.workspace_dev) + dz_bytes(d.m, d.n));
         const bool vec = d.n % 8 == 0 && operand_aligned(d.dy_dev, d.ld_dy, 2) && (d.act == ASCB200_ACT_NONE || operand_aligned(d.z_dev, d.ldz, 2));
         const int rows = act_grad_row_blocks(d.m, d.n);
         const dim3 grid((d.n + 255) / 256, rows);
         const int rc = d.kind == ASCB200_KIND_F16 ? launch_act_grad<__half>(p, d.act, vec, grid, stream) : launch_act_grad<__nv_bfloat16>(p, d.act, vec, grid, stream);
         if (rc != ASCB200_OK) return rc;
-        if (d.dbias_dev) {
+        if (d.dbias_dev && rows > 1) {
             const int rc2 = sum_partials(p.partial, d.dbias_dev, d.dbias_dtype, rows, d.n, stream);
             if (rc2 != ASCB200_OK) return rc2;
         }

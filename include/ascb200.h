@@ -545,7 +545,8 @@ ASCB200_API int ascb200_linear(const ascb200_linear_desc* desc, void* stream);
  * z as the forward call wrote it in the operands' type (not read for ACT_NONE).  dz is rounded to the operands' type for the two products, dbias
  * is summed in fp32 from the values before.  dx, dw and dbias may each be NULL (not wanted); dw and dbias: the operands' type or F32.
  * The workspace holds dz and the partial sums of dbias; without activation and dbias it is not needed when dy is
- * aligned like x.  m = 0 gives dw = 0 and dbias = 0. */
+ * aligned like x.  The order of the fp32 sums depends on the sizes and the device alone (up to 16 rows with trans_w = 1 are one kernel).
+ * m = 0 gives dw = 0 and dbias = 0. */
 typedef struct ascb200_linear_grad_desc {
     int32_t kind;
     int32_t m, n, k;
