@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t ld_element(const void* p, bool inside)
 //              not, the pairs begin one column to the left: the first pair then has only its second column);
 //   kElements  single elements, 32 columns apart, so that a warp's accesses are contiguous whatever the alignment.
 // (us, bf16 with residual and int8 codes, 65536 x 511: neighbouring columns one by one 174, kElements 71, kPairs 57, and the aligned 65536 x 512
-// 38; gradients of 8192 x 4095 / 4096: kElements 117, kPairs 69, kVec 54.)
+// 38; gradients of 8192 x 4095 / 4096: kElements 117, kPairs 69, kVec 50.)
 enum Mode : int { kElements = 0, kVec = 1, kPairs = 2 };
 // `shift`: kPairs, 1 where the row's pairs begin to the left of its first column.  The column may then be -1.
 template <int TPR, int MODE>
@@ -680,66 +680,89 @@ struct NormGradArgs {
     int gamma_f32;
 };
 
-// Blocks that have to fit an SM: 64 registers per thread with one chunk of a 16-bit row, 128 in warp rows.
+// Blocks that have to fit an SM: 64 registers per thread with one chunk of a 16-bit row, else 128.
 constexpr int grad_blocks_per_sm(int tpr, int nchunk, int bytes)
 {
-    return bytes == 4 ? 1 : tpr == 32 ? 2 : nchunk == 1 ? 1024 / tpr : 1;
+    return bytes == 4 ? 1 : tpr == 32 ? 2 : nchunk == 1 ? 1024 / tpr : 512 / tpr;
 }
 
-template <typename T, int NCHUNK>
-struct GradRow {
-    Raw8<T> dy[NCHUNK], h[NCHUNK], dh[NCHUNK];
-    float rstd;
-};
-template <typename T, int TPR, int NCHUNK, int MODE>
-__device__ __forceinline__ void load_grad_row(const NormGradArgs& p, long long row, int t, int shift, GradRow<T, NCHUNK>& r)
+// The rows to come wait in shared memory: every thread copies its own columns of dy, h and dh there (cp.async: no registers, and no barrier, since
+// nobody else reads them) and takes them up STAGES - 1 rows later; STAGES by what an SM has for its blocks.  16-bit rows up to 16384.  With
+// two chunks per thread that beats one whose next row waits in registers (us, bf16, m x k: 8192 x 4096 with dh 53.8 -> 49.6, 16384 x 2048 46.1 -> 40.2,
+// 30000 x 1024 with dh 54.0 -> 45.7, 9107 x 8192 102 -> 77, 9107 x 12288 197 -> 117, 7000 x 16384 with dh 205 -> 151: 6.1 TB/s; one chunk per
+// thread by ring 59 for the first); not where the copies have four bytes, but for long rows (pairs: 6100 x 1427 with dh 21.4 -> 27, 9107 x 9252
+// 262 -> 182), and not for fp32 (two stages: 9107 x 4096 88.5 -> 121).
+constexpr int kGradRing = 200 * 1024;
+constexpr int grad_threads(int tpr) { return tpr > 32 ? tpr : 256; }
+constexpr int grad_stage_bytes(int tpr, int nchunk, int bytes) { return grad_threads(tpr) * nchunk * 8 * bytes * 3; }
+constexpr int grad_resident(int tpr, int nchunk)  // blocks per SM that the grid is made for
 {
-    if (row >= p.m) return;
-    r.rstd = __ldg(p.rstd + row);
-    const T* dy = static_cast<const T*>(p.dy) + row * p.ld_dy;
-    const T* h = static_cast<const T*>(p.h) + row * p.ldh;
-    const T* dh = static_cast<const T*>(p.dh) + row * p.ld_dh;
-    const PairRange range = pair_range<MODE>(row, p.m, p.k);
+    return tpr == 32 ? 4 : nchunk > 1 ? (tpr >= 512 ? 1 : 512 / tpr) : tpr == 128 ? 6 : tpr == 256 ? 4 : 2;
+}
+constexpr int grad_stages(int tpr, int nchunk, int bytes, int mode)
+{
+    const int n = kGradRing / (grad_resident(tpr, nchunk) * grad_stage_bytes(tpr, nchunk, bytes));
+    return bytes == 4 || mode == kElements || (mode == kPairs && (tpr < 512 || nchunk < 2)) || n < 2 ? 0 : n > 4 ? 4 : n;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool inside)  // zeros where not inside
+{
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(inside ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(inside ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One chunk to or from its place: words of 16 bytes (kVec) or four (kPairs), those of the block's threads side by side.
+template <typename T, int MODE>
+__device__ __forceinline__ void copy_chunk(uint32_t place, const T* row, int c, int k, const PairRange& range, int threads)
+{
+    constexpr int WORDS = static_cast<int>(sizeof(T)) * 2;  // of four bytes
+    if constexpr (MODE == kVec) {
 #pragma unroll
-    for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, MODE>(t, i, shift);
-        if (c < p.k) {
-            load_chunk<T, MODE>(dy, c, p.k, range, r.dy[i]);
-            load_chunk<T, MODE>(h, c, p.k, range, r.h[i]);
-            if (p.dh) load_chunk<T, MODE>(dh, c, p.k, range, r.dh[i]);
+        for (int j = 0; j < WORDS / 4; ++j) copy_async<16>(place + (j * threads + threadIdx.x) * 16, row + c + j * 16 / sizeof(T), true);
+    } else {
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) {
+            const int col = c + 64 * j;
+            const bool inside = range.last >= range.first && static_cast<unsigned>(col - range.first) <= static_cast<unsigned>(range.last - range.first);
+            copy_async<4>(place + (j * threads + threadIdx.x) * 4, inside ? row + col : row, inside);
         }
     }
 }
-template <typename T, int TPR, int NCHUNK, int MODE>
-__device__ __forceinline__ void finish_grad_row(const NormGradArgs& p, long long row, int t, int shift, GradRow<T, NCHUNK>& r)
+template <typename T, int MODE>
+__device__ __forceinline__ void take_chunk(const uint8_t* place, int threads, Raw8<T>& r)
 {
-    if constexpr (MODE == kPairs) {
-        const PairRange range = pair_range<MODE>(row, p.m, p.k);
-#pragma unroll
-        for (int i = 0; i < NCHUNK; ++i) {
-            const int c = first_column<TPR, MODE>(t, i, shift);
-            if (c < p.k) {
-                finish_chunk<T, MODE>(static_cast<const T*>(p.dy) + row * p.ld_dy, c, p.k, range, r.dy[i]);
-                finish_chunk<T, MODE>(static_cast<const T*>(p.h) + row * p.ldh, c, p.k, range, r.h[i]);
-                if (p.dh) finish_chunk<T, MODE>(static_cast<const T*>(p.dh) + row * p.ld_dh, c, p.k, range, r.dh[i]);
-            }
-        }
+    constexpr int WORDS = static_cast<int>(sizeof(T)) * 2;
+    if constexpr (MODE == kVec) {
+        const uint4* at = reinterpret_cast<const uint4*>(place) + threadIdx.x;
+        r.v = at[0];
+        if constexpr (WORDS == 8) r.w = at[threads];
+    } else {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(place) + threadIdx.x;
+        r.v = make_uint4(at[0], at[threads], at[2 * threads], at[3 * threads]);
     }
 }
 
 // TPR threads per row as above; a block holds ROWS rows at a time (blocks of 256 threads for warp rows).  Up to two chunks per thread keep gamma,
-// dy * gamma and hat in registers from the reduction to the output, and (16-bit types) request the next row before the current one is
-// worked on; more chunks read gamma and unpack dy and h twice.
+// dy * gamma and hat in registers from the reduction to the output; more chunks unpack dy and h twice (and read gamma twice, without the ring).
 template <typename T, int TPR, int NCHUNK, int MODE>
-__global__ void __launch_bounds__(TPR > 32 ? TPR : 256, grad_blocks_per_sm(TPR, NCHUNK, sizeof(T)))
+__global__ void __launch_bounds__(grad_threads(TPR), grad_blocks_per_sm(TPR, NCHUNK, sizeof(T)))
 rms_norm_grad_kernel(const NormGradArgs p)
 {
-    constexpr int ROWS = TPR > 32 ? 1 : 8;
-    constexpr bool AHEAD = MODE != kElements && NCHUNK * sizeof(T) <= 4;  // (single elements are put together as they come, which waits for them)
+    constexpr int ROWS = TPR > 32 ? 1 : 8, THREADS = grad_threads(TPR);
+    constexpr int STAGES = grad_stages(TPR, NCHUNK, sizeof(T), MODE);
+    constexpr bool RING = STAGES > 0;
+    constexpr bool AHEAD = !RING && MODE != kElements && NCHUNK * sizeof(T) <= 4;  // the next row is requested before this one is worked on
     constexpr bool KEEP = NCHUNK == 1 || (NCHUNK == 2 && TPR > 32);
+    constexpr bool KEEP_GAMMA = KEEP || (RING && TPR > 32);
     constexpr int HELD = KEEP ? NCHUNK : 1;
+    constexpr int CHUNK_BYTES = THREADS * 8 * sizeof(T), ARRAY_BYTES = NCHUNK * CHUNK_BYTES, STAGE_BYTES = 3 * ARRAY_BYTES;
     __shared__ float2 red[2][32];
-    extern __shared__ float warp_acc[];  // warp rows: [8][TPR * NCHUNK * 8]
+    extern __shared__ uint4 dynamic_smem[];  // the ring: [STAGES][dy, h, dh][NCHUNK][THREADS] chunks; warp rows, at the end: [8][TPR * NCHUNK * 8] sums
+    uint8_t* ring = reinterpret_cast<uint8_t*>(dynamic_smem);
     grid_dependency_wait();
     const int t = TPR > 32 ? threadIdx.x : threadIdx.x & 31;
     const int sub = TPR > 32 ? 0 : threadIdx.x >> 5;
@@ -747,45 +770,100 @@ rms_norm_grad_kernel(const NormGradArgs p)
     const float inv_k = __frcp_rn(static_cast<float>(k));
     const long long step = static_cast<long long>(gridDim.x) * ROWS;
     long long row = static_cast<long long>(blockIdx.x) * ROWS + sub;
+    const T* dy = static_cast<const T*>(p.dy);
+    const T* h = static_cast<const T*>(p.h);
+    const T* dh = static_cast<const T*>(p.dh);
     // A thread's columns are the same in all of its rows: kPairs' shift too, since the rows are an even number apart (see grad_blocks).
-    const int shift = row_shift<MODE>(static_cast<const T*>(p.dy) + row * p.ld_dy);
-    float2 acc[NCHUNK][4], gamma[HELD][4], hat[HELD][4], g[HELD][4];
+    const int shift = row_shift<MODE>(dy + row * p.ld_dy);
+    float2 acc[NCHUNK][4], gamma[KEEP_GAMMA ? NCHUNK : 1][4], hat[HELD][4], g[HELD][4];
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = both(0.0f);
-        if constexpr (KEEP) {
+        if constexpr (KEEP_GAMMA) {
             const int c = first_column<TPR, MODE>(t, i, shift);
             if (c < k) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[i]);
         }
     }
-    int parity = 0;
-    GradRow<T, NCHUNK> r, next;
-    if constexpr (AHEAD) load_grad_row<T, TPR, NCHUNK, MODE>(p, row, t, shift, next);
-    for (; row < p.m; row += step, parity ^= 1) {
-        if constexpr (AHEAD) {
-            r = next;
-            load_grad_row<T, TPR, NCHUNK, MODE>(p, row + step, t, shift, next);
-        } else {
-            load_grad_row<T, TPR, NCHUNK, MODE>(p, row, t, shift, r);
+    auto request = [&](long long to_come, int stage) {  // a row into the ring
+        if (to_come < p.m) {
+            const PairRange range = pair_range<MODE>(to_come, p.m, k);
+            const uint32_t place = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + stage * STAGE_BYTES;
+#pragma unroll
+            for (int i = 0; i < NCHUNK; ++i) {
+                const int c = first_column<TPR, MODE>(t, i, shift);
+                if (c < k) {
+                    copy_chunk<T, MODE>(place + i * CHUNK_BYTES, dy + to_come * p.ld_dy, c, k, range, THREADS);
+                    copy_chunk<T, MODE>(place + ARRAY_BYTES + i * CHUNK_BYTES, h + to_come * p.ldh, c, k, range, THREADS);
+                    if (dh) copy_chunk<T, MODE>(place + 2 * ARRAY_BYTES + i * CHUNK_BYTES, dh + to_come * p.ld_dh, c, k, range, THREADS);
+                }
+            }
         }
-        finish_grad_row<T, TPR, NCHUNK, MODE>(p, row, t, shift, r);
-        const float2 rstd = both(r.rstd);
+        copies_end_group();
+    };
+    if constexpr (RING) {
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) request(row + s * step, s);
+    }
+    float next_rstd = row < p.m ? __ldg(p.rstd + row) : 0.0f;
+    int parity = 0, stage = 0;
+    constexpr int RAW = RING ? 1 : NCHUNK;
+    struct Row {
+        Raw8<T> dy[RAW], h[RAW], dh[RAW];
+    };
+    Row raw, next;
+    auto load = [&](long long to_come, Row& to) {
+        if (to_come >= p.m) return;
+        const PairRange range = pair_range<MODE>(to_come, p.m, k);
+#pragma unroll
+        for (int i = 0; i < RAW; ++i) {
+            const int c = first_column<TPR, MODE>(t, i, shift);
+            if (c < k) {
+                load_chunk<T, MODE>(dy + to_come * p.ld_dy, c, k, range, to.dy[i]);
+                load_chunk<T, MODE>(h + to_come * p.ldh, c, k, range, to.h[i]);
+                if (dh) load_chunk<T, MODE>(dh + to_come * p.ld_dh, c, k, range, to.dh[i]);
+            }
+        }
+    };
+    if constexpr (AHEAD) load(row, next);
+    for (; row < p.m; row += step, parity ^= 1) {
+        const PairRange range = pair_range<MODE>(row, p.m, k);
+        const float2 rstd = both(next_rstd);
+        if (row + step < p.m) next_rstd = __ldg(p.rstd + row + step);
+        const uint8_t* place = ring + stage * STAGE_BYTES;
+        if constexpr (RING) {
+            copies_wait_but<RING ? STAGES - 2 : 0>();
+            // the place that the row before has left: its thread has read it for the last time
+            request(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        } else if constexpr (AHEAD) {
+            raw = next;
+            load(row + step, next);
+        } else {
+            load(row, raw);
+        }
+        // chunk i of dy (0), h (1) or dh (2)
+        auto take = [&](int which, int i, int c, float2 (&f)[4]) {
+            Raw8<T>& r = which == 0 ? raw.dy[RING ? 0 : i] : which == 1 ? raw.h[RING ? 0 : i] : raw.dh[RING ? 0 : i];
+            if constexpr (RING) take_chunk<T, MODE>(place + which * ARRAY_BYTES + i * CHUNK_BYTES, THREADS, r);
+            finish_chunk<T, MODE>(which == 0 ? dy + row * p.ld_dy : which == 1 ? h + row * p.ldh : dh + row * p.ld_dh, c, k, range, r);
+            unpack8(r, f);
+        };
         float2 dot2 = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
             const int c = first_column<TPR, MODE>(t, i, shift);
-            const int held = KEEP ? i : 0;
+            const int held = KEEP ? i : 0, gi = KEEP_GAMMA ? i : 0;
             if (c < k) {
                 float2 a[4];
-                unpack8(r.dy[i], a);
-                unpack8(r.h[i], hat[held]);
-                if constexpr (!KEEP) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[held]);
+                take(0, i, c, a);
+                take(1, i, c, hat[held]);
+                if constexpr (!KEEP_GAMMA) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[0]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     hat[held][j] = mul2(hat[held][j], rstd);
                     acc[i][j] = fma2(a[j], hat[held][j], acc[i][j]);
-                    g[held][j] = mul2(a[j], gamma[held][j]);
+                    g[held][j] = mul2(a[j], gamma[gi][j]);
                     dot2 = fma2(g[held][j], hat[held][j], dot2);
                 }
             }
@@ -800,16 +878,17 @@ rms_norm_grad_kernel(const NormGradArgs p)
             const int held = KEEP ? i : 0;
             if (c < k) {
                 float2 e[4];
+                const int gi = KEEP_GAMMA ? i : 0;
                 if constexpr (!KEEP) {
                     float2 a[4];
-                    unpack8(r.dy[i], a);
-                    unpack8(r.h[i], hat[held]);
-                    load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[held]);
+                    take(0, i, c, a);
+                    take(1, i, c, hat[held]);
+                    if constexpr (!KEEP_GAMMA) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[0]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) hat[held][j] = mul2(hat[held][j], rstd), g[held][j] = mul2(a[j], gamma[held][j]);
+                    for (int j = 0; j < 4; ++j) hat[held][j] = mul2(hat[held][j], rstd), g[held][j] = mul2(a[j], gamma[gi][j]);
                 }
-                if (p.dh) {
-                    unpack8(r.dh[i], e);
+                if (dh) {
+                    take(2, i, c, e);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) e[j] = both(0.0f);
@@ -837,6 +916,9 @@ rms_norm_grad_kernel(const NormGradArgs p)
             }
     } else {
         constexpr int W = TPR * NCHUNK * 8;
+        float* warp_acc = reinterpret_cast<float*>(dynamic_smem);
+        if constexpr (RING) copies_wait_but<0>();  // (the last groups are empty)
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
@@ -854,12 +936,12 @@ rms_norm_grad_kernel(const NormGradArgs p)
     }
 }
 
-// Blocks of the gradient kernel, at most: rows of the workspace.  By k alone: as many as fill the machine at 64 registers per thread (16-bit rows of up
-// to 4096), which more than pays for the longer second sum (16384 x 2048 bf16: 80 us with 296 blocks, 56 with 592).
+// Blocks of the gradient kernel, at most: rows of the workspace.  By k alone, about what fits the machine at once (the second sum is longer with
+// more of them, but 16384 x 2048 bf16 took 80 us with 296 blocks where 592 took 56, before there was a ring).
 int grad_blocks(int m, int k)
 {
     const int chunks = (k + 7) / 8;
-    const long long most = chunks <= 64 ? 592 : chunks <= 128 ? 888 : chunks <= 256 ? 592 : 296;
+    const long long most = chunks <= 64 ? 592 : chunks <= 128 ? 888 : chunks <= 256 ? 592 : chunks <= 512 ? 296 : 148;
     const long long rows = chunks <= 64 ? (m + 7ll) / 8 : m;
     const int blocks = static_cast<int>(std::min(most, std::min(rows, std::max(148ll, rows / 4))));  // four rows at a time before a second block per SM
     return blocks > 1 ? blocks & ~1 : blocks;
@@ -868,7 +950,17 @@ int grad_blocks(int m, int k)
 template <typename T, int TPR, int NCHUNK, int MODE>
 int launch_norm_grad_as(const NormGradArgs& p, cudaStream_t st, int* blocks)
 {
-    constexpr size_t smem = TPR > 32 ? 0 : 8 * TPR * NCHUNK * 8 * sizeof(float);
+    constexpr int ring = grad_stages(TPR, NCHUNK, sizeof(T), MODE) * grad_stage_bytes(TPR, NCHUNK, sizeof(T)), sums = TPR > 32 ? 0 : 8 * TPR * NCHUNK * 8 * 4;
+    constexpr int smem = ring > sums ? ring : sums;
+    if constexpr (smem > 46 * 1024) {  // beyond what a launch may take unasked
+        static bool configured[16] = {};
+        int dev = 0;
+        ASCB200_CUDA(cudaGetDevice(&dev));
+        if (!configured[dev & 15]) {
+            ASCB200_CUDA(cudaFuncSetAttribute(rms_norm_grad_kernel<T, TPR, NCHUNK, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            configured[dev & 15] = true;
+        }
+    }
     *blocks = grad_blocks(p.m, p.k);
     ASCB200_CUDA(launch_pdl(rms_norm_grad_kernel<T, TPR, NCHUNK, MODE>, *blocks, TPR > 32 ? TPR : 256, smem, st, p));
     return ASCB200_OK;
@@ -879,9 +971,15 @@ int launch_norm_grad(const NormGradArgs& p, cudaStream_t st, int* blocks)
     const int chunks = (p.k + 7) / 8;
     if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, MODE>(p, st, blocks);
     if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, MODE>(p, st, blocks);
-    if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, MODE>(p, st, blocks);
-    if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, MODE>(p, st, blocks);
-    if (chunks <= 512) return launch_norm_grad_as<T, 512, 1, MODE>(p, st, blocks);
+    if constexpr (MODE != kVec || sizeof(T) == 4) {
+        if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, MODE>(p, st, blocks);
+        if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, MODE>(p, st, blocks);
+        if (chunks <= 512) return launch_norm_grad_as<T, 512, 1, MODE>(p, st, blocks);
+    } else {
+        if (chunks <= 128) return launch_norm_grad_as<T, 64, 2, MODE>(p, st, blocks);
+        if (chunks <= 256) return launch_norm_grad_as<T, 128, 2, MODE>(p, st, blocks);
+        if (chunks <= 512) return launch_norm_grad_as<T, 256, 2, MODE>(p, st, blocks);
+    }
     if (chunks <= 1024) return launch_norm_grad_as<T, 512, 2, MODE>(p, st, blocks);
     if (chunks <= 2048) return launch_norm_grad_as<T, 512, 4, MODE>(p, st, blocks);
     return launch_norm_grad_as<T, 1024, 4, MODE>(p, st, blocks);

@@ -252,8 +252,8 @@ def backward(m, k, dtype, gamma="same", dh=True, pad=0, offset=0, dgamma=torch.f
     near(dx.t, want, HALF_STEP[dtype] * want.abs() + 72 * F * terms + TINY[dtype], "dx")
     if dg is not None:
         dg.check()
-        # m terms added over at most m / blocks + blocks / 8 + 8 steps
-        steps = m / min(m, 296) + 64
+        # m terms added over at most m / blocks + blocks / 8 + 8 steps, with at least 148 blocks for so many rows
+        steps = m / min(m, 148) + 64
         near(dg.t[0], wantg, HALF_STEP[dgamma] * wantg.abs() + steps * F * gterms + TINY[dgamma], "dgamma")
 
 
@@ -276,6 +276,31 @@ def test_gradient_forms(k, gamma, dh, dgamma, pad, offset):
 def test_gradient_in_pairs(m, k, pad, offset):
     backward(m, k, torch.bfloat16, gamma="f32" if m % 2 else "same", pad=pad, offset=offset)
     backward(m, k, torch.float16, dh=False, pad=pad, offset=offset, dgamma=torch.float16)
+
+
+@pytest.mark.parametrize("dh,pad,offset", [(True, 0, 0), (False, 8, 8), (True, 0, 1)])
+@pytest.mark.parametrize("dtype", TORCH)
+@pytest.mark.parametrize("m,k", [(20011, 96), (9001, 328), (9001, 519), (5003, 1040), (2500, 2056), (1300, 4104), (900, 8208), (900, 8201), (300, 16400)])
+def test_gradient_of_many_rows(m, k, dtype, dh, pad, offset):
+    backward(m, k, TORCH[dtype], dh=dh, pad=pad, offset=offset)
+
+
+@pytest.mark.parametrize("over", ["dy", "h", "dh"])
+@pytest.mark.parametrize("dtype", TORCH)
+@pytest.mark.parametrize("m,k", [(3000, 200), (2000, 776), (1700, 1999), (1500, 4096), (700, 8200), (500, 9003), (300, 16392)])
+def test_gradient_in_place(m, k, dtype, over):
+    dev()
+    dtype = TORCH[dtype]
+    g = gen(m + k)
+    t = {c: torch.randn(m, k, generator=g).to(dtype).cuda() for c in ("dy", "h", "dh")}
+    rstd = (1 / torch.sqrt(t["h"].double().square().mean(1) + EPS)).float()
+    gamma = (1 + 0.3 * torch.randn(k, generator=g)).cuda()
+    want, _, terms, _ = grad_reference(t["dy"], t["h"], rstd, gamma, t["dh"])
+    d = ab.RmsNormGradDesc(m=m, k=k, dtype=CODE[dtype], gamma_dtype=ab.F32, dy_dev=ptr(t["dy"]), h_dev=ptr(t["h"]), rstd_dev=ptr(rstd), gamma_dev=ptr(gamma), dh_dev=ptr(t["dh"]),
+                           dx_dev=ptr(t[over]))
+    ab.check(ab.rms_norm_grad(d, stream()))
+    torch.cuda.synchronize()
+    near(t[over], want, HALF_STEP[dtype] * want.abs() + 72 * F * terms + TINY[dtype], "dx over " + over)
 
 
 def test_gradient_against_differences():
