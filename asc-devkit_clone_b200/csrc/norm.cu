@@ -35,7 +35,7 @@ struct Raw8<float> {
 
 // Two fp32 operations per instruction, each rounded to nearest.  The kernels move seven to eight bytes per element, so at the memory's rate an
 // SM has about 30 instruction slots per element: with unpacked arithmetic and a test per chunk for the row's end (31 instructions) the forward
-// pass took 145 us for 16383 x 7168 bf16 with residual and int8 codes; so, 131 us (6.3 TB/s).
+// pass took 145 us for 16383 x 7168 bf16 with residual and int8 codes; so, 131 us, and 124 (6.6 TB/s) since y and its code come from one product.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b)
 {
     float2 r;
@@ -89,12 +89,12 @@ __device__ __forceinline__ uint32_t ld_element(const void* p, bool inside)
 // 38; gradients of 8192 x 4095 / 4096: kElements 117, kPairs 69, kVec 50.)
 enum Mode : int { kElements = 0, kVec = 1, kPairs = 2 };
 // `shift`: kPairs, 1 where the row's pairs begin to the left of its first column.  The column may then be -1.
-template <int TPR, int MODE>
-__device__ __forceinline__ int first_column(int t, int i, int shift)
+template <int MODE>
+__device__ __forceinline__ int first_column(int threads, int t, int i, int shift)
 {
-    if constexpr (MODE == kVec) return (t + i * TPR) * 8;
-    else if constexpr (MODE == kPairs) return (i * TPR + (t & ~31)) * 8 + 2 * (t & 31) - shift;
-    else return (i * TPR + (t & ~31)) * 8 + (t & 31);
+    if constexpr (MODE == kVec) return (t + i * threads) * 8;
+    else if constexpr (MODE == kPairs) return (i * threads + (t & ~31)) * 8 + 2 * (t & 31) - shift;
+    else return (i * threads + (t & ~31)) * 8 + (t & 31);
 }
 template <int MODE>
 __device__ __forceinline__ int column(int c, int j)  // the j-th of the eight that start at c
@@ -275,7 +275,7 @@ __device__ __forceinline__ float max_abs(float m, float2 v)  // m >= 0
 // Largest of a warp's non-negative floats: their bit patterns are in the same order, and a NaN's is above infinity's.
 __device__ __forceinline__ float warp_max_abs(float v) { return __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v))); }
 
-// Sum and (of non-negative values) maximum over the TPR threads of a row; `red` holds one entry per warp and is not used again before
+// Sum and (of non-negative values) maximum over the threads of a row (TPR at most: a warp, or the block); `red` holds one entry per warp and is not used again before
 // the next barrier.
 template <int TPR, bool MAX = true>
 __device__ __forceinline__ void row_reduce(float& s, float& mx, float2* red)
@@ -285,10 +285,10 @@ __device__ __forceinline__ void row_reduce(float& s, float& mx, float2* red)
     if (MAX) mx = warp_max_abs(mx);
     if constexpr (TPR > 32) {
         constexpr int W = TPR / 32;  // a power of two
-        const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
-        if (l == 0) red[w] = make_float2(s, mx);
+        const int w = threadIdx.x >> 5, l = threadIdx.x & (W - 1);
+        if ((threadIdx.x & 31) == 0) red[w] = make_float2(s, mx);
         __syncthreads();
-        const float2 v = red[l & (W - 1)];
+        const float2 v = l < static_cast<int>(blockDim.x >> 5) ? red[l] : make_float2(0.0f, 0.0f);
         s = v.x;
 #pragma unroll
         for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
@@ -311,7 +311,7 @@ struct NormArgs {
     int q_s8;         // 8-bit output: int8, else e4m3
     int scale_mode;   // ASCB200_SCALE_*
     int group_lanes;  // PER_GROUP / MX: lanes (of eight columns) per group, a power of two up to 32
-    float eps;
+    float eps, inv_k;
 };
 
 // Largest magnitude that a code stands for, in units of the scale.
@@ -395,46 +395,46 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int c, int k, bool s8,
     }
 }
 
-// One row per TPR threads: a warp (blocks of 128 threads hold four rows) or the whole block.  Thread t owns chunks t, t + TPR, ...
-template <typename T, int TPR, int NCHUNK, int MODE>
+// One row per warp (TPR = 32; blocks of 128 threads hold four rows) or per block (of up to TPR threads).  Thread t owns chunks t, t + threads, ...
+template <typename T, int TPR, int NCHUNK, int MODE, bool RES>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 128)
 rms_norm_kernel(const NormArgs p)
 {
     __shared__ float2 red[32];
     grid_dependency_wait();
-    const int t = TPR > 32 ? threadIdx.x : threadIdx.x & 31;
+    const int t = TPR > 32 ? threadIdx.x : threadIdx.x & 31, threads = TPR > 32 ? blockDim.x : 32;
     const long long row = TPR > 32 ? blockIdx.x : blockIdx.x * 4ll + (threadIdx.x >> 5);
     if (row >= p.m) return;  // whole warps; never with a block per row
     const int k = p.k;
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const int shift = row_shift<MODE>(x);
     const PairRange range = pair_range<MODE>(row, p.m, k);
-    const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.ld_residual : nullptr;
-    Raw8<T> xr[NCHUNK], rr[NCHUNK];
+    const T* r = RES ? static_cast<const T*>(p.residual) + row * p.ld_residual : nullptr;
+    Raw8<T> xr[NCHUNK], rr[RES ? NCHUNK : 1];
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, MODE>(t, i, shift);
+        const int c = first_column<MODE>(threads, t, i, shift);
         if (c < k) {
             load_chunk<T, MODE>(x, c, k, range, xr[i]);
-            if (r) load_chunk<T, MODE>(r, c, k, range, rr[i]);
+            if constexpr (RES) load_chunk<T, MODE>(r, c, k, range, rr[i]);
         }
     }
     constexpr bool EARLY = NCHUNK == 1;  // gamma is requested with the row: where few rows leave latency to count
     float2 early[4];
     if constexpr (EARLY) {
-        const int c = first_column<TPR, MODE>(t, 0, shift);
+        const int c = first_column<MODE>(threads, t, 0, shift);
         if (c < k) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, early);
     }
     float2 hg[NCHUNK][4], ss2 = both(0.0f);
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, MODE>(t, i, shift);
+        const int c = first_column<MODE>(threads, t, i, shift);
         if (c < k) {
             float2 g[4];
             finish_chunk<T, MODE>(x, c, k, range, xr[i]);
             unpack8(xr[i], hg[i]);
-            if (r) {
+            if constexpr (RES) {
                 float2 v[4];
                 finish_chunk<T, MODE>(r, c, k, range, rr[i]);
                 unpack8(rr[i], v);
@@ -457,13 +457,13 @@ rms_norm_kernel(const NormArgs p)
     }
     float ss = ss2.x + ss2.y;
     row_reduce<TPR>(ss, amax, red);
-    const float rstd = __frsqrt_rn(__fdiv_rn(ss, static_cast<float>(k)) + p.eps);
+    const float rstd = rsqrtf(fmaf(ss, p.inv_k, p.eps));  // within two units in the last place; correctly rounded division and root took 40 instructions per warp
     if (p.rstd && t == 0) p.rstd[row] = rstd;
     if (p.y) {
         T* y = static_cast<T*>(p.y) + row * p.ldy;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = first_column<TPR, MODE>(t, i, shift);
+            const int c = first_column<MODE>(threads, t, i, shift);
             if (c < k) {
                 float2 v[4];
 #pragma unroll
@@ -475,11 +475,26 @@ rms_norm_kernel(const NormArgs p)
     if (!p.q) return;
     uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.ldq;
     const bool s8 = p.q_s8 != 0;
-    float inv = 0.0f;
     if (p.scale_mode == ASCB200_SCALE_PER_TOKEN) {
-        float scale;
+        float scale, inv;
         scale_of(amax * rstd, s8, scale, inv);
         if (t == 0) static_cast<float*>(p.scale)[row] = scale;
+        // y / scale in one product, unless its factor leaves fp32 (rows of |y| under 1e-30)
+        float once = rstd * inv;
+        if (once > 3.0e38f) {
+            once = inv;
+#pragma unroll
+            for (int i = 0; i < NCHUNK; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) hg[i][j] = mul2(hg[i][j], both(rstd));
+        }
+        const float2 mul[4] = {both(once), both(once), both(once), both(once)};
+#pragma unroll
+        for (int i = 0; i < NCHUNK; ++i) {
+            const int c = first_column<MODE>(threads, t, i, shift);
+            if (c < k) store_codes<MODE>(q, c, k, s8, hg[i], mul);
+        }
+        return;
     }
     const int lanes = p.group_lanes;
     const int group_bits = 31 - __clz(lanes * 8);  // columns per group: a power of two
@@ -498,36 +513,34 @@ rms_norm_kernel(const NormArgs p)
     };
 #pragma unroll
     for (int i = 0; i < NCHUNK; ++i) {
-        const int c = first_column<TPR, MODE>(t, i, shift);
+        const int c = first_column<MODE>(threads, t, i, shift);
         float2 y[4], mul[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = mul2(hg[i][j], both(rstd)), mul[j] = both(inv);
-        if (p.scale_mode != ASCB200_SCALE_PER_TOKEN) {
-            // the whole warp takes part in a group's maximum, columns past the row's end with zeros
-            if constexpr (MODE == kVec) {  // a group is `lanes` neighbouring lanes
-                float g = 0.0f;
+        for (int j = 0; j < 4; ++j) y[j] = mul2(hg[i][j], both(rstd));
+        // the whole warp takes part in a group's maximum, columns past the row's end with zeros
+        if constexpr (MODE == kVec) {  // a group is `lanes` neighbouring lanes
+            float g = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) g = max_abs(g, y[j]);
-                for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-                const float r = scale_group(g, c, (c / 8 & (lanes - 1)) == 0 && c < k);
+            for (int j = 0; j < 4; ++j) g = max_abs(g, y[j]);
+            for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+            const float r = scale_group(g, c, (c / 8 & (lanes - 1)) == 0 && c < k);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mul[j] = both(r);
-            } else if constexpr (MODE == kElements) {  // a group is one, two, four or eight of the warp's 32-column runs
-                float g[8];
+            for (int j = 0; j < 4; ++j) mul[j] = both(r);
+        } else if constexpr (MODE == kElements) {  // a group is one, two, four or eight of the warp's 32-column runs
+            float g[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = warp_max_abs(fabsf(j & 1 ? y[j / 2].y : y[j / 2].x));
+            for (int j = 0; j < 8; ++j) g[j] = warp_max_abs(fabsf(j & 1 ? y[j / 2].y : y[j / 2].x));
 #pragma unroll
-                for (int o = 1; o < 8; o <<= 1) {
-                    if (o * 4 >= lanes) break;
+            for (int o = 1; o < 8; o <<= 1) {
+                if (o * 4 >= lanes) break;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (!(j & o)) g[j] = g[j ^ o] = max_nan(g[j], g[j ^ o]);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = scale_group(g[j], c + j * 32, (t & 31) == 0 && (j * 4 & (lanes - 1)) == 0 && c + j * 32 < k);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mul[j] = make_float2(g[2 * j], g[2 * j + 1]);
+                for (int j = 0; j < 8; ++j)
+                    if (!(j & o)) g[j] = g[j ^ o] = max_nan(g[j], g[j ^ o]);
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] = scale_group(g[j], c + j * 32, (t & 31) == 0 && (j * 4 & (lanes - 1)) == 0 && c + j * 32 < k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mul[j] = make_float2(g[2 * j], g[2 * j + 1]);
         }
         if (c < k) store_codes<MODE>(q, c, k, s8, y, mul);
     }
@@ -535,26 +548,33 @@ rms_norm_kernel(const NormArgs p)
 
 constexpr int kMaxNormK = 32768;
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool RES>
 int launch_norm(const NormArgs& p, int sms, cudaStream_t st)
 {
     const int chunks = (p.k + (MODE == kPairs) + 7) / 8;  // pairs may begin one column early
-#define ASCB200_NORM_WARP(NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, 32, NC, MODE>, static_cast<unsigned>((p.m + 3ll) / 4), 128, 0, st, p))
-#define ASCB200_NORM_BLOCK(TPR, NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, TPR, NC, MODE>, p.m, TPR, 0, st, p))
+#define ASCB200_NORM_WARP(NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, 32, NC, MODE, RES>, static_cast<unsigned>((p.m + 3ll) / 4), 128, 0, st, p))
+#define ASCB200_NORM_BLOCK(TPR, NC) ASCB200_CUDA(launch_pdl(rms_norm_kernel<T, TPR, NC, MODE, RES>, p.m, (chunks + 32 * NC - 1) / (32 * NC) * 32, 0, st, p))
     // While all rows fit the machine at once with one chunk per thread: that, so that a row's loads are all in flight (us, bf16 with residual and e4m3
-    // codes, rows x k: 1 x 4096 2.0, 300 x 1024 2.3 against 3.4 with four chunks per lane, 1200 x 1024 3.3 against 4.8, 300 x 4096 3.3
+    // codes, rows x k: 1 x 4096 1.6, 300 x 1024 2.3 against 3.4 with four chunks per lane, 1200 x 1024 3.3 against 4.8, 300 x 4096 3.3
     // against 4.1).  More rows: two to four chunks per thread, whose reductions cost less per element (600 x 4096 4.3 against 4.8,
-    // 5000 x 4096 24.8 against 30.7, 5000 x 8192 47 against 85).
+    // 5000 x 4096 24.8 against 30.7, 5000 x 8192 47 against 85).  A block has just the threads that its chunks take (9912 x 9216 without residual
+    // 77 -> 55, with 107 -> 99; 9912 x 2100 29 -> 23).
+    // Without a residual there are few bytes per instruction, so more chunks per thread pay: four up to 512 chunks (9912 x 4096 28.4 -> 23.6 us, but
+    // with residual 44.0 -> 44.7, 9912 x 4095 by pairs 51.8 -> 58.7), six per lane of a warp up to 192 (20000 x 1200 23.0 -> 15.8; with
+    // residual 27.2 -> 27.5, by pairs 37.7 -> 57).
+    constexpr bool LIGHT = !RES && MODE == kVec;
     if (chunks > 32 && chunks <= 1024 && static_cast<long long>(p.m) * chunks <= 1536ll * sms) {
         if (chunks <= 128) ASCB200_NORM_BLOCK(128, 1);
         else if (chunks <= 256) ASCB200_NORM_BLOCK(256, 1);
         else if (chunks <= 512) ASCB200_NORM_BLOCK(512, 1);
         else ASCB200_NORM_BLOCK(1024, 1);
-    } else if (chunks <= 32) ASCB200_NORM_WARP(1);
+        return ASCB200_OK;
+    }
+    if (chunks <= 32) ASCB200_NORM_WARP(1);
     else if (chunks <= 64) ASCB200_NORM_WARP(2);
     else if (chunks <= 128) ASCB200_NORM_WARP(4);
-    else if (chunks <= 256) ASCB200_NORM_BLOCK(128, 2);
-    else if (chunks <= 512) ASCB200_NORM_BLOCK(256, 2);
+    else if (LIGHT && chunks <= 192) ASCB200_NORM_WARP((LIGHT ? 6 : 4));
+    else if (!LIGHT && chunks <= 512) ASCB200_NORM_BLOCK(256, (LIGHT ? 4 : 2));
     else if (chunks <= 1024) ASCB200_NORM_BLOCK(256, 4);
     else if (chunks <= 2048) ASCB200_NORM_BLOCK(512, 4);
     else ASCB200_NORM_BLOCK(1024, 4);
@@ -588,13 +608,18 @@ struct PairPlace {
         first = f, step = s;
     }
 };
-template <typename T>
+template <typename T, bool RES>
 int launch_norm_mode(const NormArgs& p, int mode, int sms, cudaStream_t st)
 {
-    if (mode == kVec) return launch_norm<T, kVec>(p, sms, st);
+    if (mode == kVec) return launch_norm<T, kVec, RES>(p, sms, st);
     if constexpr (sizeof(T) == 2)
-        if (mode == kPairs) return launch_norm<T, kPairs>(p, sms, st);
-    return launch_norm<T, kElements>(p, sms, st);
+        if (mode == kPairs) return launch_norm<T, kPairs, RES>(p, sms, st);
+    return launch_norm<T, kElements, RES>(p, sms, st);
+}
+template <typename T>
+int launch_norm_type(const NormArgs& p, int mode, int sms, cudaStream_t st)
+{
+    return p.residual ? launch_norm_mode<T, true>(p, mode, sms, st) : launch_norm_mode<T, false>(p, mode, sms, st);
 }
 
 int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
@@ -647,7 +672,7 @@ int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
     p.x = d.x_dev, p.residual = d.residual_dev, p.gamma = d.gamma_dev, p.sum = d.sum_dev, p.y = d.y_dev, p.q = d.q_dev, p.scale = d.scale_dev;
     p.rstd = d.rstd_dev;
     p.ldx = d.ldx, p.ld_residual = d.ld_residual, p.ld_sum = d.ld_sum, p.ldy = d.ldy, p.ldq = d.ldq;
-    p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32, p.q_s8 = d.q_dtype == ASCB200_S8, p.scale_mode = d.scale_mode, p.eps = d.eps;
+    p.m = d.m, p.k = d.k, p.gamma_f32 = d.gamma_dtype == ASCB200_F32, p.q_s8 = d.q_dtype == ASCB200_S8, p.scale_mode = d.scale_mode, p.eps = d.eps, p.inv_k = 1.0f / static_cast<float>(d.k);
     const bool vec = d.k % 8 == 0 && rows_aligned(d.x_dev, d.ldx, esz, 16) && rows_aligned(d.residual_dev, d.ld_residual, esz, 16) &&
                      rows_aligned(d.sum_dev, d.ld_sum, esz, 16) && rows_aligned(d.y_dev, d.ldy, esz, 16) && rows_aligned(d.q_dev, d.ldq, 1, 8) &&
                      (!d.gamma_dev || aligned_to(d.gamma_dev, 16));
@@ -658,9 +683,9 @@ int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
     const int mode = vec ? kVec : esz == 2 && pairs.same && (!d.q_dev || d.scale_mode == ASCB200_SCALE_PER_TOKEN) ? kPairs : kElements;
     const int sms = st->sm_count;
     switch (d.dtype) {
-        case ASCB200_F16: return launch_norm_mode<__half>(p, mode, sms, stream);
-        case ASCB200_BF16: return launch_norm_mode<__nv_bfloat16>(p, mode, sms, stream);
-        default: return launch_norm_mode<float>(p, mode, sms, stream);
+        case ASCB200_F16: return launch_norm_type<__half>(p, mode, sms, stream);
+        case ASCB200_BF16: return launch_norm_type<__nv_bfloat16>(p, mode, sms, stream);
+        default: return launch_norm_type<float>(p, mode, sms, stream);
     }
 }
 
@@ -781,7 +806,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = both(0.0f);
         if constexpr (KEEP_GAMMA) {
-            const int c = first_column<TPR, MODE>(t, i, shift);
+            const int c = first_column<MODE>(TPR, t, i, shift);
             if (c < k) load_gamma<T, MODE>(p.gamma, p.gamma_f32, c, k, gamma[i]);
         }
     }
@@ -791,7 +816,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
             const uint32_t place = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + stage * STAGE_BYTES;
 #pragma unroll
             for (int i = 0; i < NCHUNK; ++i) {
-                const int c = first_column<TPR, MODE>(t, i, shift);
+                const int c = first_column<MODE>(TPR, t, i, shift);
                 if (c < k) {
                     copy_chunk<T, MODE>(place + i * CHUNK_BYTES, dy + to_come * p.ld_dy, c, k, range, THREADS);
                     copy_chunk<T, MODE>(place + ARRAY_BYTES + i * CHUNK_BYTES, h + to_come * p.ldh, c, k, range, THREADS);
@@ -817,7 +842,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
         const PairRange range = pair_range<MODE>(to_come, p.m, k);
 #pragma unroll
         for (int i = 0; i < RAW; ++i) {
-            const int c = first_column<TPR, MODE>(t, i, shift);
+            const int c = first_column<MODE>(TPR, t, i, shift);
             if (c < k) {
                 load_chunk<T, MODE>(dy + to_come * p.ld_dy, c, k, range, to.dy[i]);
                 load_chunk<T, MODE>(h + to_come * p.ldh, c, k, range, to.h[i]);
@@ -852,7 +877,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
         float2 dot2 = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = first_column<TPR, MODE>(t, i, shift);
+            const int c = first_column<MODE>(TPR, t, i, shift);
             const int held = KEEP ? i : 0, gi = KEEP_GAMMA ? i : 0;
             if (c < k) {
                 float2 a[4];
@@ -874,7 +899,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
         T* dx = static_cast<T*>(p.dx) + row * p.ld_dx;
 #pragma unroll
         for (int i = 0; i < NCHUNK; ++i) {
-            const int c = first_column<TPR, MODE>(t, i, shift);
+            const int c = first_column<MODE>(TPR, t, i, shift);
             const int held = KEEP ? i : 0;
             if (c < k) {
                 float2 e[4];
@@ -911,7 +936,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int col = column<MODE>(first_column<TPR, MODE>(t, i, shift), j);
+                const int col = column<MODE>(first_column<MODE>(TPR, t, i, shift), j);
                 if (in_row(col, k)) put(col, j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
             }
     } else {
@@ -923,7 +948,7 @@ rms_norm_grad_kernel(const NormGradArgs p)
         for (int i = 0; i < NCHUNK; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int col = column<MODE>(first_column<TPR, MODE>(t, i, shift), j);
+                const int col = column<MODE>(first_column<MODE>(TPR, t, i, shift), j);
                 if (in_row(col, k)) warp_acc[sub * W + col] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
             }
         __syncthreads();

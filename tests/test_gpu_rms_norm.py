@@ -204,6 +204,27 @@ def test_extreme_magnitudes():
     assert (out["sum"].t == 65504).all() and (out["y"].t == 1).all()
 
 
+@pytest.mark.parametrize("q", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("k", [64, 1001, 4096])
+def test_codes_of_tiny_rows(k, q):
+    # |y| near 1e-36 from |h| near 1e-2: the codes' factor, rstd / scale, is beyond fp32
+    dev()
+    x, w = torch.randn(3, k, generator=gen(8)) * 0.01, torch.full((k,), 1e-36)
+    _, _, y = reference(x, None, w, 0.0)
+    xs, ws, codes, scale = x.cuda(), w.cuda(), torch.empty(3, k, dtype=q, device="cuda"), torch.empty(3, device="cuda")
+    ab.check(ab.rms_norm(ab.RmsNormDesc(m=3, k=k, dtype=ab.F32, gamma_dtype=ab.F32, x_dev=ptr(xs), gamma_dev=ptr(ws), q_dev=ptr(codes), scale_dev=ptr(scale), q_dtype=CODE[q],
+                                        scale_mode=ab.SCALE_PER_TOKEN), stream()))
+    torch.cuda.synchronize()
+    top = 127 if q == torch.int8 else 448
+    want = y.abs().amax(1) / top
+    kept = want > 2.0**-126
+    # h * gamma near 1e-38 is below the normal numbers: a step is 2^-149, so its half is up to 2^-24 of the largest of a row and more of its smaller values
+    near(scale, torch.where(kept, want, torch.zeros_like(want)), 64 * F * want + 200 * 2.0**-149 / top, "scale")
+    v = torch.where(kept[:, None], y / want[:, None], torch.zeros_like(y))
+    step = 200 * 2.0**-149 / want.clamp(min=2.0**-126)[:, None]  # rstd is near 100
+    near(codes.float(), v, (0.5 if q == torch.int8 else (v.abs() * 2.0**-4).clamp(min=2.0**-10) * (1 + 1e-4)) + v.abs() * 64 * F + step, "codes")
+
+
 def test_in_place():
     dev()
     x, r = torch.randn(37, 1030, generator=gen(6)).bfloat16().cuda(), torch.randn(37, 1030, generator=gen(7)).bfloat16().cuda()
