@@ -34,7 +34,8 @@ def test_layout_matches_the_header(name, tmp_path):
 
 def test_workspace_sizes():
     assert ab.rms_norm_grad_workspace_bytes(0, 64) == 0 and ab.rms_norm_grad_workspace_bytes(-3, 64) == 0 and ab.rms_norm_grad_workspace_bytes(4, -1) == 0
-    assert ab.rms_norm_grad_workspace_bytes(1, 64) == 256 and ab.rms_norm_grad_workspace_bytes(1 << 30, 32768) == 296 * 32768 * 4
+    many = ab.rms_norm_grad_workspace_bytes(1 << 30, 32768)  # whole rows of partial sums, a bounded number of them
+    assert ab.rms_norm_grad_workspace_bytes(1, 64) == 256 and many % (32768 * 4) == 0 and 0 < many <= 1024 * 32768 * 4
     assert ab.route_workspace_bytes(1, 1024) == 0 and ab.route_workspace_bytes(0, 8) == 0 and ab.route_workspace_bytes(2**31 - 1, 1024) > 0
     assert ab.linear_grad_workspace_bytes(0, 8) == 0 and ab.linear_grad_workspace_bytes(100, 9) >= 100 * 16 * 2
     big = ab.linear_grad_workspace_bytes(1 << 20, 1 << 15)   # past 32 bits
