@@ -326,10 +326,13 @@ __device__ __forceinline__ void dequant_store8(DT* out, const float (&v)[8])
 
 // Vector form (n % 8 == 0): eight elements per thread, two vectors per thread in flight; with SHARED (n % 32 == 0, scale
 // constant over 32 aligned columns) one lane in four fetches the scale and shuffles hand it to its neighbours.
+// Vectors of eight elements per thread: int8 sources bring an eighth of a line per vector, so four of them keep as much in flight.
+template <typename SRC>
+constexpr int dequant_vecs_per_thread() { return sizeof(SRC) == 1 ? 4 : 2; }
 template <typename SRC, typename ST, typename DT, bool SHARED>
 __global__ void __launch_bounds__(256) dequant_policy_vec_kernel(const DequantPolicyArgs a)
 {
-    constexpr int VPT = 2;
+    constexpr int VPT = dequant_vecs_per_thread<SRC>();
     const size_t vecs = static_cast<size_t>(a.m) * a.n / 8;
     const SRC* src = static_cast<const SRC*>(a.src);
     DT* dst = static_cast<DT*>(a.dst);
@@ -343,8 +346,13 @@ __global__ void __launch_bounds__(256) dequant_policy_vec_kernel(const DequantPo
         const size_t vi = base + static_cast<size_t>(u) * 256;
         if (vi < vecs) {
             const size_t e = vi * 8;
-            raw[u][0] = __ldg(reinterpret_cast<const uint4*>(src + e));
-            raw[u][1] = __ldg(reinterpret_cast<const uint4*>(src + e) + 1);
+            if constexpr (sizeof(SRC) == 1) {
+                const uint2 bytes = __ldg(reinterpret_cast<const uint2*>(src + e));
+                raw[u][0].x = bytes.x, raw[u][0].y = bytes.y;
+            } else {
+                raw[u][0] = __ldg(reinterpret_cast<const uint4*>(src + e));
+                raw[u][1] = __ldg(reinterpret_cast<const uint4*>(src + e) + 1);
+            }
             row[u] = e < 0xFFFFFFFFull ? static_cast<int>(static_cast<uint32_t>(e) / static_cast<uint32_t>(a.n)) : static_cast<int>(e / a.n);
             col[u] = static_cast<int>(e - static_cast<size_t>(row[u]) * a.n);
             if (!SHARED || (lane & 3) == 0) sc[u] = dequant_scale_at<ST>(a, row[u], col[u]);
@@ -359,7 +367,9 @@ __global__ void __launch_bounds__(256) dequant_policy_vec_kernel(const DequantPo
         const bool per_col = a.per_group && a.k_dim == 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t w = j < 4 ? (&raw[u][0].x)[j] : (&raw[u][1].x)[j - 4];
+            uint32_t w;
+            if constexpr (sizeof(SRC) == 1) w = static_cast<uint32_t>(static_cast<int32_t>(static_cast<int8_t>((j < 4 ? raw[u][0].x : raw[u][0].y) >> (8 * (j & 3)))));
+            else w = j < 4 ? (&raw[u][0].x)[j] : (&raw[u][1].x)[j - 4];
             const float x = std::is_same<SRC, float>::value ? __uint_as_float(w) : __int2float_rn(static_cast<int>(w));
             const float s = (per_col && j > 0) ? dequant_scale_at<ST>(a, row[u], col[u] + j) : sc[u];
             v[j] = __fmul_rn(x, s);
@@ -388,7 +398,8 @@ template <typename SRC, typename ST, typename DT>
 int dequant_policy_launch(const DequantPolicyArgs& a, bool vec, unsigned grid, cudaStream_t s)
 {
     if (vec) {
-        const size_t blocks = (static_cast<size_t>(a.m) * a.n / 8 + 511) / 512;
+        constexpr size_t kPerBlock = 256 * dequant_vecs_per_thread<SRC>();
+        const size_t blocks = (static_cast<size_t>(a.m) * a.n / 8 + kPerBlock - 1) / kPerBlock;
         if (blocks > 0x7FFFFFFFull) return ASCB200_ETOOBIG;
         const bool shared = a.n % 32 == 0 && !(a.per_group && a.k_dim == 0);
         if (shared) dequant_policy_vec_kernel<SRC, ST, DT, true><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
@@ -554,7 +565,7 @@ extern "C" int ascb200_dequant_policy(const void* src, void* dst, int32_t m, int
     if (!src || !dst || !scale || m < 0 || n < 0) return ASCB200_EINVAL;
     if (policy != ASCB200_DEQUANT_PER_TOKEN && policy != ASCB200_DEQUANT_PER_GROUP) return ASCB200_EUNSUPPORTED;
     if (policy == ASCB200_DEQUANT_PER_GROUP && (group_size <= 0 || group_size % 32 != 0 || (k_dim != 0 && k_dim != 1))) return ASCB200_EINVAL;
-    if (src_dtype != ASCB200_S32 && src_dtype != ASCB200_F32) return ASCB200_EUNSUPPORTED;
+    if (src_dtype != ASCB200_S32 && src_dtype != ASCB200_F32 && src_dtype != ASCB200_S8) return ASCB200_EUNSUPPORTED;
     if (!aligned_to(src, 16) || !aligned_to(dst, 4)) return ASCB200_EALIGN;
     if (m == 0 || n == 0) return ASCB200_OK;
     DequantPolicyArgs a;
@@ -571,6 +582,7 @@ extern "C" int ascb200_dequant_policy(const void* src, void* dst, int32_t m, int
     const unsigned grid = static_cast<unsigned>(std::min<size_t>((threads + 255) / 256, static_cast<size_t>(st->sm_count) * 16));
     const bool vec = n % 8 == 0 && aligned_to(dst, 16);  // src is 16-byte aligned (checked above)
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (src_dtype == ASCB200_S8) return dequant_policy_scale<int8_t>(a, scale_dtype, dst_dtype, vec, grid, s);
     if (src_dtype == ASCB200_S32) return dequant_policy_scale<int32_t>(a, scale_dtype, dst_dtype, vec, grid, s);
     return dequant_policy_scale<float>(a, scale_dtype, dst_dtype, vec, grid, s);
 }

@@ -368,7 +368,8 @@ ASCB200_API int ascb200_quant_policy_rm(const void* src_dev, void* dst_dev, int3
 /* AscendDequant with a policy (include/adv_api/quantization/ascend_dequant.h:293-318, AscendDeQuantPolicy / AscendDeQuantParam of
  * include/adv_api/quantization/ascend_dequant_utils.h:32-44): dst[i,j] = cast(float(src[i,j]) * float(scale)), scale per row
  * (PER_TOKEN: [m]) or per group (PER_GROUP: k_dim 1 -> [m, ceil(n / group_size)], k_dim 0 -> [ceil(m / group_size), n]).
- * src S32 / F32; scale F32 / F16 / BF16; dst F32 / F16 / BF16.  The interface's offset tensor is unused by the reference. */
+ * src S32 / F32 / S8 (the codes of ascb200_rms_norm and of AscendQuant, with their fp32 scales); scale F32 / F16 / BF16; dst F32 / F16 / BF16.
+ * The interface's offset tensor is unused by the reference. */
 enum { ASCB200_DEQUANT_PER_TOKEN = 0, ASCB200_DEQUANT_PER_GROUP = 1 };  /* values of AscendDeQuantPolicy */
 ASCB200_API int ascb200_dequant_policy(const void* src_dev, void* dst_dev, int32_t m, int32_t n, int32_t src_dtype, int32_t scale_dtype,
                                        int32_t dst_dtype, int32_t policy, int32_t k_dim, int32_t group_size, const void* scale_dev,

@@ -6,7 +6,7 @@ import torch
 
 import ascb200 as ab
 from test_gpu_linear import act
-from torch_util import dev, ptr, stream
+from torch_util import CODE, HALF_STEP, Out, dev, near, ptr, stream
 
 pytestmark = pytest.mark.gpu
 EPS = 1e-6
@@ -186,3 +186,21 @@ def test_training_step():
     assert rel(out, od) < 0.01 and abs(float(loss) - float(ld)) < 0.01 * float(ld)
     for name, got, leaf in (("x", dx, xd), ("w1", dw1, w1d), ("w2", dw2, w2d), ("router", dwr, wrd), ("gamma", dgamma, gd), ("bias", db1, bd)):
         assert rel(got, leaf.grad) < 11 * 2.0**-8, name
+
+
+@pytest.mark.parametrize("policy,group", [(ab.DEQUANT_PER_TOKEN, 0), (ab.DEQUANT_PER_GROUP, 32), (ab.DEQUANT_PER_GROUP, 64)])
+@pytest.mark.parametrize("dst,scale_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32), (torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("m,n", [(1, 1), (3, 7), (5, 8), (4, 96), (33, 1000), (7, 1001), (300, 4096), (2, 40960)])
+def test_values_of_int8_codes(m, n, dst, scale_dtype, policy, group):
+    """dst = cast(code * scale): one product, one rounding, so within half a step of it and equal for fp32."""
+    dev()
+    g = torch.Generator().manual_seed(m + n)
+    codes = torch.randint(-128, 128, (m, n), generator=g).to(torch.int8)
+    scale = (torch.rand(m, 1 if group == 0 else -(-n // group), generator=g) * 0.1 + 1e-3).to(scale_dtype)
+    cs, ss, out = codes.cuda(), scale.cuda(), Out(m, n, dst)
+    ab.check(ab.dequant_policy(ptr(cs), out.ptr(), m, n, ab.S8, CODE[scale_dtype], CODE[dst], policy, ptr(ss), k_dim=1, group_size=group, stream=stream()))
+    torch.cuda.synchronize()
+    out.check()
+    wide = scale.double().repeat_interleave(group or n, 1)[:, :n]
+    want = codes.double() * wide
+    near(out.t, want, HALF_STEP[dst] * (1 + 2.0**-10) * want.abs() + 2.0**-24 * want.abs(), "values")
