@@ -345,16 +345,11 @@ def _norm_own(s):
             d.q_dev, d.scale_dev, d.q_dtype = _ptr(codes), _ptr(out["scale"]), ab.S8 if q == "int8" else ab.FP8_E4M3
             d.scale_mode = {"fp8 group": ab.SCALE_PER_GROUP, "mx": ab.SCALE_MX}.get(q, ab.SCALE_PER_TOKEN)
             d.group_size = 128 if q == "fp8 group" else 0
-        narrow = torch.empty(m, device="cuda", dtype=out["q"].dtype) if q == "int8" and k % 32 == 0 else None
-        s["plan"] = (d, out, codes, narrow)
-    d, out, codes, narrow = s["plan"]
+        s["plan"] = (d, out, codes)
+    d, out, codes = s["plan"]
     ab.check(ab.rms_norm(d, _stream(x)))
     if c["q"] == "int8":  # the values that the int8 codes stand for
-        if narrow is None:
-            torch.mul(codes, out["scale"][:, None], out=out["q"])
-        else:  # AscendAntiQuant per row, which takes the scales in the output's type
-            narrow.copy_(out["scale"])
-            ab.check(ab.antiquant(_ptr(codes), _ptr(out["q"]), c["m"], c["k"], _dt(ab, out["q"]), 2, scale=_ptr(narrow), stream=_stream(x)))
+        ab.check(ab.dequant_policy(_ptr(codes), _ptr(out["q"]), c["m"], c["k"], ab.S8, ab.F32, _dt(ab, out["q"]), ab.DEQUANT_PER_TOKEN, _ptr(out["scale"]), stream=_stream(x)))
     return out
 
 
