@@ -424,16 +424,17 @@ int launch_act_grad(const ActGradArgs& p, int act, bool vec, dim3 grid, cudaStre
 //         meet in shared memory, of the block and then of the cluster, always in the same order.
 //   dw    tiles of 64 x 256: one instruction per 16 x 8 outputs sums all rows.
 //   dbias 256 columns.
-// Each job makes the dz that it needs itself, rounded to the operands' type like the dz of the other path.
+// Each job makes the dz that it needs itself, as the sum of two numbers of the operands' type: with so few terms in a sum, a single rounding of dz would
+// show beside that of the result (1 x 64 x 64: the error of dw up to twice as large), and the matrix instructions have the time.
 //
 // As in the kernel for a few tokens, the order of the summands and of the columns is free as long as the operands agree.  dx: lane (g, q) reads
 // 16 bytes, columns 8 g .. 8 g + 7, of rows 4 q .. 4 q + 3; the i-th of eight instructions takes the i-th of each lane's columns, two
 // rows packed by one byte permutation.  dw: the columns of an instruction are those that leave a lane with eight neighbours after four.
 //
 // One launch instead of four, of which two are GEMMs of mostly empty tiles (us, bf16 silu with dbias, n x k, 16 rows here against 17 on the GEMMs: 320 x 481
-// 5.2 / 11.1, 1792 x 3864 14.5 / 25.6, 4096 x 4096 23.4 / 30.4, 11008 x 4096 54 / 61, 4096 x 11008 50 / 60; one row of the last two 46 and 47,
-// 3.9 TB/s).  What keeps it from the memory's rate is the latency of a block's loads: dx alone of 1 x 11008 x 4096 runs at 3.6 TB/s, dw
-// alone at 4.6; 128 registers per thread leave room for two blocks per SM.
+// 5.5 / 11.1, 1792 x 3864 15.4 / 25.6, 4096 x 4096 25.0 / 30.4, 11008 x 4096 57 / 61, 4096 x 11008 54 / 60; one row of the last two 51, 3.5 TB/s;
+// the second part of dz takes 5 to 10 % of that).  What keeps it from the memory's rate is the latency of a block's loads: dx alone of
+// 1 x 11008 x 4096 runs at 3.6 TB/s, dw alone at 4.6; 128 registers per thread leave room for two blocks per SM.
 constexpr int kGradRows = 16;
 constexpr int kGradThreads = 256, kGradWarps = 8;
 constexpr int kGradStrip = 64;                         // columns of dx per cluster
@@ -492,12 +493,32 @@ __device__ __forceinline__ RawQuad load_dz(const GradRowsArgs& p, int t, int c)
     }
     return r;
 }
-template <typename T, int ACT>
-__device__ __forceinline__ uint2 dz_of(const RawQuad& r)
+// dz = high + low; the slopes of no activation and of RELU leave dy as it is, or nothing.
+template <int ACT>
+constexpr bool exact_dz() { return ACT == ASCB200_ACT_NONE || ACT == ASCB200_ACT_RELU; }
+template <typename T>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& high, uint32_t& low)
 {
+    high = pack_pair<T>(a, b);
+    const float2 h = unpack_pair<T>(high);
+    // (an infinity or NaN is in `high`; fp16 saturates, and what is beyond stays out of `low` as it does of dz)
+    const float la = a - h.x, lb = b - h.y;
+    low = pack_pair<T>(fabsf(la) <= fabsf(h.x) * 0.00390625f ? la : 0.0f, fabsf(lb) <= fabsf(h.y) * 0.00390625f ? lb : 0.0f);
+}
+template <typename T, int ACT>
+__device__ __forceinline__ uint2 dz_of(const RawQuad& r, uint2& low)
+{
+    low = make_uint2(0u, 0u);
     if constexpr (ACT == ASCB200_ACT_NONE) return r.dy;
     const float2 a = unpack_pair<T>(r.dy.x), b = unpack_pair<T>(r.dy.y), za = unpack_pair<T>(r.z.x), zb = unpack_pair<T>(r.z.y);
-    return make_uint2(pack_pair<T>(a.x * act::slope<ACT>(za.x), a.y * act::slope<ACT>(za.y)), pack_pair<T>(b.x * act::slope<ACT>(zb.x), b.y * act::slope<ACT>(zb.y)));
+    uint2 high;
+    if constexpr (exact_dz<ACT>()) {
+        high = make_uint2(pack_pair<T>(a.x * act::slope<ACT>(za.x), a.y * act::slope<ACT>(za.y)), pack_pair<T>(b.x * act::slope<ACT>(zb.x), b.y * act::slope<ACT>(zb.y)));
+    } else {
+        split_pair<T>(a.x * act::slope<ACT>(za.x), a.y * act::slope<ACT>(za.y), high.x, low.x);
+        split_pair<T>(b.x * act::slope<ACT>(zb.x), b.y * act::slope<ACT>(zb.y), high.y, low.y);
+    }
+    return high;
 }
 __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
@@ -530,13 +551,19 @@ __device__ __forceinline__ void grad_rows_dx(const GradRowsArgs& p, float (*part
         for (int h = 0; h < 2; ++h) to.dz[h] = load_dz<ACT>(p, end > 0 ? g + 8 * h : kGradRows, row);
     };
     auto add = [&](const Piece& from) {
-        const uint2 lo = dz_of<T, ACT>(from.dz[0]), hi = dz_of<T, ACT>(from.dz[1]);
+        uint2 first_low, second_low;  // rows g and g + 8
+        const uint2 first_high = dz_of<T, ACT>(from.dz[0], first_low), second_high = dz_of<T, ACT>(from.dz[1], second_low);
         const uint32_t r0[4] = {from.v[0].x, from.v[0].y, from.v[0].z, from.v[0].w}, r1[4] = {from.v[1].x, from.v[1].y, from.v[1].z, from.v[1].w};
         const uint32_t r2[4] = {from.v[2].x, from.v[2].y, from.v[2].z, from.v[2].w}, r3[4] = {from.v[3].x, from.v[3].y, from.v[3].z, from.v[3].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            mma_16x8<kind_of<T>()>(acc[2 * i], lo.x, hi.x, lo.y, hi.y, low_halves(r0[i], r1[i]), low_halves(r2[i], r3[i]));
-            mma_16x8<kind_of<T>()>(acc[2 * i + 1], lo.x, hi.x, lo.y, hi.y, high_halves(r0[i], r1[i]), high_halves(r2[i], r3[i]));
+            const uint32_t b0 = low_halves(r0[i], r1[i]), b1 = low_halves(r2[i], r3[i]), c0 = high_halves(r0[i], r1[i]), c1 = high_halves(r2[i], r3[i]);
+            mma_16x8<kind_of<T>()>(acc[2 * i], first_high.x, second_high.x, first_high.y, second_high.y, b0, b1);
+            mma_16x8<kind_of<T>()>(acc[2 * i + 1], first_high.x, second_high.x, first_high.y, second_high.y, c0, c1);
+            if constexpr (!exact_dz<ACT>()) {
+                mma_16x8<kind_of<T>()>(acc[2 * i], first_low.x, second_low.x, first_low.y, second_low.y, b0, b1);
+                mma_16x8<kind_of<T>()>(acc[2 * i + 1], first_low.x, second_low.x, first_low.y, second_low.y, c0, c1);
+            }
         }
     };
     Piece even, odd;  // one is worked on while the other is on its way
@@ -595,7 +622,7 @@ __device__ __forceinline__ void grad_rows_dx(const GradRowsArgs& p, float (*part
 constexpr int kALd = kGradTileRows + 8, kBLd = kGradTileCols + 2;  // words; so that a warp's reads fall into different banks
 constexpr int kRunBytes = 256, kRunLd = kRunBytes + 16;            // of a row that a warp writes at once where rows do not start on 16 bytes
 struct DwTile {
-    uint32_t a[kGradRows / 2][kALd];  // rows 2 i and 2 i + 1 of dz, packed
+    uint32_t a[2][kGradRows / 2][kALd];  // rows 2 i and 2 i + 1 of dz, packed: high and low parts
     uint32_t b[kGradRows / 2][kBLd];  // and of x
     alignas(16) uint8_t out[kGradWarps][16][kRunLd];
 };
@@ -669,7 +696,12 @@ __device__ __forceinline__ void grad_rows_dw(const GradRowsArgs& p, DwTile& s)
     for (int tile = first; tile < last; ++tile) {
         const int row0 = tile / across * kGradTileRows, col0 = tile % across * kGradTileCols;
         __syncthreads();  // the tile before has been read
-        if (has_a) put_pairs(&s.a[pair_a][c_a], dz_of<T, ACT>(raw_a[0]), dz_of<T, ACT>(raw_a[1]));
+        if (has_a) {
+            uint2 low[2];
+            const uint2 even = dz_of<T, ACT>(raw_a[0], low[0]), odd = dz_of<T, ACT>(raw_a[1], low[1]);
+            put_pairs(&s.a[0][pair_a][c_a], even, odd);
+            if constexpr (!exact_dz<ACT>()) put_pairs(&s.a[1][pair_a][c_a], low[0], low[1]);
+        }
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
             const int at = threadIdx.x + i * kGradThreads;
@@ -679,7 +711,9 @@ __device__ __forceinline__ void grad_rows_dw(const GradRowsArgs& p, DwTile& s)
         if (tile + 1 < last) fetch(tile + 1);
         const int r = (warp & 3) * 16, half = (warp >> 2) * 128;
         const int run = p.dw_f32 ? 64 : 128;  // columns per run
-        const uint32_t a0 = s.a[q][r + g], a1 = s.a[q][r + g + 8], a2 = s.a[q + 4][r + g], a3 = s.a[q + 4][r + g + 8];
+        uint32_t a[2][4];
+#pragma unroll
+        for (int h = 0; h < (exact_dz<ACT>() ? 1 : 2); ++h) a[h][0] = s.a[h][q][r + g], a[h][1] = s.a[h][q][r + g + 8], a[h][2] = s.a[h][q + 4][r + g], a[h][3] = s.a[h][q + 4][r + g + 8];
 #pragma unroll
         for (int set = 0; set < 4; ++set) {  // 32 columns: the lane gets eight of rows g and g + 8
             uint32_t d[4][4] = {};
@@ -687,7 +721,9 @@ __device__ __forceinline__ void grad_rows_dw(const GradRowsArgs& p, DwTile& s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = c + 8 * (g >> 1) + 2 * i + (g & 1);
-                mma_16x8<kind_of<T>()>(d[i], a0, a1, a2, a3, s.b[q][at], s.b[q + 4][at]);
+                const uint32_t b0 = s.b[q][at], b1 = s.b[q + 4][at];
+                mma_16x8<kind_of<T>()>(d[i], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
+                if constexpr (!exact_dz<ACT>()) mma_16x8<kind_of<T>()>(d[i], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {

@@ -543,7 +543,8 @@ ASCB200_API int ascb200_linear(const ascb200_linear_desc* desc, void* stream);
 
 /* Its gradients, F16 / BF16 (the residual's is dy):
  *   dz = dy * act'(z);  dbias = sum over rows of dz;  dx = dz w;  dw = dz^T x ([n, k], or [k, n] with trans_w = 0).
- * z as the forward call wrote it in the operands' type (not read for ACT_NONE).  dz is rounded to the operands' type for the two products, dbias
+ * z as the forward call wrote it in the operands' type (not read for ACT_NONE).  dz is rounded to the operands' type for the two products (up to
+ * 16 rows with trans_w = 1: split into two numbers of it), dbias
  * is summed in fp32 from the values before.  dx, dw and dbias may each be NULL (not wanted); dw and dbias: the operands' type or F32.
  * The workspace holds dz and the partial sums of dbias; without activation and dbias it is not needed when dy is
  * aligned like x.  The order of the fp32 sums depends on the sizes and the device alone (up to 16 rows with trans_w = 1 are one kernel).

@@ -268,7 +268,9 @@ def backward(m, n, k, dtype, name="silu", trans_w=1, pad=0, dx=True, dw=True, db
     dz = dy * slope
     exact = name in ("none", "relu")
     err32 = torch.zeros_like(dz) if exact else dy.abs() * (2.0**-18 + z.abs() * 2.0**-22) + F * dz.abs()
-    err16 = err32 + (0 if exact else (HALF_STEP[dtype] * (dz.abs() + err32) + TINY[dtype]))
+    # up to 16 rows: two numbers of the type, the second of which holds the first one's rounding and is rounded itself
+    half = HALF_STEP[dtype] ** 2 if m <= 16 and trans_w else HALF_STEP[dtype]
+    err16 = err32 + (0 if exact else (half * (dz.abs() + err32) + 2 * TINY[dtype]))
     if dx:
         gx.check()
         want = dz @ w
