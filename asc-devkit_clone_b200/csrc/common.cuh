@@ -83,10 +83,12 @@ inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 
 }
 // Lets the next kernel of the stream start its launch, then waits until every kernel before this one has completed and its
 // writes are visible.  A no-op pair when the kernel was launched without the attribute.
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_only_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait()
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_dependents_launch();
+    grid_dependency_only_wait();
 }
 #endif
 

@@ -14,6 +14,8 @@ struct FixedResources {
     long long l2_bytes;  // 0: unknown, tiles keep the plain order
 };
 
+constexpr int kFirstOfTwo = 1, kSecondOfTwo = 2;
+
 // What a linear layer adds to the product's output stage: y = act(z) + residual, z = product (scaled, for int8) + bias.
 // Its z, when wanted, is the descriptor's second output.
 struct LinearArgs {
@@ -22,6 +24,7 @@ struct LinearArgs {
     int act;               // ASCB200_ACT_*
     const void* residual;  // [m][ld_residual] of y's type, or nullptr
     long long ld_residual;
+    int order = 0;  // kFirstOfTwo, kSecondOfTwo: this product and the next / the one before do not depend on each other and may overlap
 };
 
 int run_gemm(const ascb200_gemm_desc* d, const int64_t* group_counts, int groups, cudaStream_t stream, const FixedResources* fixed = nullptr,

@@ -17,6 +17,7 @@
 #include <cstdlib>
 
 #include "activation.cuh"
+#include "gemm_host.cuh"
 #include "tc_common.cuh"
 
 namespace ascb200 {
@@ -60,6 +61,7 @@ struct EpiParams {
     long long ld_residual;
     int lin_bias_f32, lin_act;
     int vec_residual;        // rows of the residual are 16-byte aligned at every 32-column boundary
+    int order;               // kFirstOfTwo / kSecondOfTwo: see linear_wait
 };
 
 // Builds of the kernels.  The grouped one has the group tables, the per-group tile search and the swapped blocks, the linear one
@@ -88,6 +90,32 @@ struct GemmParams {
     uint32_t* status;
     EpiParams epi;
 };
+
+// Two products that do not depend on each other may run side by side (linear build).  The first lets the second start only when it has itself
+// waited for everything before it, so the second need not wait at its start; it waits for the first at its end instead, so that whatever
+// follows and waits for the second has waited for both.
+template <int BUILD>
+__device__ __forceinline__ void wait_at_start(const GemmParams& p)
+{
+    if constexpr (BUILD == kBuildLinear) {
+        if (p.epi.order == kFirstOfTwo) {
+            grid_dependency_only_wait();
+            grid_dependents_launch();
+            return;
+        }
+        if (p.epi.order == kSecondOfTwo) {
+            grid_dependents_launch();
+            return;
+        }
+    }
+    grid_dependency_wait();
+}
+template <int BUILD>
+__device__ __forceinline__ void wait_at_end(const GemmParams& p)
+{
+    if constexpr (BUILD == kBuildLinear)
+        if (p.epi.order == kSecondOfTwo) grid_dependency_only_wait();
+}
 
 template <int KIND, int BLOCK_N>
 struct Cfg {
@@ -1325,7 +1353,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     // Launched with programmatic stream serialisation: everything above overlaps the tail of the previous kernel in the
     // stream; from here on global memory is read and written, so that kernel must have completed.
-    grid_dependency_wait();
+    wait_at_start<BUILD>(p);
     if (warp == 0 && p.groups > 0) build_group_tables(p.group_counts, p.groups, num_n, BLOCK_M, row_start, tile_start);
     if (warp == 2) {
         tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
@@ -1491,6 +1519,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         tc_fence_after();
         tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
+    wait_at_end<BUILD>(p);
 }
 
 // ---- the CTA-pair kernel -----------------------------------------------------------------------
@@ -1603,7 +1632,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         tma_prefetch_desc(&tmap_a);
         tma_prefetch_desc(&tmap_b);
     }
-    grid_dependency_wait();  // see gemm_tc_kernel
+    wait_at_start<BUILD>(p);  // see gemm_tc_kernel
     if (warp == 3 && p.groups > 0) build_group_tables(p.group_counts, p.groups, num_n, PAIR_M, row_start, tile_start);
     if (warp == 2) {
         tmem_alloc_pair(smem_u32(tmem_slot), C::TMEM_COLS);
@@ -1824,6 +1853,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
     }
+    wait_at_end<BUILD>(p);
 }
 
 // ---- launches ---------------------------------------------------------------------------------

@@ -402,6 +402,7 @@ int run_gemm(const ascb200_gemm_desc* d, const int64_t* group_counts, int groups
         e.lin_act = linear->act;
         e.residual = linear->residual;
         e.ld_residual = linear->ld_residual;
+        e.order = linear->order;
         e.vec_residual = aligned_to(e.residual, 16) && (e.ld_residual * out_bytes(e.c_dtype)) % 16 == 0;
     }
     p.epi = e;

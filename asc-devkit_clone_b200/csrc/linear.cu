@@ -859,10 +859,16 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
 
     // A product whose rows do not start on 16 bytes is stored by the linear build's output stage, which writes runs of a row through shared
     // memory (gradients of 777 x 1000 x 515 fp16: 39.1 us in all with the plain build's element stores, 21.7 so).
-    const gemm::LinearArgs nothing = {nullptr, 0, ASCB200_ACT_NONE, nullptr, 0};
-    auto product = [&](const ascb200_gemm_desc& q) {
+    // Products of few tiles leave most SMs idle, and each has its latency: then both run side by side (us, all of the gradient, m x n x k: 777 x 1000 x 515
+    // 20.9 -> 14.1, 85 x 128 x 100 10.9 -> 7.6, 420 x 8256 x 755 44.6 -> 38.9, 35 x 5417 x 2742 41.3 -> 37.2; nothing for 2048 x 2048 x 2048, and
+    // 4096 x 4096 x 1024 76 -> 81: there the plain build and the order of two full waves are better).
+    auto tiles = [](long long rows, long long cols) { return (rows + 127) / 128 * ((cols + 127) / 128); };
+    const bool together = d.dx_dev && d.dw_dev && tiles(d.m, d.k) + tiles(w_rows, w_cols) <= 8ll * state->sm_count;
+    gemm::LinearArgs nothing = {nullptr, 0, ASCB200_ACT_NONE, nullptr, 0};
+    auto product = [&](const ascb200_gemm_desc& q, int order) {
         const bool aligned = aligned_to(q.c_dev, 16) && (q.ldc * float_bytes(q.c_dtype)) % 16 == 0;
-        return gemm::run_gemm(&q, nullptr, 0, stream, nullptr, aligned ? nullptr : &nothing);
+        nothing.order = together ? order : 0;
+        return gemm::run_gemm(&q, nullptr, 0, stream, nullptr, aligned && !together ? nullptr : &nothing);
     };
     const bool products = d.dx_dev || d.dw_dev;
     // dy itself is the operand where there is no activation and it can be one
@@ -906,7 +912,7 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
         q.kind = d.kind, q.m = d.m, q.n = d.k, q.k = d.n;
         q.a_dev = dz, q.lda = ld_dz, q.b_dev = d.w_dev, q.ldb = d.ldw, q.trans_b = !d.trans_w;
         q.c_dev = d.dx_dev, q.ldc = d.ld_dx, q.c_dtype = own;
-        const int rc = product(q);
+        const int rc = product(q, gemm::kFirstOfTwo);
         if (rc != ASCB200_OK) return rc;
     }
     if (d.dw_dev) {  // [n, k] = dz^T x, or [k, n] = x^T dz
@@ -915,7 +921,7 @@ int run_linear_grad(const ascb200_linear_grad_desc* desc, cudaStream_t stream)
         q.a_dev = d.trans_w ? dz : d.x_dev, q.lda = d.trans_w ? ld_dz : d.ldx;
         q.b_dev = d.trans_w ? d.x_dev : dz, q.ldb = d.trans_w ? d.ldx : ld_dz;
         q.c_dev = d.dw_dev, q.ldc = d.ld_dw, q.c_dtype = d.dw_dtype;
-        const int rc = product(q);
+        const int rc = product(q, gemm::kSecondOfTwo);
         if (rc != ASCB200_OK) return rc;
     }
     return ASCB200_OK;

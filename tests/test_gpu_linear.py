@@ -446,3 +446,31 @@ def test_captured_and_replayed():
         near(db, dz.sum(0), (dy.abs() * 2.0**-17 + 128 * F * dz.abs()).sum(0), "dbias")
     graph.destroy()
     ab.lib().ascb200_stream_destroy(side)
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_side_by_side_products_in_a_row(act):
+    """Gradients back to back on one stream, each reading what the call before wrote: dx of one is dy of the next, and a workspace is shared."""
+    dev()
+    m, n, k, calls = 200, 136, 136, 12
+    g = gen(5)
+    w = (torch.randn(n, k, generator=g) / math.sqrt(k)).half().cuda()
+    x, z = torch.randn(m, k, generator=g).half().cuda(), torch.randn(m, n, generator=g).half().cuda()
+    d = [torch.randn(m, n, generator=g).half().cuda()] + [torch.empty(m, k, device="cuda", dtype=torch.float16) for _ in range(calls)]
+    dw, db = torch.empty(calls, n, k, device="cuda", dtype=torch.float16), torch.empty(calls, n, device="cuda")
+    room = torch.empty(ab.linear_grad_workspace_bytes(m, n), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(calls):
+        ab.check(ab.linear_grad(ab.LinearGradDesc(kind=ab.KIND_F16, m=m, n=n, k=k, act=ACTS[act], trans_w=1, dy_dev=ptr(d[i]), z_dev=ptr(z), x_dev=ptr(x), w_dev=ptr(w),
+                                                  dx_dev=ptr(d[i + 1]), dw_dev=ptr(dw[i]), dw_dtype=ab.F16, dbias_dev=ptr(db[i]), workspace_dev=ptr(room),
+                                                  workspace_bytes=room.numel()), stream()))
+    torch.cuda.synchronize()
+    for i in range(calls):
+        # each call against its own input as it was written
+        dy = d[i].double()
+        dz, wd, xd = dy * globals()["act"](z.double(), act)[1], w.double(), x.double()
+        err = 0 if act == "none" else dy.abs() * (2.0**-18 + z.double().abs() * 2.0**-22) + 2.0**-11 * 1.01 * dz.abs() + 2.0**-24
+        err = err if torch.is_tensor(err) else torch.zeros_like(dz)
+        near(d[i + 1], dz @ wd, err @ wd.abs() + 2.0**-11 * (dz @ wd).abs() + 100 * F * (dz.abs() @ wd.abs()) + TINY[torch.float16], f"dx {i}")
+        near(dw[i], dz.t() @ xd, err.t() @ xd.abs() + 2.0**-11 * (dz.t() @ xd).abs() + 100 * F * (dz.abs().t() @ xd.abs()) + TINY[torch.float16], f"dw {i}")
+        near(db[i], dz.sum(0), err.sum(0) + 120 * F * dz.abs().sum(0) + 2.0**-149, f"dbias {i}")
