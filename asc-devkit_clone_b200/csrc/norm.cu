@@ -708,7 +708,7 @@ struct NormGradArgs {
 // Blocks that have to fit an SM: 64 registers per thread with one chunk of a 16-bit row, else 128.
 constexpr int grad_blocks_per_sm(int tpr, int nchunk, int bytes)
 {
-    return bytes == 4 ? 1 : tpr == 32 ? 2 : nchunk == 1 ? 1024 / tpr : 512 / tpr;
+    return bytes == 4 ? (nchunk == 2 && tpr > 32 && tpr < 512 ? 512 / tpr : 1) : tpr == 32 ? 2 : nchunk == 1 ? 1024 / tpr : 512 / tpr;
 }
 
 // The rows to come wait in shared memory: every thread copies its own columns of dy, h and dh there (cp.async: no registers, and no barrier, since
@@ -996,6 +996,12 @@ int launch_norm_grad(const NormGradArgs& p, cudaStream_t st, int* blocks)
     const int chunks = (p.k + 7) / 8;
     if (chunks <= 32) return launch_norm_grad_as<T, 32, 1, MODE>(p, st, blocks);
     if (chunks <= 64) return launch_norm_grad_as<T, 32, 2, MODE>(p, st, blocks);
+    if constexpr (MODE == kElements && sizeof(T) == 4) {
+        // Single fp32 elements of many rows: two chunks per thread leave two blocks per SM instead of one (us: 23233 x 2635 228 -> 166, 9107 x 4095 with dh
+        // 128 -> 115, 20000 x 2047 109 -> 95; but 1000 x 1111 6.3 -> 8.5, and 9107 x 4096 by 16 bytes 89 -> 95).
+        if (p.m >= 4096 && chunks > 128 && chunks <= 256) return launch_norm_grad_as<T, 128, 2, MODE>(p, st, blocks);
+        if (p.m >= 4096 && chunks > 256 && chunks <= 512) return launch_norm_grad_as<T, 256, 2, MODE>(p, st, blocks);
+    }
     if constexpr (MODE != kVec || sizeof(T) == 4) {
         if (chunks <= 128) return launch_norm_grad_as<T, 128, 1, MODE>(p, st, blocks);
         if (chunks <= 256) return launch_norm_grad_as<T, 256, 1, MODE>(p, st, blocks);

@@ -301,7 +301,7 @@ def test_gradient_in_pairs(m, k, pad, offset):
 
 @pytest.mark.parametrize("dh,pad,offset", [(True, 0, 0), (False, 8, 8), (True, 0, 1)])
 @pytest.mark.parametrize("dtype", TORCH)
-@pytest.mark.parametrize("m,k", [(20011, 96), (9001, 328), (9001, 519), (5003, 1040), (2500, 2056), (1300, 4104), (900, 8208), (900, 8201), (300, 16400)])
+@pytest.mark.parametrize("m,k", [(20011, 96), (9001, 328), (9001, 519), (5003, 1040), (2500, 2056), (1300, 4104), (900, 8208), (900, 8201), (300, 16400), (4200, 1500), (4200, 3001)])
 def test_gradient_of_many_rows(m, k, dtype, dh, pad, offset):
     backward(m, k, TORCH[dtype], dh=dh, pad=pad, offset=offset)
 
