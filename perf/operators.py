@@ -311,11 +311,6 @@ def _dt(ab, tensor):
     return {torch.float32: ab.F32, torch.float16: ab.F16, torch.bfloat16: ab.BF16, torch.int8: ab.S8}[tensor.dtype]
 
 
-def _stream(tensor):
-    """The handle of the current stream, without an object around it (torch.cuda.current_stream() takes longer than a small kernel)."""
-    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
-
-
 def _ptr(tensor):
     return None if tensor is None else tensor.data_ptr()
 
@@ -347,9 +342,9 @@ def _norm_own(s):
             d.group_size = 128 if q == "fp8 group" else 0
         s["plan"] = (d, out, codes)
     d, out, codes = s["plan"]
-    ab.check(ab.rms_norm(d, _stream(x)))
+    ab.check(ab.rms_norm(d, torch.cuda.current_stream().cuda_stream))
     if c["q"] == "int8":  # the values that the int8 codes stand for
-        ab.check(ab.dequant_policy(_ptr(codes), _ptr(out["q"]), c["m"], c["k"], ab.S8, ab.F32, _dt(ab, out["q"]), ab.DEQUANT_PER_TOKEN, _ptr(out["scale"]), stream=_stream(x)))
+        torch.mul(codes, out["scale"][:, None], out=out["q"])
     return out
 
 
@@ -365,7 +360,7 @@ def _norm_grad_own(s):
                                workspace_bytes=room.numel())
         s["plan"] = (d, out, room)
     d, out, _ = s["plan"]
-    ab.check(ab.rms_norm_grad(d, _stream(h)))
+    ab.check(ab.rms_norm_grad(d, torch.cuda.current_stream().cuda_stream))
     return out
 
 
@@ -390,7 +385,7 @@ def _linear_own(s):
                           ld_residual=_ld(r), y_dev=_ptr(out["y"]), y_dtype=_dt(ab, out["y"]), z_dev=_ptr(out.get("z")))
         s["plan"] = (d, out)
     d, out = s["plan"]
-    ab.check(ab.linear(d, _stream(x)))
+    ab.check(ab.linear(d, torch.cuda.current_stream().cuda_stream))
     return out
 
 
@@ -407,7 +402,7 @@ def _linear_grad_own(s):
                               dw_dtype=_dt(ab, out["dw"]), dbias_dev=_ptr(out.get("dbias")), workspace_dev=_ptr(room), workspace_bytes=room.numel())
         s["plan"] = (d, out, room)
     d, out, _ = s["plan"]
-    ab.check(ab.linear_grad(d, _stream(x)))
+    ab.check(ab.linear_grad(d, torch.cuda.current_stream().cuda_stream))
     return out
 
 
@@ -424,7 +419,7 @@ def _route_own(s):
                          prob_mean_dev=_ptr(out["mean"]), loss_dev=_ptr(out["loss"]), workspace_dev=_ptr(room), workspace_bytes=room.numel())
         s["plan"] = (d, out, room)
     d, out, _ = s["plan"]
-    ab.check(ab.route(d, _stream(x)))
+    ab.check(ab.route(d, torch.cuda.current_stream().cuda_stream))
     return out
 
 
@@ -437,7 +432,7 @@ def _route_grad_own(s):
                              dweights_dev=_ptr(s["dweights"]), dlogits_dev=_ptr(out["dlogits"]))
         s["plan"] = (d, out)
     d, out = s["plan"]
-    ab.check(ab.route_grad(d, _stream(x)))
+    ab.check(ab.route_grad(d, torch.cuda.current_stream().cuda_stream))
     return out
 
 
