@@ -78,9 +78,10 @@ __device__ __forceinline__ int order_key(float x, int e, int low_bits)
     const int b = __float_as_int(__fadd_rn(x, 0.0f));  // -0 as +0
     return ((b ^ ((b >> 31) & 0x7FFFFFFF)) & ~low_bits) | (low_bits - e);
 }
+// The logit of a key, exactly where the logit's low bits are zero: those of a negative one are ones in the order.
 __device__ __forceinline__ float key_value(int key, int low_bits)
 {
-    const int b = key & ~low_bits;
+    const int b = key < 0 ? key | low_bits : key & ~low_bits;
     return __int_as_float(b ^ ((b >> 31) & 0x7FFFFFFF));
 }
 struct Best3 {
@@ -273,7 +274,7 @@ route_kernel(const RouteArgs p)
             Best3 best;
             best.scan(key);
             int top = __reduce_max_sync(kAll, best.v1);
-            float m;  // the largest logit, exactly: a low bit of 1e6 less would make exp(x - m) overflow
+            float m;  // the largest logit, exactly: a few low bits of a value beyond 1e6 less would make exp(x - m) overflow
             if constexpr (sizeof(T) == 2) {
                 m = key_value(top, low_bits);
             } else {

@@ -325,3 +325,27 @@ def test_close_and_large_logits(e):
     _, out = forward(big, torch.float32, min(8, e), 1)
     idx, w, counts, n, _, _, _ = reference(big, None, min(8, e), 1)
     assert torch.equal(out["idx"].t.cpu().long(), idx) and torch.isfinite(out["w"].t).all() and torch.equal(out["counts"].t[0].cpu(), counts)
+
+
+@pytest.mark.parametrize("e", [1, 8, 32, 72, 256, 300, 1000, 1024])
+@pytest.mark.parametrize("dtype", TORCH)
+def test_large_negative_logits(dtype, e):
+    """Rows whose every open logit is far below zero: exp(x - max) is of their differences, which the row's true maximum alone keeps at or below zero."""
+    lowest = float(torch.finfo(TORCH[dtype]).min)
+    levels = (-1.5, -60000.0) if dtype == "f16" else (-1.5, -1e7, -1e9, -1e30, lowest)
+    x = torch.cat([torch.full((4, e), v) for v in levels])
+    steps = 1 - torch.randint(0, 3, x.shape, generator=gen(e)) * 2.0**-7   # of the type; downwards, so that the lowest stays finite
+    x[1::4] *= steps[1::4]
+    x[2::4, e // 2 + 1 :] = -INF
+    x[3::4] = torch.where(torch.arange(e) % 3 == 1, -INF, x[3::4] * steps[3::4])
+    x = x.to(TORCH[dtype])
+    for renorm in (0, 1):
+        k = min(4, e)
+        _, out = forward(x, TORCH[dtype], k, renorm)
+        idx, w, counts, n, mean, loss, _ = reference(x, None, k, renorm)
+        assert torch.equal(out["idx"].t.cpu().long(), idx) and torch.equal(out["counts"].t[0].cpu(), counts) and int(out["n"].t) == n
+        # the levels' logits are equal or so far apart that only the largest count, but for those of -1.5, which differ by at most 1/32
+        rel = (e / 32 + 24) * F
+        near(out["w"].t, w, 2 * rel * w.abs() + 2.0**-126, "weights")
+        near(out["mean"].t[0], mean, (rel + 96 * F) * mean.abs() + 2.0**-126, "means")
+        near(out["loss"].t[0], torch.tensor([loss]), (rel + 160 * F) * abs(loss), "loss")
