@@ -1022,10 +1022,13 @@ __device__ __forceinline__ void linear_tile(const GemmParams& p, const TileInfo&
         st_shared_v4(stage_smem + kEpiChOffset + lane * 16, __float_as_uint(pre.ch.x), __float_as_uint(pre.ch.y), __float_as_uint(pre.ch.z), __float_as_uint(pre.ch.w));
     st_shared_v4(stage_smem + kEpiBiasOffset + lane * 16, __float_as_uint(pre.bias.x), __float_as_uint(pre.bias.y), __float_as_uint(pre.bias.z),
                  __float_as_uint(pre.bias.w));
+    // A tile of 64 rows uses the staging buffer with plain stores (by_runs below), which the bulk store of the tile before, one of 128 rows, may still
+    // be reading.
+    if ((DT == OUT_F16 || DT == OUT_BF16) && e.tma_c && t.m64 && elect_one()) bulk_wait_group_read<0>();
     __syncwarp();
     const int row_base = t.row0 + quad * 32, n_end = min(p.n, t.n_end);
     const bool stage_c = (DT == OUT_F16 || DT == OUT_BF16) && e.tma_c && !t.m64;
-    // rows that do not start on 16 bytes go through the staging buffer where no bulk store of y may still be reading it, else lane by lane
+    // rows that do not start on 16 bytes go through the staging buffer where this tile issues no bulk stores of y from it, else lane by lane
     const bool by_runs = !stage_c;
     const int base_row = t.m64 ? t.row0 + quad * 16 : row_base, rows = max(0, min(t.m64 ? 16 : 32, t.row_end - base_row));
 #pragma unroll 1

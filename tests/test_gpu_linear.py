@@ -474,3 +474,42 @@ def test_side_by_side_products_in_a_row(act):
         near(d[i + 1], dz @ wd, err @ wd.abs() + 2.0**-11 * (dz @ wd).abs() + 100 * F * (dz.abs() @ wd.abs()) + TINY[torch.float16], f"dx {i}")
         near(dw[i], dz.t() @ xd, err.t() @ xd.abs() + 2.0**-11 * (dz.t() @ xd).abs() + 100 * F * (dz.abs().t() @ xd.abs()) + TINY[torch.float16], f"dw {i}")
         near(db[i], dz.sum(0), err.sum(0) + 120 * F * dz.abs().sum(0) + 2.0**-149, f"dbias {i}")
+
+
+@pytest.mark.parametrize("r_pad,z_pad", [(3, None), (0, 1), (None, 5), (7, 3)])
+@pytest.mark.parametrize("m,n,trans_w", [(700, 6272, 0), (513, 7488, 1), (1560, 5504, 1)])
+def test_last_rows_behind_a_full_tile(m, n, trans_w, r_pad, z_pad):
+    """About two tiles per SM, of which the second may be the matrix' last block of at most 64 rows: its residual and z, off 16 bytes, pass
+    through shared memory from which the first tile's y may still be on its way."""
+    dev()
+    for dtype, k in ((torch.bfloat16, 64), (torch.float16, 200), (torch.int8, 64)):
+        if dtype == torch.int8 and z_pad is not None:
+            continue
+        out = torch.bfloat16 if dtype == torch.int8 else dtype
+        x, w, xs, ws = operands(m, n, k, dtype, trans_w, 0)
+        g = gen(m + n)
+        r = None if r_pad is None else torch.randn(m, n, generator=g).to(out)
+        rs = None if r is None else rows_in(r, out, r_pad)
+        y, z = Out(m, n, out), None if z_pad is None else Out(m, n, out, z_pad)
+        d = ab.LinearDesc(kind=KIND[dtype], m=m, n=n, k=k, x_dev=ptr(xs), ldx=xs.stride(0), w_dev=ptr(ws), ldw=ws.stride(0), trans_w=trans_w, y_dev=y.ptr(), ldy=y.ld, y_dtype=CODE[out])
+        if r is not None:
+            d.residual_dev, d.ld_residual = ptr(rs), n + r_pad
+        if z is not None:
+            d.z_dev, d.ldz = z.ptr(), z.ld
+        xd, wd = x.cuda().double(), w.cuda().double()
+        want, mass = xd @ wd.t(), xd.abs() @ wd.abs().t()
+        tol = (k / 16 + 32) * 2 * F * mass
+        if dtype == torch.int8:
+            ch = (torch.rand(n, generator=g) + 0.5).cuda() * 0.001
+            d.ch_scale_dev = ptr(ch)
+            want = want * ch.double()
+            tol = 4 * F * want.abs()
+        ab.check(ab.linear(d, stream()))
+        torch.cuda.synchronize()
+        y.check()
+        if z is not None:
+            z.check()
+            near(z.t, want, tol + (HALF_STEP[out] + 4 * F) * want.abs() + TINY[out], "z")
+        if r is not None:
+            want = want + r.cuda().double()
+        near(y.t, want, tol + (HALF_STEP[out] + 4 * F) * want.abs() + TINY[out], "y")
