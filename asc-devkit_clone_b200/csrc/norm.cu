@@ -740,6 +740,12 @@ __device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.comm
 template <int N>
 __device__ __forceinline__ void copies_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// kPairs: the element whose address a copy of the pair at `col` is given.  A copy that brings nothing is not to leave the row far behind, but needs an
+// address on four bytes all the same: pairs start there, so any element of the pair's parity has one, the row itself only where its pairs begin with it.
+constexpr int pair_source(int col, bool inside) { return inside ? col : col & 1; }
+static_assert(pair_source(-1, false) == 1 && pair_source(63, false) == 1 && pair_source(64, false) == 0 && pair_source(63, true) == 63 && pair_source(-1, true) == -1,
+              "a whole number of pairs from the pair's own place");
+
 // One chunk to or from its place: words of 16 bytes (kVec) or four (kPairs), those of the block's threads side by side.
 template <typename T, int MODE>
 __device__ __forceinline__ void copy_chunk(uint32_t place, const T* row, int c, int k, const PairRange& range, int threads)
@@ -753,7 +759,7 @@ __device__ __forceinline__ void copy_chunk(uint32_t place, const T* row, int c, 
         for (int j = 0; j < WORDS; ++j) {
             const int col = c + 64 * j;
             const bool inside = range.last >= range.first && static_cast<unsigned>(col - range.first) <= static_cast<unsigned>(range.last - range.first);
-            copy_async<4>(place + (j * threads + threadIdx.x) * 4, inside ? row + col : row, inside);
+            copy_async<4>(place + (j * threads + threadIdx.x) * 4, row + pair_source(col, inside), inside);
         }
     }
 }

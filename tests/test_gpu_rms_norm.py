@@ -463,3 +463,11 @@ def test_same_inputs_give_the_same_bits():
         torch.cuda.synchronize()
         first = first or (dx, dg)
         assert torch.equal(dx, first[0]) and torch.equal(dg, first[1])
+
+
+@pytest.mark.parametrize("pad,offset", [(0, 0), (0, 1), (1, 0), (1, 1), (2, 1)])
+@pytest.mark.parametrize("m,k", [(1, 8193), (2, 8197), (400, 8201), (301, 12289), (299, 16381)])
+def test_gradient_of_long_rows_in_pairs(m, k, pad, offset):
+    """Rows of either parity through the ring in shared memory, with threads whose pairs lie behind the row's end."""
+    backward(m, k, torch.bfloat16, pad=pad, offset=offset)
+    backward(m, k, torch.float16, dh=False, gamma="f32", pad=pad, offset=offset)
