@@ -679,8 +679,8 @@ int run_rms_norm(const ascb200_rms_norm_desc* desc, cudaStream_t stream)
     PairPlace pairs;
     pairs.add(d.x_dev, d.ldx, esz), pairs.add(d.residual_dev, d.ld_residual, esz), pairs.add(d.sum_dev, d.ld_sum, esz), pairs.add(d.y_dev, d.ldy, esz);
     pairs.add(d.q_dev, d.ldq, 1);
-    // (groups of columns end inside pairs that begin one column early)
-    const int mode = vec ? kVec : esz == 2 && pairs.same && (!d.q_dev || d.scale_mode == ASCB200_SCALE_PER_TOKEN) ? kPairs : kElements;
+    // (groups of columns end inside pairs that begin one column early; and the longest rows would take a column more than a block has threads for)
+    const int mode = vec ? kVec : esz == 2 && pairs.same && d.k < kMaxNormK && (!d.q_dev || d.scale_mode == ASCB200_SCALE_PER_TOKEN) ? kPairs : kElements;
     const int sms = st->sm_count;
     switch (d.dtype) {
         case ASCB200_F16: return launch_norm_type<__half>(p, mode, sms, stream);

@@ -471,3 +471,17 @@ def test_gradient_of_long_rows_in_pairs(m, k, pad, offset):
     """Rows of either parity through the ring in shared memory, with threads whose pairs lie behind the row's end."""
     backward(m, k, torch.bfloat16, pad=pad, offset=offset)
     backward(m, k, torch.float16, dh=False, gamma="f32", pad=pad, offset=offset)
+
+
+@pytest.mark.parametrize("residual", [True, False])
+@pytest.mark.parametrize("pad,offset", [(1, 0), (0, 1), (1, 1), (2, 1), (8, 0), (3, 5)])
+@pytest.mark.parametrize("k", [32760, 32761, 32766, 32768])
+def test_the_longest_rows_at_every_place(k, pad, offset, residual):
+    for dtype in (torch.bfloat16, torch.float16):
+        x, r, w, out = forward(3, k, dtype, residual=residual, pad=pad, offset=offset, gamma="f32")
+        check_floats(x, r, w, out, dtype)
+        x, r, w, out = forward(2, k, dtype, residual=residual, pad=pad, offset=offset, q=torch.int8, y=False)
+        h, _, y = reference(x, r, w)
+        near(out["sum"].t, h, (HALF_STEP[dtype] + F) * h.abs() + TINY[dtype], "sum")
+        check_codes(y, out, torch.int8, ab.SCALE_PER_TOKEN, 0)
+        backward(3, k, dtype, pad=pad, offset=offset, dh=residual)
