@@ -25,9 +25,15 @@ __device__ __forceinline__ float sigmoid(float x) { return rcp_fast(1.0f + exp2_
 // GELU's tanh form is z * sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3).  Beyond |z| = 32 the sigmoid is 0 or 1 to the last bit;
 // the clamp keeps z^3 and z^2 finite.
 constexpr float kTanh2u = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+__device__ __forceinline__ float clamp_nan(float z, float top)  // a NaN stays
+{
+    float r;
+    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, %2;\n\tmin.NaN.f32 %0, t, %3;\n\t}" : "=f"(r) : "f"(z), "f"(-top), "f"(top));
+    return r;
+}
 __device__ __forceinline__ float tanh_arg(float z)
 {
-    const float c = fminf(fmaxf(z, -32.0f), 32.0f);
+    const float c = clamp_nan(z, 32.0f);
     return kTanh2u * c * fmaf(0.044715f * c, c, 1.0f);
 }
 
@@ -74,8 +80,8 @@ __device__ __forceinline__ float slope(float z)
         const float tail = normal_tail(z, e);
         return fmaf(z * 0.3989422804014327f, e, z > 0.0f ? 1.0f - tail : tail);
     } else if constexpr (ACT == ASCB200_ACT_GELU_TANH) {
-        const float c = fminf(fmaxf(z, -32.0f), 32.0f);
-        const float g = sigmoid(tanh_arg(z));
+        const float c = clamp_nan(z, 32.0f);
+        const float g = sigmoid(tanh_arg(c));
         return g * fmaf(kTanh2u * c * fmaf(0.134145f * c, c, 1.0f), 1.0f - g, 1.0f);
     } else if constexpr (ACT == ASCB200_ACT_SILU) {
         const float g = sigmoid(z);

@@ -513,3 +513,22 @@ def test_last_rows_behind_a_full_tile(m, n, trans_w, r_pad, z_pad):
         if r is not None:
             want = want + r.cuda().double()
         near(y.t, want, tol + (HALF_STEP[out] + 4 * F) * want.abs() + TINY[out], "y")
+
+
+@pytest.mark.parametrize("name", [a for a in ACTS if a not in ("none", "relu")])  # (the slopes of these are 1, and 1 or 0 by a comparison)
+@pytest.mark.parametrize("m", [1, 5, 60])
+def test_the_slope_of_nan_is_nan(m, name):
+    dev()
+    n, k = 24, 16
+    z, dy = torch.randn(m, n, generator=gen(m)), torch.randn(m, n, generator=gen(m + 1))
+    z[m // 2, 7] = math.nan
+    x, w = torch.randn(m, k, generator=gen(m + 2)), torch.randn(n, k, generator=gen(m + 3))
+    x, w, dy, z = (t.bfloat16().cuda() for t in (x, w, dy, z))
+    dx, dw, db = torch.empty(m, k, device="cuda"), torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+    dx = dx.bfloat16()
+    room = torch.empty(ab.linear_grad_workspace_bytes(m, n), dtype=torch.uint8, device="cuda")
+    ab.check(ab.linear_grad(ab.LinearGradDesc(kind=ab.KIND_BF16, m=m, n=n, k=k, act=ACTS[name], trans_w=1, dy_dev=ptr(dy), z_dev=ptr(z), x_dev=ptr(x), w_dev=ptr(w), dx_dev=ptr(dx),
+                                              dw_dev=ptr(dw), dw_dtype=ab.F32, dbias_dev=ptr(db), dbias_dtype=ab.F32, workspace_dev=ptr(room), workspace_bytes=room.numel()), stream()))
+    torch.cuda.synchronize()
+    rows, cols = torch.arange(m) == m // 2, torch.arange(n) == 7
+    assert torch.equal(torch.isnan(dx).cpu(), rows[:, None].expand(m, k)) and torch.equal(torch.isnan(dw).cpu(), cols[:, None].expand(n, k)) and torch.equal(torch.isnan(db).cpu(), cols)
