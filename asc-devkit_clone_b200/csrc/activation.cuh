@@ -37,18 +37,24 @@ __device__ __forceinline__ float tanh_arg(float z)
     return kTanh2u * c * fmaf(0.044715f * c, c, 1.0f);
 }
 
-// Upper tail of the normal distribution at |z|, and e^(-z^2 / 2): erfc by the rational approximation 7.1.26 of Abramowitz and Stegun
-// (absolute error of erf up to 1.5e-7).  Working with the tail keeps small results of negative z free of cancellation.
+// Upper tail of the normal distribution at |z|, and e = e^(-z^2 / 2).  The tail is e * R with a smooth R, which is t P(t) in t = 1 / (1 + 0.21 |z|): P of degree
+// eight, fitted to R / t for |z| up to 14 with the smallest relative error (1.6e-8).  A tail that is right relative to itself keeps GELU so where z is
+// negative: within 6e-7 of itself to |z| = 3, 2e-6 to 6, 8e-6 to 13 (z^2 times its rounding in the exponent); an approximation of
+// erf with an absolute error of 1.5e-7 was off by 5e-4 at -4 and 1e-2 at -8 (its four steps less took 100.4 us instead of 102.1 in the layer of 4096 x
+// 11008 x 1024 bf16 with z).  Beyond 13.2 e is below the normal numbers and taken as 0.
 __device__ __forceinline__ float normal_tail(float z, float& e)
 {
-    const float x = fabsf(z) * 0.7071067811865476f;
-    const float t = rcp_fast(fmaf(0.3275911f, x, 1.0f));
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    e = exp2_fast(-kLog2e * x * x);
-    return 0.5f * p * t * e;
+    const float t = rcp_fast(fmaf(0.21f, fabsf(z), 1.0f));
+    float p = fmaf(-0.07165637f, t, 0.28358883f);
+    p = fmaf(p, t, -0.33025384f);
+    p = fmaf(p, t, 0.3494015f);
+    p = fmaf(p, t, -0.09392552f);
+    p = fmaf(p, t, 0.12487286f);
+    p = fmaf(p, t, 0.069192134f);
+    p = fmaf(p, t, 0.08506887f);
+    p = fmaf(p, t, 0.08371157f);
+    e = exp2_fast(-0.5f * kLog2e * (z * z));
+    return p * t * e;
 }
 
 template <int ACT>

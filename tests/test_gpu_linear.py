@@ -532,3 +532,49 @@ def test_the_slope_of_nan_is_nan(m, name):
     torch.cuda.synchronize()
     rows, cols = torch.arange(m) == m // 2, torch.arange(n) == 7
     assert torch.equal(torch.isnan(dx).cpu(), rows[:, None].expand(m, k)) and torch.equal(torch.isnan(dw).cpu(), cols[:, None].expand(n, k)) and torch.equal(torch.isnan(db).cpu(), cols)
+
+
+def normal(z):
+    """(upper tail at |z|, density at z) in 64 bits."""
+    return 0.5 * torch.erfc(z.abs() / math.sqrt(2)), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+
+
+# Relative errors of the tail: the exponent's rounding, up to 2.5 * 2^-24 of z^2 / 2 and so 1.25 z^2 2^-24; ex2 2^-22, the fit 1.7e-8, rcp and the polynomial's nine steps, whose
+# terms add up to at most three times the result, together under 2^-20; below the normal numbers (from |z| = 13 on) a tail is 0.
+def tail_error(z):
+    return 2.0**-20 + z * z * 2.0**-23
+
+
+@pytest.mark.parametrize("m", [2, 300])
+def test_gelu_of_far_negative_values(m):
+    """GELU is right relative to itself, not to z: its fp32 output shows it."""
+    dev()
+    z = torch.cat([torch.linspace(-13, 13, 417), torch.tensor([-1e-3, 1e-3, -1e-30, 0.0, -14.0, -40.0, 14.0, 40.0])])
+    n = len(z)
+    x, w = torch.zeros(m, 16, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, 16, dtype=torch.bfloat16, device="cuda")
+    bias, y = z.cuda(), torch.empty(m, n, device="cuda")
+    ab.check(ab.linear(ab.LinearDesc(kind=ab.KIND_BF16, m=m, n=n, k=16, x_dev=ptr(x), w_dev=ptr(w), trans_w=1, act=ab.ACT_GELU, bias_dev=ptr(bias), bias_dtype=ab.F32, y_dev=ptr(y),
+                                     y_dtype=ab.F32), stream()))
+    torch.cuda.synchronize()
+    z = z.double()
+    tail, _ = normal(z)
+    want = torch.where(z > 0, z - z * tail, z * tail)
+    tol = (z * tail).abs() * (tail_error(z) + F) + F * want.abs() + 2.0**-122
+    near(y, want.expand(m, n), tol.expand(m, n), "y")
+
+
+@pytest.mark.parametrize("m", [1, 40])
+def test_gelu_slope_of_far_negative_values(m):
+    dev()
+    z = torch.linspace(-13, 13, 417).half()
+    n = len(z)
+    zs, dy, db = torch.zeros(m, n, dtype=torch.float16, device="cuda"), torch.zeros(m, n, dtype=torch.float16, device="cuda"), torch.empty(n, device="cuda")
+    zs[0], dy[0] = z.cuda(), 1.0
+    room = torch.empty(ab.linear_grad_workspace_bytes(m, n), dtype=torch.uint8, device="cuda")
+    ab.check(ab.linear_grad(ab.LinearGradDesc(kind=ab.KIND_F16, m=m, n=n, k=16, act=ab.ACT_GELU, trans_w=1, dy_dev=ptr(dy), z_dev=ptr(zs), dbias_dev=ptr(db), dbias_dtype=ab.F32,
+                                              workspace_dev=ptr(room), workspace_bytes=room.numel()), stream()))
+    torch.cuda.synchronize()
+    z = z.double()
+    tail, phi = normal(z)
+    want = torch.where(z > 0, 1 - tail, tail) + z * phi
+    near(db, want, (tail + (z * phi).abs()) * (tail_error(z) + 3 * F) + 2 * F * want.abs() + 2.0**-120, "slope")
