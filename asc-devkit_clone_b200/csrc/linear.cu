@@ -520,6 +520,17 @@ __device__ __forceinline__ uint2 dz_of(const RawQuad& r, uint2& low)
     }
     return high;
 }
+// An infinity in the other operand meets the high part alone: times a low part of the other sign, or of zero, it would make the sum NaN.  `not_finite` is not zero where
+// a 16-bit number of the words has all bits of its exponent set (those then carry into the sign's place); `finite_only` takes these numbers out.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w)
+{
+    constexpr uint32_t EXPONENT = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u, LOWEST = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+    return ((w & EXPONENT) + LOWEST) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) { return w & ~((not_finite<T>(w) >> 15) * 0xFFFFu); }
+
 __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
 template <typename T>
@@ -534,7 +545,7 @@ __device__ __forceinline__ void grad_rows_dx(const GradRowsArgs& p, float (*part
     const int first = rank * per, last = min(chunks, first + per);
     const uint8_t* w = static_cast<const uint8_t*>(p.w);
     const long long ldw = p.ldw * 2;
-    uint32_t acc[8][4] = {};
+    uint32_t acc[8][4];
     struct Piece {  // 16 rows x 64 columns of w, with the dz that meets them
         uint4 v[4];
         RawQuad dz[2];
@@ -550,45 +561,62 @@ __device__ __forceinline__ void grad_rows_dx(const GradRowsArgs& p, float (*part
 #pragma unroll
         for (int h = 0; h < 2; ++h) to.dz[h] = load_dz<ACT>(p, end > 0 ? g + 8 * h : kGradRows, row);
     };
-    auto add = [&](const Piece& from) {
+    // clean: the low parts meet finite weights alone
+    auto add = [&](const Piece& from, auto clean) {
         uint2 first_low, second_low;  // rows g and g + 8
         const uint2 first_high = dz_of<T, ACT>(from.dz[0], first_low), second_high = dz_of<T, ACT>(from.dz[1], second_low);
         const uint32_t r0[4] = {from.v[0].x, from.v[0].y, from.v[0].z, from.v[0].w}, r1[4] = {from.v[1].x, from.v[1].y, from.v[1].z, from.v[1].w};
         const uint32_t r2[4] = {from.v[2].x, from.v[2].y, from.v[2].z, from.v[2].w}, r3[4] = {from.v[3].x, from.v[3].y, from.v[3].z, from.v[3].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t b0 = low_halves(r0[i], r1[i]), b1 = low_halves(r2[i], r3[i]), c0 = high_halves(r0[i], r1[i]), c1 = high_halves(r2[i], r3[i]);
+            uint32_t b0 = low_halves(r0[i], r1[i]), b1 = low_halves(r2[i], r3[i]), c0 = high_halves(r0[i], r1[i]), c1 = high_halves(r2[i], r3[i]);
             mma_16x8<kind_of<T>()>(acc[2 * i], first_high.x, second_high.x, first_high.y, second_high.y, b0, b1);
             mma_16x8<kind_of<T>()>(acc[2 * i + 1], first_high.x, second_high.x, first_high.y, second_high.y, c0, c1);
             if constexpr (!exact_dz<ACT>()) {
+                if constexpr (clean.value) b0 = finite_only<T>(b0), b1 = finite_only<T>(b1), c0 = finite_only<T>(c0), c1 = finite_only<T>(c1);
                 mma_16x8<kind_of<T>()>(acc[2 * i], first_low.x, second_low.x, first_low.y, second_low.y, b0, b1);
                 mma_16x8<kind_of<T>()>(acc[2 * i + 1], first_low.x, second_low.x, first_low.y, second_low.y, c0, c1);
             }
         }
     };
-    Piece even, odd;  // one is worked on while the other is on its way
-    load(first + warp, even);
-    for (int ch = first + warp; ch < last; ch += 2 * kGradWarps) {
-        load(ch + kGradWarps, odd);
-        add(even);
-        if (ch + kGradWarps >= last) break;
-        load(ch + 2 * kGradWarps, even);
-        add(odd);
-    }
-    // place i * 8 + s holds column 8 s + i
+    // Returns whether one of the thread's sums is not finite.
+    auto strip = [&](auto clean) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<float2*>(&part[warp][g + 8 * h][i * 8 + 2 * q]) = make_float2(__uint_as_float(acc[i][2 * h]), __uint_as_float(acc[i][2 * h + 1]));
-    __syncthreads();
-    for (int i = threadIdx.x; i < kGradRows * kGradStrip; i += kGradThreads) {
-        float* at = &part[0][i / kGradStrip][i % kGradStrip];
-        float s = at[0];
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0u;
+        Piece even, odd;  // one is worked on while the other is on its way
+        load(first + warp, even);
+        for (int ch = first + warp; ch < last; ch += 2 * kGradWarps) {
+            load(ch + kGradWarps, odd);
+            add(even, clean);
+            if (ch + kGradWarps >= last) break;
+            load(ch + 2 * kGradWarps, even);
+            add(odd, clean);
+        }
+        // place i * 8 + s holds column 8 s + i
 #pragma unroll
-        for (int v = 1; v < kGradWarps; ++v) s += at[v * kGradRows * kPartLd];
-        at[0] = s;
-    }
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float2*>(&part[warp][g + 8 * h][i * 8 + 2 * q]) = make_float2(__uint_as_float(acc[i][2 * h]), __uint_as_float(acc[i][2 * h + 1]));
+        __syncthreads();
+        bool bad = false;
+        for (int i = threadIdx.x; i < kGradRows * kGradStrip; i += kGradThreads) {
+            float* at = &part[0][i / kGradStrip][i % kGradStrip];
+            float s = at[0];
+#pragma unroll
+            for (int v = 1; v < kGradWarps; ++v) s += at[v * kGradRows * kPartLd];
+            at[0] = s;
+            bad |= !(fabsf(s) < __builtin_huge_valf());
+        }
+        return bad;
+    };
+    // A sum that is not finite: an infinite weight may have met a low part.  The strip is then made once more, with the low parts meeting finite weights alone.
+    // (Looking for infinities in every piece took up to 2 % of the whole.)
+    const bool bad = strip(std::false_type());
+    if constexpr (!exact_dz<ACT>())
+        if (__syncthreads_or(bad)) strip(std::true_type());
     if (p.splits > 1) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -702,56 +730,68 @@ __device__ __forceinline__ void grad_rows_dw(const GradRowsArgs& p, DwTile& s)
             put_pairs(&s.a[0][pair_a][c_a], even, odd);
             if constexpr (!exact_dz<ACT>()) put_pairs(&s.a[1][pair_a][c_a], low[0], low[1]);
         }
+        uint32_t any = 0u;
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
             const int at = threadIdx.x + i * kGradThreads;
             put_pairs(&s.b[at / kQuadsB][at % kQuadsB * 4], raw_b[i][0], raw_b[i][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) any |= not_finite<T>(raw_b[i][h].x) | not_finite<T>(raw_b[i][h].y);
         }
-        __syncthreads();
+        bool infinities = false;
+        if constexpr (exact_dz<ACT>()) __syncthreads();
+        else infinities = __syncthreads_or(any != 0u);
         if (tile + 1 < last) fetch(tile + 1);
         const int r = (warp & 3) * 16, half = (warp >> 2) * 128;
         const int run = p.dw_f32 ? 64 : 128;  // columns per run
         uint32_t a[2][4];
 #pragma unroll
         for (int h = 0; h < (exact_dz<ACT>() ? 1 : 2); ++h) a[h][0] = s.a[h][q][r + g], a[h][1] = s.a[h][q][r + g + 8], a[h][2] = s.a[h][q + 4][r + g], a[h][3] = s.a[h][q + 4][r + g + 8];
+        auto sets = [&](auto clean) {  // clean: the low parts meet finite numbers of x alone
 #pragma unroll
-        for (int set = 0; set < 4; ++set) {  // 32 columns: the lane gets eight of rows g and g + 8
-            uint32_t d[4][4] = {};
-            const int c = half + set * 32;
+            for (int set = 0; set < 4; ++set) {  // 32 columns: the lane gets eight of rows g and g + 8
+                uint32_t d[4][4] = {};
+                const int c = half + set * 32;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = c + 8 * (g >> 1) + 2 * i + (g & 1);
-                const uint32_t b0 = s.b[q][at], b1 = s.b[q + 4][at];
-                mma_16x8<kind_of<T>()>(d[i], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
-                if constexpr (!exact_dz<ACT>()) mma_16x8<kind_of<T>()>(d[i], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
-            }
+                for (int i = 0; i < 4; ++i) {
+                    const int at = c + 8 * (g >> 1) + 2 * i + (g & 1);
+                    uint32_t b0 = s.b[q][at], b1 = s.b[q + 4][at];
+                    mma_16x8<kind_of<T>()>(d[i], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
+                    if constexpr (!exact_dz<ACT>()) {
+                        if constexpr (clean.value) b0 = finite_only<T>(b0), b1 = finite_only<T>(b1);
+                        mma_16x8<kind_of<T>()>(d[i], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
+                    }
+                }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = row0 + r + g + 8 * h, col = col0 + c + 8 * q;
-                uint8_t* staged = s.out[warp][g + 8 * h];
-                if (p.dw_f32) {
-                    const uint4 v0 = make_uint4(d[0][2 * h], d[0][2 * h + 1], d[1][2 * h], d[1][2 * h + 1]), v1 = make_uint4(d[2][2 * h], d[2][2 * h + 1], d[3][2 * h], d[3][2 * h + 1]);
-                    uint4* out = p.dw_vec ? reinterpret_cast<uint4*>(static_cast<float*>(p.dw) + row * p.ld_dw + col) : reinterpret_cast<uint4*>(staged + ((set & 1) * 32 + 8 * q) * 4);
-                    if (!p.dw_vec || (row < p.n && col < p.k)) out[0] = v0, out[1] = v1;
-                } else {
-                    uint32_t v[4];
+                for (int h = 0; h < 2; ++h) {
+                    const int row = row0 + r + g + 8 * h, col = col0 + c + 8 * q;
+                    uint8_t* staged = s.out[warp][g + 8 * h];
+                    if (p.dw_f32) {
+                        const uint4 v0 = make_uint4(d[0][2 * h], d[0][2 * h + 1], d[1][2 * h], d[1][2 * h + 1]), v1 = make_uint4(d[2][2 * h], d[2][2 * h + 1], d[3][2 * h], d[3][2 * h + 1]);
+                        uint4* out = p.dw_vec ? reinterpret_cast<uint4*>(static_cast<float*>(p.dw) + row * p.ld_dw + col) : reinterpret_cast<uint4*>(staged + ((set & 1) * 32 + 8 * q) * 4);
+                        if (!p.dw_vec || (row < p.n && col < p.k)) out[0] = v0, out[1] = v1;
+                    } else {
+                        uint32_t v[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = pack_pair<T>(__uint_as_float(d[i][2 * h]), __uint_as_float(d[i][2 * h + 1]));
-                    uint4* out = p.dw_vec ? reinterpret_cast<uint4*>(static_cast<T*>(p.dw) + row * p.ld_dw + col) : reinterpret_cast<uint4*>(staged + (set * 32 + 8 * q) * 2);
-                    if (!p.dw_vec || (row < p.n && col < p.k)) *out = make_uint4(v[0], v[1], v[2], v[3]);
+                        for (int i = 0; i < 4; ++i) v[i] = pack_pair<T>(__uint_as_float(d[i][2 * h]), __uint_as_float(d[i][2 * h + 1]));
+                        uint4* out = p.dw_vec ? reinterpret_cast<uint4*>(static_cast<T*>(p.dw) + row * p.ld_dw + col) : reinterpret_cast<uint4*>(staged + (set * 32 + 8 * q) * 2);
+                        if (!p.dw_vec || (row < p.n && col < p.k)) *out = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                }
+                if (!p.dw_vec && (set == 3 || (p.dw_f32 && set == 1))) {  // a run of 256 bytes per row is together
+                    __syncwarp();
+                    const int col = col0 + half + (p.dw_f32 ? (set >> 1) * 64 : 0), count = min(run, p.k - col), rows = min(16, p.n - row0 - r);
+                    const long long at = static_cast<long long>(row0 + r) * p.ld_dw + col;
+                    if (count > 0 && rows > 0) {
+                        if (p.dw_f32) store_runs<4>(static_cast<uint8_t*>(p.dw) + at * 4, p.ld_dw, rows, count, s.out[warp], lane);
+                        else store_runs<2>(static_cast<uint8_t*>(p.dw) + at * 2, p.ld_dw, rows, count, s.out[warp], lane);
+                    }
+                    __syncwarp();
                 }
             }
-            if (!p.dw_vec && (set == 3 || (p.dw_f32 && set == 1))) {  // a run of 256 bytes per row is together
-                __syncwarp();
-                const int col = col0 + half + (p.dw_f32 ? (set >> 1) * 64 : 0), count = min(run, p.k - col), rows = min(16, p.n - row0 - r);
-                const long long at = static_cast<long long>(row0 + r) * p.ld_dw + col;
-                if (count > 0 && rows > 0) {
-                    if (p.dw_f32) store_runs<4>(static_cast<uint8_t*>(p.dw) + at * 4, p.ld_dw, rows, count, s.out[warp], lane);
-                    else store_runs<2>(static_cast<uint8_t*>(p.dw) + at * 2, p.ld_dw, rows, count, s.out[warp], lane);
-                }
-                __syncwarp();
-            }
-        }
+        };
+        if (infinities) sets(std::true_type());
+        else sets(std::false_type());
     }
 }
 

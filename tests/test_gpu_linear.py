@@ -578,3 +578,38 @@ def test_gelu_slope_of_far_negative_values(m):
     tail, phi = normal(z)
     want = torch.where(z > 0, 1 - tail, tail) + z * phi
     near(db, want, (tail + (z * phi).abs()) * (tail_error(z) + 3 * F) + 2 * F * want.abs() + 2.0**-120, "slope")
+
+
+@pytest.mark.parametrize("name", ["silu", "gelu", "none"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 40])
+def test_gradient_with_infinities_in_the_operands(m, dtype, name):
+    """An infinity in w or x makes the products that it enters infinite with their sign (two of opposite signs, or one times 0, NaN), on both sides of
+    16 rows; the columns beside them are what they are without it."""
+    dev()
+    n, k = 72, 520
+    g = gen(m + 5)
+    x, w, dy, z = (torch.randn(a, b, generator=g).to(dtype) for a, b in ((m, k), (n, k), (m, n), (m, n)))
+    w[5, 7], w[33, 300], w[5, 301], w[6, 301], w[60, 519] = math.inf, -math.inf, math.inf, math.inf, math.nan
+    x[m // 2, 9], x[0, 256], x[m - 1, 511] = -math.inf, math.inf, math.nan
+    xs, ws, ds, zs = x.cuda(), w.cuda(), dy.cuda(), z.cuda()
+    dx, dw = Out(m, k, dtype), Out(n, k, torch.float32)
+    room = torch.empty(ab.linear_grad_workspace_bytes(m, n), dtype=torch.uint8, device="cuda")
+    ab.check(ab.linear_grad(ab.LinearGradDesc(kind=KIND[dtype], m=m, n=n, k=k, act=ACTS[name], trans_w=1, dy_dev=ptr(ds), z_dev=ptr(zs), x_dev=ptr(xs), w_dev=ptr(ws), dx_dev=dx.ptr(),
+                                              dw_dev=dw.ptr(), dw_dtype=ab.F32, workspace_dev=ptr(room), workspace_bytes=room.numel()), stream()))
+    torch.cuda.synchronize()
+    dx.check()
+    dw.check()
+    x, w, dy, z = x.double(), w.double(), dy.double(), z.double()
+    dz = dy * act(z, name)[1]
+    xf, wf = (torch.where(torch.isfinite(t), t, torch.zeros_like(t)).abs() for t in (x, w))  # what the tolerances count
+    err = torch.zeros_like(dz) if name == "none" else dy.abs() * (2.0**-18 + z.abs() * 2.0**-22) + F * dz.abs()
+    half = HALF_STEP[dtype] ** 2 if m <= 16 else HALF_STEP[dtype]
+    err = err + (0 if name == "none" else half * (dz.abs() + err) + 2 * TINY[dtype])
+    want = dz @ w
+    top = 65504.0 if dtype == torch.float16 else math.inf  # F16 outputs saturate
+    finite = torch.where(torch.isfinite(want), want, torch.zeros_like(want)).abs()
+    near(dx.t, want.clamp(-top, top), err @ wf + (n / 16 + 32) * 2 * F * (dz.abs() @ wf) * 1.01 + HALF_STEP[dtype] * finite + TINY[dtype], "dx")
+    want = dz.t() @ x
+    finite = torch.where(torch.isfinite(want), want, torch.zeros_like(want)).abs()
+    near(dw.t, want, err.t() @ xf + (m / 16 + 32) * 2 * F * (dz.abs().t() @ xf) * 1.01 + F * finite + 2.0**-149, "dw")
