@@ -608,7 +608,8 @@ __device__ __forceinline__ void grad_rows_dx(const GradRowsArgs& p, float (*part
 #pragma unroll
             for (int v = 1; v < kGradWarps; ++v) s += at[v * kGradRows * kPartLd];
             at[0] = s;
-            bad |= !(fabsf(s) < __builtin_huge_valf());
+            const int place = i % kGradStrip;
+            bad |= !(fabsf(s) < __builtin_huge_valf()) && col0 + 8 * (place & 7) + (place >> 3) < p.k;
         }
         return bad;
     };
