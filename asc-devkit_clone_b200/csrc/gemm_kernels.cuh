@@ -61,7 +61,7 @@ struct EpiParams {
     long long ld_residual;
     int lin_bias_f32, lin_act;
     int vec_residual;        // rows of the residual are 16-byte aligned at every 32-column boundary
-    int order;               // kFirstOfTwo / kSecondOfTwo: see linear_wait
+    int order;               // kFirstOfTwo / kSecondOfTwo: see wait_at_start
 };
 
 // Builds of the kernels.  The grouped one has the group tables, the per-group tile search and the swapped blocks, the linear one

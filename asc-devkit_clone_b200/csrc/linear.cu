@@ -213,8 +213,9 @@ RowsCut cut_rows(int m, int n, int64_t k_bytes, int sms)
     c.steps = static_cast<int>((k_bytes + kRowsWarps * kRowsUnroll * 64 - 1) / (kRowsWarps * kRowsUnroll * 64));
     return c;
 }
-// Up to 16 tokens the kernel above is the faster one at every size measured (us, bf16, m x n x k: 1 x 4096 x 4096 6.8, 16 x 4096 x 4096 8.8 against
-// 12.4 on the GEMM kernels at 17 rows, 16 x 11008 x 4096 20.2 against 21.4, 16 x 512 x 512 2.4 against 5.8).  Up to 256, while every block has one
+// Up to 16 tokens the kernel above is the faster one at every size measured (us, bf16, m x n x k, weights in L2: 1 x 4096 x 4096 6.7, 16 x 4096 x 4096 8.5 against
+// 12.8 on the GEMM kernels at 17 rows, 16 x 11008 x 4096 19.5 against 21.4, 16 x 512 x 512 2.4 against 5.8; weights from memory: 8.4, 10.8 against 13.7,
+// 21.1 against 24.2 at 32 rows).  Up to 256, while every block has one
 // or two tiles and a short k, it still is: 128 x 512 x 512 2.7 against 5.9, 256 x 256 x 4096 8.0 against 10.3, 32 x 4096 x 1024 5.6 against
 // 9.4, 64 x 2048 x 2048 8.1 against 9.0; but 32 x 4096 x 4096 (two tiles, four steps) 13.8 against 12.5, 64 x 4096 x 256 (four tiles) 8.7 against 5.7.
 bool rows_suit(int m, int n, int64_t k_bytes, int sms)
@@ -303,7 +304,8 @@ int run_linear(const ascb200_linear_desc* desc, cudaStream_t stream)
 
 // ---- gradients --------------------------------------------------------------------------------------------------------------
 // dz = dy * act'(z), rounded to the operands' type for the two products that follow (the rounding that any 16-bit product of it
-// needs); dbias from the fp32 values before that rounding.  A thread owns eight columns and walks down rows; memory bound.
+// needs: beside the rounding of the results it raises their error from 0.0017 to 0.0023 of their size in bf16, 0.00021 to 0.00029 in fp16; with dz as two
+// numbers both products would have twice the work); dbias from the fp32 values before that rounding.  A thread owns eight columns and walks down rows; memory bound.
 struct ActGradArgs {
     const void* dy;
     const void* z;
@@ -432,8 +434,8 @@ int launch_act_grad(const ActGradArgs& p, int act, bool vec, dim3 grid, cudaStre
 // rows packed by one byte permutation.  dw: the columns of an instruction are those that leave a lane with eight neighbours after four.
 //
 // One launch instead of four, of which two are GEMMs of mostly empty tiles (us, bf16 silu with dbias, n x k, 16 rows here against 17 on the GEMMs: 320 x 481
-// 5.5 / 11.1, 1792 x 3864 15.4 / 25.6, 4096 x 4096 25.0 / 30.4, 11008 x 4096 57 / 61, 4096 x 11008 54 / 60; one row of the last two 51, 3.5 TB/s;
-// the second part of dz takes 5 to 10 % of that).  What keeps it from the memory's rate is the latency of a block's loads: dx alone of
+// 5.8 / 11.1, 1792 x 3864 16.9 / 25.6, 4096 x 4096 26.8 / 30.4, 11008 x 4096 58.8 / 60.3, 4096 x 11008 56.5 / 60; one row of 11008 x 4096 52.7, 3.4 TB/s;
+// the second part of dz takes 5 to 10 % of that, keeping infinities from it 3 %).  What keeps it from the memory's rate is the latency of a block's loads: dx alone of
 // 1 x 11008 x 4096 runs at 3.6 TB/s, dw alone at 4.6; 128 registers per thread leave room for two blocks per SM.
 constexpr int kGradRows = 16;
 constexpr int kGradThreads = 256, kGradWarps = 8;

@@ -324,11 +324,12 @@ __device__ __forceinline__ void dequant_store8(DT* out, const float (&v)[8])
     }
 }
 
-// Vector form (n % 8 == 0): eight elements per thread, two vectors per thread in flight; with SHARED (n % 32 == 0, scale
-// constant over 32 aligned columns) one lane in four fetches the scale and shuffles hand it to its neighbours.
-// Vectors of eight elements per thread: int8 sources bring an eighth of a line per vector, so four of them keep as much in flight.
+// Vectors of eight elements that a thread of the vector form has in flight: two of the four-byte sources (64 bytes), four of int8, whose vectors have eight
+// bytes (us, int8 to bf16 with a scale per row, with 2 / 4 / 8 vectors: 16383 x 7168 55.2 / 53.7 / 64.0, 65536 x 512 17.6 / 17.3 / 20.8, 300 x 1024 1.9 / 2.4 / 3.6).
 template <typename SRC>
 constexpr int dequant_vecs_per_thread() { return sizeof(SRC) == 1 ? 4 : 2; }
+// Vector form (n % 8 == 0); with SHARED (n % 32 == 0, scale constant over 32 aligned columns) one lane in four fetches the scale and shuffles hand it
+// to its neighbours.
 template <typename SRC, typename ST, typename DT, bool SHARED>
 __global__ void __launch_bounds__(256) dequant_policy_vec_kernel(const DequantPolicyArgs a)
 {

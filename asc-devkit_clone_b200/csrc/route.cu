@@ -22,7 +22,9 @@ namespace {
 constexpr int kMaxExperts = 1024;     // what ascb200_grouped_gemm takes
 constexpr int kMaxTopK = 32;          // one choice per lane
 constexpr int kRouteWarps = 16;       // tokens at a time per block
-constexpr int kMaxRouteBlocks = 296;  // rows of the workspace
+// Rows of the workspace, whose size a caller asks for without a device: two blocks on each of a B200's 148 SMs (us with 148 / 296 / 592: 32768 x 256 fp32, 8 choices
+// 40 / 27 / 32, 32768 x 64 bf16, 6 choices 27 / 18 / 21, 4096 x 128 bf16, 8 choices 9.1 / 8.6 / 8.6).
+constexpr int kMaxRouteBlocks = 296;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr unsigned kAll = 0xFFFFFFFFu;
 
